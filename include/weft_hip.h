@@ -287,6 +287,7 @@ void q4_k_q8_k_gemv_contract(const uint8_t *W, const uint8_t *X, float *Y, size_
 /* enum ggml_type values (ggml/include/ggml.h:389-431) of this path */
 enum {
   WEFT_GGML_TYPE_F32 = 0,
+  WEFT_GGML_TYPE_F16 = 1, /* activations and cache rows; no MUL_MAT type here */
   WEFT_GGML_TYPE_Q4_0 = 2,
   WEFT_GGML_TYPE_Q4_1 = 3,
   WEFT_GGML_TYPE_Q8_0 = 8,
@@ -297,6 +298,7 @@ enum {
   WEFT_GGML_TYPE_Q8_K = 15,
   WEFT_GGML_TYPE_IQ2_XXS = 16,
   WEFT_GGML_TYPE_IQ2_XS = 17,
+  WEFT_GGML_TYPE_I32 = 26,
   WEFT_GGML_TYPE_MXFP4 = 39,
   WEFT_GGML_TYPE_NVFP4 = 40
 };
@@ -348,6 +350,67 @@ int weft_ggml_mul_mat_id(const weft_ggml_tensor *src0, const weft_ggml_tensor *s
 #define WEFT_GGML_NOALLOC_SCRATCH_BYTES ((size_t)32 << 20)
 int weft_ggml_mul_mat_id_noalloc(const weft_ggml_tensor *src0, const weft_ggml_tensor *src1,
                                  const weft_ggml_tensor *ids, const weft_ggml_tensor *dst);
+
+/* ------------------------------------- a decoder layer between the products */
+/* No counterpart in the reference: the operators that a decoder layer runs
+ * around MUL_MAT, over the same tensor descriptors.  Every call is
+ * stream-ordered, allocates nothing and returns 0 or the error it also
+ * records; tables and lengths are read on the device, so the calls can be
+ * captured into a graph and replayed as they change. */
+
+/* dst = norm(x + residual) * weight with norm(s) = s / sqrt(mean(s^2) + eps),
+ * the mean over a row.  x, residual, sum: F32 (K, rows); weight: F32 (K);
+ * residual, weight and sum may be NULL (zeros, ones, not kept); sum may be x's
+ * or residual's own memory.  dst (K, rows): F32, F16, or Q8_0 / Q8_1 / Q8_K, the
+ * records that MUL_MAT takes as an src1 already quantized (an all-zero Q8_K
+ * record gets zero sums).  K: a multiple of dst's record, else any. */
+int weft_ggml_add_rms_norm(const weft_ggml_tensor *x, const weft_ggml_tensor *residual,
+                           const weft_ggml_tensor *weight, const weft_ggml_tensor *sum,
+                           const weft_ggml_tensor *dst, float eps);
+
+/* A batch of sequences over a paged cache.  Sequence s has new tokens
+ * starts[s] .. starts[s+1] - 1 of the call's token rows (in order; none is
+ * fine), they are its last ones, and it is lengths[s] tokens long with them;
+ * its token at position p is in page pages[s][p / page size].  An entry that is
+ * no page of the pool (-1) makes its positions absent. */
+typedef struct weft_ggml_kv_batch {
+  weft_ggml_tensor pages;   /* I32 (pages a sequence, sequences) */
+  weft_ggml_tensor starts;  /* I32 (sequences + 1) */
+  weft_ggml_tensor lengths; /* I32 (sequences) */
+} weft_ggml_kv_batch;
+
+/* Caches are (D, page size, kv heads, pages) of F16, Q8_0 or Q4_0, D a multiple
+ * of 32, any page size, any 2-byte-aligned strides (heads and slots may be
+ * swapped); keys and values have one type and shape.
+ *
+ * Quantizes rows k, v (D, kv heads, tokens; F32 or F16, any strides) into
+ * their sequences' slots.  Tokens of no sequence, and absent positions, are
+ * skipped; two tokens on one slot leave either. */
+int weft_ggml_kv_write(const weft_ggml_tensor *k, const weft_ggml_tensor *v,
+                       const weft_ggml_kv_batch *batch, const weft_ggml_tensor *k_cache,
+                       const weft_ggml_tensor *v_cache);
+/* Reads positions 0 .. n-1 of every sequence into k, v (D, kv heads, n,
+ * sequences; F32 or F16): the records' values, zeros at absent positions and
+ * past a sequence's length.  starts is not read. */
+int weft_ggml_kv_read(const weft_ggml_tensor *k_cache, const weft_ggml_tensor *v_cache,
+                      const weft_ggml_kv_batch *batch, const weft_ggml_tensor *k,
+                      const weft_ggml_tensor *v);
+
+/* dst = attention of the new tokens' queries q (D, heads, tokens; F32 or F16)
+ * over their sequences' cache, whose new rows are written already: head h reads
+ * kv head h / (heads / kv heads); a query at position p sees the keys j <= p,
+ * with window > 0 those of j > p - window or j < sinks, absent ones left out.
+ * dst (D, heads, tokens): F32 or F16; a query that sees nothing gets zeros,
+ * rows of no sequence stay as they are.  D: 64, 96, 128, 192 or 256.
+ * wdata: weft_ggml_attention_work_size bytes, 16-byte aligned (scratch; its
+ * content need not be kept or cleared). */
+size_t weft_ggml_attention_work_size(const weft_ggml_tensor *q, const weft_ggml_tensor *k_cache,
+                                     const weft_ggml_tensor *v_cache,
+                                     const weft_ggml_kv_batch *batch);
+int weft_ggml_attention(const weft_ggml_tensor *q, const weft_ggml_tensor *k_cache,
+                        const weft_ggml_tensor *v_cache, const weft_ggml_kv_batch *batch,
+                        const weft_ggml_tensor *dst, float scale, int64_t window, int64_t sinks,
+                        void *wdata, size_t wsize);
 
 #ifdef __cplusplus
 }

@@ -102,7 +102,7 @@ def load() -> ctypes.CDLL:
 
 
 def _bind_ggml(lib: ctypes.CDLL) -> None:
-    """Types of the GGML MUL_MAT boundary (weft_ggml_*)."""
+    """Types of the GGML operator boundary (weft_ggml_*)."""
     i32, i64, sz, vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
     for name, args, res in (("weft_ggml_type_size", [i32], sz), ("weft_ggml_blck_size", [i32], i64),
                             ("weft_ggml_row_size", [i32, i64], sz),
@@ -111,7 +111,13 @@ def _bind_ggml(lib: ctypes.CDLL) -> None:
                             ("weft_ggml_mul_mat", [vp, vp, vp, vp, sz], ctypes.c_int),
                             ("weft_ggml_mul_mat_id_work_size", [vp, vp, vp], sz),
                             ("weft_ggml_mul_mat_id", [vp, vp, vp, vp, vp, sz], ctypes.c_int),
-                            ("weft_ggml_mul_mat_id_noalloc", [vp, vp, vp, vp], ctypes.c_int)):
+                            ("weft_ggml_mul_mat_id_noalloc", [vp, vp, vp, vp], ctypes.c_int),
+                            ("weft_ggml_add_rms_norm", [vp, vp, vp, vp, vp, ctypes.c_float], ctypes.c_int),
+                            ("weft_ggml_kv_write", [vp, vp, vp, vp, vp], ctypes.c_int),
+                            ("weft_ggml_kv_read", [vp, vp, vp, vp, vp], ctypes.c_int),
+                            ("weft_ggml_attention_work_size", [vp, vp, vp, vp], sz),
+                            ("weft_ggml_attention",
+                             [vp, vp, vp, vp, vp, ctypes.c_float, i64, i64, vp, sz], ctypes.c_int)):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, res
 

@@ -1,4 +1,6 @@
-"""GGML MUL_MAT / MUL_MAT_ID boundary of libweft_hip from Python.
+"""GGML operator boundary of libweft_hip from Python: MUL_MAT / MUL_MAT_ID and,
+between them in a decoder layer, the residual norm, the paged key / value
+cache and the attention over it.
 
 ``Tensor`` is the part of ``struct ggml_tensor`` (ggml/include/ggml.h:667-692)
 that MUL_MAT reads: type id, ``ne``, byte strides ``nb`` and a device data
@@ -17,6 +19,11 @@ from . import _lib
 # enum ggml_type (ggml/include/ggml.h:389-431), the types of this path
 F32, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K, IQ2_XXS, I32, MXFP4, NVFP4 = 0, 2, 8, 12, 13, 14, 15, 16, 26, 39, 40
 Q4_1, Q8_1, IQ2_XS = 3, 9, 17
+F16 = 1  # activations and cache rows; no MUL_MAT type
+
+
+# bytes of the types that are no records and that MUL_MAT does not know
+_PLAIN = {I32: 4, F16: 2}
 
 
 class Tensor(ctypes.Structure):
@@ -46,8 +53,8 @@ def tensor(t: int, ne: Sequence[int], data: int = 0, nb: Sequence[int] | None = 
     unless ``nb`` is given."""
     ne = list(ne) + [1] * (4 - len(ne))
     if nb is None:
-        size = 4 if t == I32 else type_size(t)
-        nb = [size, size * ne[0] if t == I32 else row_size(t, ne[0])]
+        size = _PLAIN.get(t) or type_size(t)
+        nb = [size, size * ne[0] if t in _PLAIN else row_size(t, ne[0])]
         nb += [nb[1] * ne[1], nb[1] * ne[1] * ne[2]]
     return Tensor(t, (ctypes.c_int64 * 4)(*ne), (ctypes.c_size_t * 4)(*nb), data)
 
@@ -96,3 +103,66 @@ def mul_mat_id_noalloc(src0: Tensor, src1: Tensor, ids: Tensor, dst: Tensor) -> 
         lib.weft_hip_get_last_error()
         raise _lib.HipError(code, "weft_ggml_mul_mat_id_noalloc")
 
+
+class KvBatch(ctypes.Structure):
+    """A batch of sequences over a paged cache (weft_ggml_kv_batch): I32 tensors
+    ``pages`` (pages a sequence, sequences), ``starts`` (sequences + 1, where
+    each sequence's new tokens begin among the call's rows) and ``lengths``
+    (sequences, with the new tokens).  All three are read on the device."""
+    _fields_ = [("pages", Tensor), ("starts", Tensor), ("lengths", Tensor)]
+
+
+def kv_batch(pages: Tensor, starts: Tensor, lengths: Tensor) -> KvBatch:
+    return KvBatch(pages, starts, lengths)
+
+
+def _done(lib: ctypes.CDLL, code: int, where: str) -> None:
+    if code != 0:
+        lib.weft_hip_get_last_error()  # the same error, recorded: clear it
+        raise _lib.HipError(code, where)
+
+
+def _ref(t: ctypes.Structure | None):
+    return None if t is None else ctypes.byref(t)
+
+
+def add_rms_norm(x: Tensor, residual: Tensor | None, weight: Tensor | None, total: Tensor | None, dst: Tensor,
+                 eps: float) -> None:
+    """Enqueue dst = norm(x + residual) * weight, the mean square over a row;
+    ``total`` (which may be x's own memory) keeps the sum.  dst is F32, F16, or the Q8_0 /
+    Q8_1 / Q8_K records that mul_mat takes as a quantized src1."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_add_rms_norm(_ref(x), _ref(residual), _ref(weight), _ref(total), _ref(dst), eps),
+          "weft_ggml_add_rms_norm")
+
+
+def kv_write(k: Tensor, v: Tensor, batch: KvBatch, k_cache: Tensor, v_cache: Tensor) -> None:
+    """Enqueue the quantization of new rows k, v (D, kv heads, tokens) into
+    their sequences' pages; caches are (D, page size, kv heads, pages) of F16,
+    Q8_0 or Q4_0."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_kv_write(_ref(k), _ref(v), _ref(batch), _ref(k_cache), _ref(v_cache)),
+          "weft_ggml_kv_write")
+
+
+def kv_read(k_cache: Tensor, v_cache: Tensor, batch: KvBatch, k: Tensor, v: Tensor) -> None:
+    """Enqueue the read of every sequence's first n positions into k, v
+    (D, kv heads, n, sequences), zeros past its length."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_kv_read(_ref(k_cache), _ref(v_cache), _ref(batch), _ref(k), _ref(v)),
+          "weft_ggml_kv_read")
+
+
+def attention_work_size(q: Tensor, k_cache: Tensor, v_cache: Tensor, batch: KvBatch) -> int:
+    return _lib.load().weft_ggml_attention_work_size(_ref(q), _ref(k_cache), _ref(v_cache), _ref(batch))
+
+
+def attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, batch: KvBatch, dst: Tensor, scale: float,
+              window: int = 0, sinks: int = 0, wdata: int = 0, wsize: int = 0) -> None:
+    """Enqueue dst = causal attention of the new tokens' queries (D, heads,
+    tokens) over their sequences' cache; with a window, a query sees the last
+    ``window`` positions and the first ``sinks``."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_attention(_ref(q), _ref(k_cache), _ref(v_cache), _ref(batch), _ref(dst), scale, window,
+                                       sinks, wdata, wsize),
+          "weft_ggml_attention")
