@@ -5,93 +5,114 @@
 // over the keys j <= p that lie in a page of the pool and, with a window, have
 // j > p - window or j < sinks.  A query that sees no key gets zeros.
 //
-// One wave a (token, head): 64 keys a step, a key a lane for the scores, then a
-// value a lane for the sum, with the running maximum and sum in 32 bits.
+// attend_few reads the cache once for a tile of 16 or 32 query rows; this file
+// checks calls, chooses tiles and splits, and joins the splits.
 #include <algorithm>
 
-#include "kv_cache.h"
+#include "attention.h"
 #include "runtime.h"
 
 namespace weft {
 namespace {
 
-struct AttendArgs {
-  KvSeqs seqs;
-  KvPool k, v;
-  const uint8_t* q;
-  uint8_t* o;
-  long long q_head, q_token, o_head, o_token;  // byte strides
-  int heads, share, d, window, sinks;
-  float scale;
-  bool half_q, half_o;
-};
-
-template <int T>
-__device__ __forceinline__ float value_of(const uint8_t* row, int i) {
-  const uint8_t* rec = row + (i / 32) * KvRecord<T>::kBytes;
-  const int e = i & 31;
-  if constexpr (T == kKvF16) return fp16_to_fp32(ld_u16(rec + 2 * e));
-  const float d = fp16_to_fp32(ld_u16(rec));
-  if constexpr (T == kKvQ8_0) return d * (float)(int8_t)rec[2 + e];
-  return d * (float)((int)(rec[2 + (e & 15)] >> (e & 16 ? 4 : 0) & 15) - 8);
-}
-
-template <int T>
-__global__ void __launch_bounds__(kWave) attend_simple_kernel(AttendArgs a) {
-  __shared__ float qs[256];
-  __shared__ float ps[kWave];
-  __shared__ int pg[kWave], sl[kWave];
-  const int lane = threadIdx.x, t = blockIdx.x, h = blockIdx.y, kvh = h / a.share;
+// The splits of a (token, head) row, each with its maximum, sum and weighted
+// values: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  One workgroup a row;
+// groups of lanes take every so-many-th split, four values a lane.
+constexpr int kJoinThreads = 256, kMaxSplits = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttendArgs a) {
+  constexpr int kLanes = D <= 128 ? 32 : 64;  // of which D / 4 work
+  constexpr int kGroups = kJoinThreads / kLanes;
+  __shared__ float weight[kMaxSplits];
+  __shared__ float wave_top[kJoinThreads / kWave], wave_sums[kJoinThreads / kWave];
+  __shared__ f32x4 sums[kGroups][kLanes];
+  const int t = (int)blockIdx.x, head = (int)blockIdx.y, tid = threadIdx.x;
+  const int kvh = head / a.share;
   const int seq = kv_sequence_of(a.seqs, t);
   if (seq < 0) return;
-  const long long pos = kv_position(a.seqs, seq, t);
-  const uint8_t* qrow = a.q + t * a.q_token + h * a.q_head;
-  for (int i = lane; i < a.d; i += kWave)
-    qs[i] = a.scale * (a.half_q ? fp16_to_fp32(ld_u16(qrow + 2 * i)) : *reinterpret_cast<const float*>(qrow + 4 * i));
-  const int last = (int)min(pos, (long long)INT32_MAX - 64);
-  float m = -INFINITY, l = 0.f, acc[4] = {};
-  // no key lies past the table, whatever a length says
-  const int end = (int)min((long long)last + 1, min((long long)a.seqs.max_pages * a.seqs.page_size, (long long)INT32_MAX - 64));
-  const int first = min(a.window > 0 ? max(0, last - a.window + 1) : 0, end);
-  const int sinks = min(a.sinks, first);
-  for (int base = 0; base < sinks + end - first; base += kWave) {
-    __syncthreads();
-    const int n = base + lane, j = n < sinks ? n : n - sinks + first;
-    int page = -1, slot = 0;
-    const bool there = j < end && kv_place(a.seqs, seq, j, page, slot);
-    float s = -INFINITY;
-    if (there) {
-      const uint8_t* row = a.k.data + page * a.k.page + slot * a.k.slot + kvh * a.k.head;
-      s = 0.f;
-      for (int i = 0; i < a.d; ++i) s += qs[i] * value_of<T>(row, i);
+  int first;
+  seq_tokens(a.seqs, seq, first);
+  const int row = (t - first) * a.share + head - kvh * a.share;
+  TileRows rows;
+  if (!tile_rows(a, seq, row / a.tile, rows)) return;
+  const int each = split_steps(a), n = (rows.range.steps + each - 1) / each;
+  if (n <= 1) return;  // written by its only split
+  const int item = (tiles_before(a, seq) + row / a.tile) * a.kv_heads + kvh;
+  const float* part = a.part + (long long)item * a.splits * a.tile * (D + 2) + (row % a.tile) * (D + 2);
+  const long long stride = (long long)a.tile * (D + 2);
+  float m = -INFINITY, l = 0.f;
+  if (tid < n) m = part[tid * stride + D], l = part[tid * stride + D + 1];
+  const float wt = wave_max(m);
+  if (tid % kWave == 0) wave_top[tid / kWave] = wt;
+  __syncthreads();
+  float top = wave_top[0];
+#pragma unroll
+  for (int i = 1; i < kJoinThreads / kWave; ++i) top = fmaxf(top, wave_top[i]);
+  const float w = top == -INFINITY ? 0.f : exp2_fast(m - top);
+  weight[tid] = w;
+  // a split that saw nothing adds nothing; one that met a NaN passes it on
+  const float ws = wave_sum(tid < n ? w * l : 0.f);
+  if (tid % kWave == 0) wave_sums[tid / kWave] = ws;
+  __syncthreads();
+  float all = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / kWave; ++i) all += wave_sums[i];
+  const int lane = tid % kLanes, group = tid / kLanes;
+  f32x4 x = {};
+  if (4 * lane < D)
+    for (int i = group; i < n; i += kGroups) {
+      const float* p = part + i * stride + 4 * lane;
+      const f32x4 v = {p[0], p[1], p[2], p[3]};
+      x += weight[i] * v;
     }
-    const float m1 = fmaxf(m, wave_max(s));
-    if (m1 == -INFINITY) continue;
-    const float p = __expf(s - m1), f = __expf(m - m1);
-    l = l * f + wave_sum(p);
-    m = m1;
-    ps[lane] = p;
-    pg[lane] = there ? page : -1;
-    sl[lane] = slot;
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) acc[i] *= f;
-    for (int c = 0; c < kWave; ++c) {
-      if (pg[c] < 0) continue;
-      const uint8_t* row = a.v.data + pg[c] * a.v.page + sl[c] * a.v.slot + kvh * a.v.head;
-      for (int i = 0; i < 4; ++i)
-        if (lane + kWave * i < a.d) acc[i] += ps[c] * value_of<T>(row, lane + kWave * i);
-    }
+  sums[group][lane] = x;
+  __syncthreads();
+  if (group != 0 || 4 * lane >= D) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) x += sums[i][lane];
+  x *= all == 0.f ? 0.f : 1.f / all;
+  uint8_t* dst = a.o + (long long)t * a.o_token + (long long)head * a.o_head;
+  if (a.half_o) {
+    const f16x4 h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+    *reinterpret_cast<Bytes8*>(dst + 8 * lane) = __builtin_bit_cast(Bytes8, h);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(dst)[4 * lane + i] = x[i];
   }
-  uint8_t* orow = a.o + t * a.o_token + h * a.o_head;
-  for (int i = 0; i < 4; ++i) {
-    const int e = lane + kWave * i;
-    if (e >= a.d) break;
-    const float y = l == 0.f ? 0.f : acc[i] / l;  // l NaN: a visible key was
-    if (a.half_o)
-      *reinterpret_cast<_Float16*>(orow + 2 * e) = (_Float16)y;
-    else
-      *reinterpret_cast<float*>(orow + 4 * e) = y;
+}
+
+void join(int d, const AttendArgs& a, int heads, hipStream_t st) {
+  const dim3 grid((unsigned)a.seqs.n_tokens, (unsigned)heads);
+  switch (d) {
+    case 64: attend_join_kernel<64><<<grid, kJoinThreads, 0, st>>>(a); break;
+    case 96: attend_join_kernel<96><<<grid, kJoinThreads, 0, st>>>(a); break;
+    case 128: attend_join_kernel<128><<<grid, kJoinThreads, 0, st>>>(a); break;
+    case 192: attend_join_kernel<192><<<grid, kJoinThreads, 0, st>>>(a); break;
+    default: attend_join_kernel<256><<<grid, kJoinThreads, 0, st>>>(a); break;
   }
+  check_launch("attend_join_kernel");
+}
+
+// Tiles and splits of a call, from what the host knows of it.
+struct Plan {
+  int tile, tiles, splits, least;
+  size_t work;
+};
+
+Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
+  Plan p;
+  const int64_t tokens = q->ne[2], share = q->ne[1] / w.heads, seqs = w.seqs.n_seqs;
+  const int64_t rows = tokens * share;
+  p.tile = 16;
+  p.tiles = (int)std::min(tokens * ((share + p.tile - 1) / p.tile), rows / p.tile + std::min(tokens, seqs));
+  p.least = 8;
+  // as many workgroups as run at once, unless there are that many tiles
+  const int64_t items = (int64_t)p.tiles * w.heads, want = 3 * (int64_t)cu_count();
+  const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + kStep - 1) / kStep;
+  p.splits = (int)std::max<int64_t>(
+      1, std::min({(want + items - 1) / items, (steps + p.least - 1) / p.least, (int64_t)kMaxSplits}));
+  p.work = p.splits == 1 ? 0 : (size_t)items * p.splits * p.tile * (w.d + 2) * sizeof(float);
+  return p;
 }
 
 hipError_t fail(hipError_t e) {
@@ -129,9 +150,18 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
     return fail(hipErrorInvalidValue);
   if (q->ne[2] == 0 || w.seqs.n_seqs == 0) return hipSuccess;
   if (q->data == nullptr || dst->data == nullptr) return fail(hipErrorInvalidValue);
+  const Plan p = plan_of(q, w);
+  if (p.work > 0 && (work == nullptr || !aligned(work, 16) || work_size < p.work)) return fail(hipErrorInvalidValue);
+  if (w.seqs.n_pages == 0) w.seqs.max_pages = 0;
   AttendArgs a{};
   a.seqs = w.seqs;
   a.seqs.n_tokens = (int)q->ne[2];
+  a.part = p.splits > 1 ? static_cast<float*>(work) : nullptr;
+  a.tile = p.tile;
+  a.splits = p.splits;
+  a.least = p.least;
+  a.kv_heads = w.heads;
+  a.whole16 = w.seqs.page_size % 16 == 0 && w.k.slot >= 0 && w.k.slot < 1 << 26 && w.v.slot >= 0 && w.v.slot < 1 << 26;
   a.k = w.k;
   a.v = w.v;
   a.q = static_cast<const uint8_t*>(q->data);
@@ -140,33 +170,36 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.q_token = (long long)q->nb[2];
   a.o_head = (long long)dst->nb[1];
   a.o_token = (long long)dst->nb[2];
-  a.heads = (int)q->ne[1];
-  a.share = a.heads / w.heads;
-  a.d = w.d;
+  a.share = (int)(q->ne[1] / w.heads);
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
   a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX);
-  a.scale = scale;
+  a.scale = scale * 1.44269504f;  // weights are powers of two
   a.half_q = q->type == WEFT_GGML_TYPE_F16;
   a.half_o = dst->type == WEFT_GGML_TYPE_F16;
-  const dim3 grid((unsigned)a.seqs.n_tokens, (unsigned)a.heads);
   const hipStream_t st = current_stream();
-  switch (w.type) {
-    case kKvF16: attend_simple_kernel<kKvF16><<<grid, kWave, 0, st>>>(a); break;
-    case kKvQ8_0: attend_simple_kernel<kKvQ8_0><<<grid, kWave, 0, st>>>(a); break;
-    default: attend_simple_kernel<kKvQ4_0><<<grid, kWave, 0, st>>>(a); break;
-  }
-  check_launch("attend_simple_kernel");
+  attend_few(w.type, w.d, a, p.tiles * w.heads, st);
+  if (p.splits > 1) join(w.d, a, (int)q->ne[1], st);
   return pending_error();
 }
 
 }  // namespace
 }  // namespace weft
 
+static __attribute__((aligned(16))) char w_stand_in[16];
+
 extern "C" {
 
 size_t weft_ggml_attention_work_size(const weft_ggml_tensor* q, const weft_ggml_tensor* k_cache,
                                      const weft_ggml_tensor* v_cache, const weft_ggml_kv_batch* batch) {
-  return 0;
+  if (q == nullptr || k_cache == nullptr || v_cache == nullptr || batch == nullptr) return 0;
+  // the shapes alone count: buffers may be allocated later
+  weft_ggml_tensor k = *k_cache, v = *v_cache;
+  weft_ggml_kv_batch b = *batch;
+  for (weft_ggml_tensor* t : {&k, &v, &b.pages, &b.starts, &b.lengths})
+    if (t->data == nullptr) t->data = w_stand_in;
+  weft::KvView w;
+  if (weft::kv_view(&k, &v, &b, &w) != hipSuccess || weft::shapes(q, w) != hipSuccess) return 0;
+  return q->ne[2] == 0 || w.seqs.n_seqs == 0 ? 0 : weft::plan_of(q, w).work;
 }
 
 int weft_ggml_attention(const weft_ggml_tensor* q, const weft_ggml_tensor* k_cache, const weft_ggml_tensor* v_cache,
