@@ -8,8 +8,10 @@
 // code j in the low and code j + 16 in the high half of byte j.
 //
 // Both directions are one pass bound by memory: a workgroup's threads take
-// consecutive groups of four (write) or sixteen (read) values, keys and values
+// consecutive groups of four (write) or eight (read) values, keys and values
 // in one launch.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "kv_cache.h"
@@ -101,94 +103,139 @@ __device__ __forceinline__ void store_record(uint8_t* row, int block, int part, 
   }
 }
 
-// blockIdx.x: token, blockIdx.y: keys or values.  A token's row is heads x d
-// values; each 8 lanes own a record.
+// `waves` waves a token, blockIdx.y: keys or values.  A token's row is heads x d
+// values, each 8 lanes own a record of it, and a lane has up to four groups of
+// four values in flight; the first are on their way while the row's place is
+// looked up (starts, length, page: three dependent loads, most of a small call).
 template <int T, bool kHalfSrc>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvSeqs seqs, KvPool k, KvPool v, Rows kx, Rows vx, int d,
-                                                            int heads) {
-  const int t = (int)blockIdx.x;
+                                                            int heads, int waves) {
+  constexpr int U = 4;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int t = (int)blockIdx.x * (kThreads / kWave / waves) + wave / waves;
+  const int stride = waves * kWave, first = wave % waves * kWave;
+  if (t >= seqs.n_tokens) return;
   const KvPool pool = blockIdx.y ? v : k;
   const Rows rows = blockIdx.y ? vx : kx;
+  const uint8_t* src = rows.data + t * rows.token;
+  const int per_head = d / 4, total = heads * per_head;
+  float4 x[U];
+  int h[U], c[U];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * stride >= total) break;
+      const int i = min(i0 + u * stride + lane, total - 1);  // past the row: its last values, not stored
+      h[u] = i / per_head;
+      c[u] = i - h[u] * per_head;
+      x[u] = load4<kHalfSrc>(src + h[u] * rows.head + (long long)c[u] * (kHalfSrc ? 8 : 16));
+    }
+  };
+  load(first);
   const int seq = kv_sequence_of(seqs, t);
   if (seq < 0) return;
   const long long pos = kv_position(seqs, seq, t);
   int page, slot;
   if (pos < 0 || pos > INT32_MAX || !kv_place(seqs, seq, (int)pos, page, slot)) return;
   uint8_t* at = pool.data + page * pool.page + slot * pool.slot;
-  const uint8_t* src = rows.data + t * rows.token;
-  const int per_head = d / 4, total = heads * per_head;
-  // whole waves stay in the loop: a record's lanes exchange values
-  for (int i0 = 0; i0 < total; i0 += kThreads) {
-    const int i = i0 + (int)threadIdx.x;
-    const bool live = i < total;
-    const int h = live ? i / per_head : 0, c = live ? i - h * per_head : 0;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live) x = load4<kHalfSrc>(src + h * rows.head + (long long)c * (kHalfSrc ? 8 : 16));
-    store_record<T>(at + h * pool.head, c / 8, c & 7, x, live);
+  for (int i0 = first; i0 < total; i0 += U * stride) {
+    if (i0 > first) load(i0);
+    // whole waves: a record's lanes exchange values
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * stride < total)
+        store_record<T>(at + h[u] * pool.head, c[u] / 8, c[u] & 7, x[u], i0 + u * stride + lane < total);
   }
 }
 
-// sixteen values of half a record
+// Eight values (the part-th of a record's four groups) in 16 bits, bit for bit
+// the 32-bit value rounded once, or in 32.
 template <int T>
-__device__ __forceinline__ void read16(const uint8_t* rec, int part, float (&x)[16]) {
+__device__ __forceinline__ Bytes16 load8(const uint8_t* rec, int part, uint32_t& step) {
+  Bytes16 b{};
+  if constexpr (T == kKvF16) {
+    b = *reinterpret_cast<const Bytes16*>(rec + 16 * part);
+  } else {
+    step = ld_u16(rec);
+    // Q4_0: parts 0 and 1 are the low, 2 and 3 the high halves of the bytes
+    const Bytes8 w = *reinterpret_cast<const Bytes8*>(rec + 2 + 8 * (T == kKvQ8_0 ? part : part & 1));
+    b.w[0] = w.w[0];
+    b.w[1] = w.w[1];
+  }
+  return b;
+}
+template <int T>
+__device__ __forceinline__ void values8(const Bytes16& b, int part, uint32_t step, float (&x)[8]) {
   if constexpr (T == kKvF16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const half4 h = __builtin_bit_cast(half4, *reinterpret_cast<const Bytes8*>(rec + 32 * part + 8 * j));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * j + i] = (float)h[i];
-    }
-  } else if constexpr (T == kKvQ8_0) {
-    const float d = fp16_to_fp32(ld_u16(rec));
-    const Bytes16 b = *reinterpret_cast<const Bytes16*>(rec + 2 + 16 * part);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = d * (float)(int8_t)(b.w[i / 4] >> (8 * (i & 3)));
+    for (int i = 0; i < 8; ++i) x[i] = fp16_to_fp32(b.w[i / 2] >> (16 * (i & 1)) & 0xffffu);
   } else {
-    const float d = fp16_to_fp32(ld_u16(rec));
-    const Bytes16 b = *reinterpret_cast<const Bytes16*>(rec + 2);
+    const float d = fp16_to_fp32(step);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = d * (float)((int)(b.w[i / 4] >> (8 * (i & 3) + 4 * part) & 15u) - 8);
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t w = b.w[i / 4] >> (8 * (i & 3));
+      x[i] = d * (float)(T == kKvQ8_0 ? (int)(int8_t)w : (int)(w >> (part & 2 ? 4 : 0) & 15u) - 8);
+    }
   }
 }
 
-// blockIdx.x: 16 positions, blockIdx.y: sequence, blockIdx.z: keys or values;
-// zeros where the sequence has no value.
-constexpr int kReadTokens = 16;
+// blockIdx.x: kReadTokens positions, blockIdx.y: sequence, blockIdx.z: keys or
+// values; zeros where the sequence has no value.  The positions' rows are looked
+// up once; then a thread has four groups of eight values in flight, and a wave
+// writes 1 KiB of F16 in one store.
+constexpr int kReadTokens = 8;
 template <int T, bool kHalfOut>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvSeqs seqs, KvPool k, KvPool v, Rows ko, Rows vo,
                                                            long long k_seq, long long v_seq, int d, int heads,
                                                            int n_pos) {
+  __shared__ long long place[kReadTokens];
   const int seq = (int)blockIdx.y;
   const KvPool pool = blockIdx.z ? v : k;
   const Rows out = blockIdx.z ? vo : ko;
-  uint8_t* dst = out.data + seq * (blockIdx.z ? v_seq : k_seq);
-  const int length = seqs.lengths[seq];
   const int p0 = (int)blockIdx.x * kReadTokens;
   const int n = min(kReadTokens, n_pos - p0);
-  const int per_head = d / 16, per_token = heads * per_head, total = n * per_token;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int j = i / per_token, r = i - j * per_token, h = r / per_head, c = r - h * per_head;
-    const int pos = p0 + j;
-    float x[16];
+  if ((int)threadIdx.x < n) {
+    const int pos = p0 + (int)threadIdx.x;
     int page, slot;
-    if (pos < length && kv_place(seqs, seq, pos, page, slot)) {
-      read16<T>(pool.data + page * pool.page + slot * pool.slot + h * pool.head + (c / 2) * KvRecord<T>::kBytes, c & 1,
-                x);
-    } else {
+    place[threadIdx.x] = pos < seqs.lengths[seq] && kv_place(seqs, seq, pos, page, slot)
+                             ? page * pool.page + slot * pool.slot
+                             : LLONG_MIN;
+  }
+  __syncthreads();
+  uint8_t* dst = out.data + seq * (blockIdx.z ? v_seq : k_seq) + p0 * out.token;
+  const int per_head = d / 8, per_token = heads * per_head, total = n * per_token;
+  constexpr int U = 4;
+  for (int i0 = threadIdx.x; i0 < total; i0 += U * kThreads) {
+    Bytes16 b[U];
+    uint32_t step[U];
+    uint8_t* to[U];
+    int part[U];
+    bool there[U];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = 0.f;
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads;
+      const int j = i / per_token, r = i - j * per_token, h = r / per_head, c = r - h * per_head;
+      to[u] = i < total ? dst + j * out.token + h * out.head + (long long)c * (kHalfOut ? 16 : 32) : nullptr;
+      const long long at = i < total ? place[j] : LLONG_MIN;
+      there[u] = at != LLONG_MIN;
+      part[u] = c & 3;
+      if (there[u])
+        b[u] = load8<T>(pool.data + at + h * pool.head + (c / 4) * KvRecord<T>::kBytes, c & 3, step[u]);
     }
-    uint8_t* y = dst + pos * out.token + h * out.head + (long long)c * (kHalfOut ? 32 : 64);
-    if constexpr (kHalfOut) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const half4 v4 = {(_Float16)x[4 * e], (_Float16)x[4 * e + 1], (_Float16)x[4 * e + 2], (_Float16)x[4 * e + 3]};
-        reinterpret_cast<Bytes8*>(y)[e] = __builtin_bit_cast(Bytes8, v4);
+    for (int u = 0; u < U; ++u) {
+      if (to[u] == nullptr) continue;
+      float x[8] = {};
+      if (there[u]) values8<T>(b[u], part[u], step[u], x);
+      if constexpr (kHalfOut) {
+        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+        const half8 y = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
+                         (_Float16)x[4], (_Float16)x[5], (_Float16)x[6], (_Float16)x[7]};
+        *reinterpret_cast<Bytes16*>(to[u]) = __builtin_bit_cast(Bytes16, y);
+      } else {
+        *reinterpret_cast<Floats4*>(to[u]) = Floats4{{x[0], x[1], x[2], x[3]}};
+        *reinterpret_cast<Floats4*>(to[u] + 16) = Floats4{{x[4], x[5], x[6], x[7]}};
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        reinterpret_cast<Floats4*>(y)[e] = Floats4{{x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]}};
     }
   }
 }
@@ -230,12 +277,16 @@ hipError_t kv_write(const weft_ggml_tensor* kx, const weft_ggml_tensor* vx, cons
   w.seqs.n_tokens = (int)kx->ne[2];
   const Rows kr{static_cast<uint8_t*>(kx->data), (long long)kx->nb[1], (long long)kx->nb[2]};
   const Rows vr{static_cast<uint8_t*>(vx->data), (long long)vx->nb[1], (long long)vx->nb[2]};
-  const dim3 grid((unsigned)w.seqs.n_tokens, 2);
+  // few tokens: a workgroup each, one group a lane (8 x 128 values, one token:
+  // 2.8 us against 4.6); more than are resident at once: a wave each (6,500 tokens of
+  // Q4_0: 16.9 us against 19.4)
+  const int waves = 2 * w.seqs.n_tokens <= 8 * cu_count() ? 4 : 1;
+  const dim3 grid((unsigned)((w.seqs.n_tokens + 4 / waves - 1) / (4 / waves)), 2);
   const bool half = kx->type == WEFT_GGML_TYPE_F16;
   const hipStream_t st = current_stream();
 #define WEFT_KV_WRITE(T)                                                                                         \
-  (half ? kv_write_kernel<T, true><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads)            \
-        : kv_write_kernel<T, false><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads))
+  (half ? kv_write_kernel<T, true><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads, waves)     \
+        : kv_write_kernel<T, false><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads, waves))
   switch (w.type) {
     case kKvF16: WEFT_KV_WRITE(kKvF16); break;
     case kKvQ8_0: WEFT_KV_WRITE(kKvQ8_0); break;
