@@ -3,16 +3,14 @@
 //
 // The queries of one kv head of a sequence are rows r = token * share + head:
 // they read the same keys and values, so a tile of rows may hold several heads
-// of one token, several tokens, or both.  Keys go in steps of 32 at positions
-// that are multiples of 32: first those that hold visible sinks, then those of
-// the rows' windows.
+// of one token, several tokens, or both.  Keys go in steps of 32 or 64 at
+// positions that are multiples of that: first those that hold visible sinks, then
+// those of the rows' windows.
 #pragma once
 
 #include "kv_cache.h"
 
 namespace weft {
-
-constexpr int kStep = 32;  // keys a step
 
 struct AttendArgs {
   KvSeqs seqs;
@@ -23,11 +21,13 @@ struct AttendArgs {
   long long q_head, q_token, o_head, o_token;  // byte strides
   int share, kv_heads, window, sinks;
   int tile;        // rows a tile
+  int step;        // keys a step, 32 or 64
   int splits;      // the most splits of a tile's steps
   int least;       // the fewest steps a split is made for
   float scale;     // times log2 e
   bool half_q, half_o;
   bool whole16;    // pages hold whole groups of 16 slots, strides below 2^26
+  bool whole32;    // of 32
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -48,7 +48,7 @@ __device__ __forceinline__ int seq_tokens(const KvSeqs& s, int seq, int& first) 
 }
 
 struct Range {
-  int sink_steps;   // steps at positions 0, 32, ..
+  int sink_steps;   // steps at positions 0, step, ..
   int begin;        // position of the first step after them
   int steps;        // all steps
   int end;          // no visible key at or past it
@@ -58,16 +58,29 @@ struct Range {
 __device__ __forceinline__ Range visible_range(const AttendArgs& a, long long p0, long long p1) {
   Range r;
   const long long table = (long long)a.seqs.max_pages * a.seqs.page_size;
-  r.end = (int)max(0ll, min(min(p1 + 1, table), (long long)INT32_MAX - 64));
+  r.end = (int)max(0ll, min(min(p1 + 1, table), (long long)INT32_MAX - 128));
   const long long first = a.window > 0 ? max(0ll, p0 - a.window + 1) : 0;
-  r.begin = (int)min(first, (long long)r.end) & ~(kStep - 1);
-  r.sink_steps = (min(a.sinks, r.begin) + kStep - 1) / kStep;
-  r.steps = r.sink_steps + (r.end - r.begin + kStep - 1) / kStep;
+  r.begin = (int)min(first, (long long)r.end) & -a.step;
+  r.sink_steps = (min(a.sinks, r.begin) + a.step - 1) / a.step;
+  r.steps = r.sink_steps + (r.end - r.begin + a.step - 1) / a.step;
   return r;
 }
 
+template <int kStep>
 __device__ __forceinline__ int step_position(const Range& r, int step) {
   return step < r.sink_steps ? step * kStep : r.begin + (step - r.sink_steps) * kStep;
+}
+
+// The keys of a step at `pos` that a query at `qpos` sees, key i as bit i;
+// `present`: the keys that are there.
+__device__ __forceinline__ unsigned long long first_bits(int n) {
+  return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+__device__ __forceinline__ unsigned long long seen_bits(const AttendArgs& a, unsigned long long present, int pos,
+                                                        int qpos) {
+  present &= first_bits(qpos - pos + 1);
+  if (a.window > 0) present &= ~first_bits(qpos - a.window - pos + 1) | first_bits(a.sinks - pos);
+  return present;
 }
 
 // Steps a split takes, the same for every tile of the call, so that a batch of
@@ -164,7 +177,12 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// exp2 of an argument <= 0 (results below 2^-126 are zero)
+// A row's maximum moves only when a score is more than 2^kLag times its weight's
+// scale: weights up to 2^kLag keep their 11 bits in 16, and the sums are not
+// rescaled at nearly every step.
+constexpr float kLag = 8.f;
+
+// exp2 of an argument <= kLag (results below 2^-126 are zero)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Four code bytes as 16-bit integers, exactly: byte u as 0x6400 | u is 1024 + u.
@@ -189,7 +207,11 @@ __device__ __forceinline__ float value_of(const uint8_t* row, int i) {
 
 __device__ __forceinline__ bool half_not_finite(uint32_t h) { return (h & 0x7c00u) == 0x7c00u; }
 
-// launches of the kernels by cache type (attention_few.hip)
-void attend_few(int type, int d, const AttendArgs& a, int items, hipStream_t st);
+// the many-row kernel's keys a step
+__host__ __device__ constexpr int many_step(int d) { return d > 192 ? 32 : 64; }
+
+// launches of the kernels
+void attend_few(int type, int d, const AttendArgs& a, int items, hipStream_t st);   // tile 16, step 32
+void attend_many(int type, int d, const AttendArgs& a, int items, hipStream_t st);  // tile 128, step many_step
 
 }  // namespace weft

@@ -5,8 +5,8 @@
 // over the keys j <= p that lie in a page of the pool and, with a window, have
 // j > p - window or j < sinks.  A query that sees no key gets zeros.
 //
-// attend_few reads the cache once for a tile of 16 or 32 query rows; this file
-// checks calls, chooses tiles and splits, and joins the splits.
+// attention_few.hip has tiles of 16 query rows, attention_many.hip of 128; this
+// file checks calls, chooses tiles and splits, and joins the splits.
 #include <algorithm>
 
 #include "attention.h"
@@ -95,7 +95,8 @@ void join(int d, const AttendArgs& a, int heads, hipStream_t st) {
 
 // Tiles and splits of a call, from what the host knows of it.
 struct Plan {
-  int tile, tiles, splits, least;
+  bool many;
+  int tile, step, tiles, splits, least;
   size_t work;
 };
 
@@ -103,12 +104,16 @@ Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
   Plan p;
   const int64_t tokens = q->ne[2], share = q->ne[1] / w.heads, seqs = w.seqs.n_seqs;
   const int64_t rows = tokens * share;
-  p.tile = 16;
+  // 32 rows a sequence on average: below, a tile of 16 rows reads the cache at its
+  // full rate; above, 128 rows share a step's conversion
+  p.many = rows > 32 * seqs;
+  p.tile = p.many ? 128 : 16;
+  p.step = p.many ? many_step(w.d) : 32;
   p.tiles = (int)std::min(tokens * ((share + p.tile - 1) / p.tile), rows / p.tile + std::min(tokens, seqs));
-  p.least = 8;
+  p.least = p.many ? 4 : 8;
   // as many workgroups as run at once, unless there are that many tiles
-  const int64_t items = (int64_t)p.tiles * w.heads, want = 3 * (int64_t)cu_count();
-  const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + kStep - 1) / kStep;
+  const int64_t items = (int64_t)p.tiles * w.heads, want = (p.many ? 2 : 3) * (int64_t)cu_count();
+  const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + p.step - 1) / p.step;
   p.splits = (int)std::max<int64_t>(
       1, std::min({(want + items - 1) / items, (steps + p.least - 1) / p.least, (int64_t)kMaxSplits}));
   p.work = p.splits == 1 ? 0 : (size_t)items * p.splits * p.tile * (w.d + 2) * sizeof(float);
@@ -158,10 +163,13 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.seqs.n_tokens = (int)q->ne[2];
   a.part = p.splits > 1 ? static_cast<float*>(work) : nullptr;
   a.tile = p.tile;
+  a.step = p.step;
   a.splits = p.splits;
   a.least = p.least;
   a.kv_heads = w.heads;
-  a.whole16 = w.seqs.page_size % 16 == 0 && w.k.slot >= 0 && w.k.slot < 1 << 26 && w.v.slot >= 0 && w.v.slot < 1 << 26;
+  const bool near = w.k.slot >= 0 && w.k.slot < 1 << 26 && w.v.slot >= 0 && w.v.slot < 1 << 26;
+  a.whole16 = near && w.seqs.page_size % 16 == 0;
+  a.whole32 = near && w.seqs.page_size % 32 == 0;
   a.k = w.k;
   a.v = w.v;
   a.q = static_cast<const uint8_t*>(q->data);
@@ -177,7 +185,7 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.half_q = q->type == WEFT_GGML_TYPE_F16;
   a.half_o = dst->type == WEFT_GGML_TYPE_F16;
   const hipStream_t st = current_stream();
-  attend_few(w.type, w.d, a, p.tiles * w.heads, st);
+  (p.many ? attend_many : attend_few)(w.type, w.d, a, p.tiles * w.heads, st);
   if (p.splits > 1) join(w.d, a, (int)q->ne[1], st);
   return pending_error();
 }

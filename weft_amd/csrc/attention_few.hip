@@ -1,8 +1,8 @@
 // Attention of few query rows a kv head: decode steps and short chunks.
 //
 // Bound by reading the cache.  Each of a workgroup's four waves takes every
-// fourth step of 32 keys of its split, alone, for all rows of the tile (16 or
-// 32), and the waves' results are joined in LDS at the end; splits are joined
+// fourth step of 32 keys of its split, alone, for the 16 rows of the tile,
+// and the waves' results are joined in LDS at the end; splits are joined
 // by a second kernel (attention.hip).
 //
 // The scores are formed transposed, S^T = K Q^T, with 16x16x32 products: keys
@@ -30,7 +30,7 @@
 namespace weft {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 4, kStep = 32;
 
 template <int T, int NB>
 struct Raw {  // a step's records: K as operands, V as rows
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
   auto pages_of = [&](int step) {
     int page = -1, slot;
     if (step < step1) {
-      const int pos = step_position(t.range, step) + (lane & 31);
+      const int pos = step_position<kStep>(t.range, step) + (lane & 31);
       const bool seen = pos < t.range.end && (a.window == 0 || pos > first_pos - a.window || pos < a.sinks);
       if (!kv_place(a.seqs, seq, pos, page, slot) || !seen) page = -1;
     }
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
   };
   // addresses: key's row in a pool, absent keys at the pool's first row
   auto load = [&](int step, int page, R& r) {
-    const int pos = step_position(t.range, step);
+    const int pos = step_position<kStep>(t.range, step);
     const long long kh = (long long)kvh * a.k.head, vh = (long long)kvh * a.v.head;
     if (a.whole16) {
       const uint8_t *kb[2], *vb[2];
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
   int page = pages_of(step), next_page = pages_of(step + kWaves);
   if (step < step1) load(step, page, raw);
   for (; step < step1; step += kWaves) {
-    const int pos = step_position(t.range, step);
+    const int pos = step_position<kStep>(t.range, step);
     const uint32_t present = (uint32_t)__ballot(page >= 0);  // key i: bit i
     // rows see different keys of this step
     const bool mixed = pos + kStep - 1 > first_pos ||
@@ -344,18 +344,14 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
         if constexpr (T == kKvF16) x[e] *= a.scale;
       }
       if (masked) {
+        // value e: key 16 (e / 4) + 4 g + e % 4
+        const uint32_t seen = (uint32_t)seen_bits(a, present, pos, qpos[rt]) >> (4 * g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = 16 * (e / 4) + 4 * g + e % 4;
-          const int at = pos + key;
-          const bool seen = (present >> key & 1u) && at <= qpos[rt] &&
-                            (a.window == 0 || at > qpos[rt] - a.window || at < a.sinks);
-          x[e] = seen ? x[e] : -INFINITY;
-        }
+        for (int e = 0; e < 8; ++e) x[e] = seen & 1u << (16 * (e / 4) + e % 4) ? x[e] : -INFINITY;
       }
       float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
       top = quarters_max(top);
-      if (__ballot(top > m[rt])) {
+      if (__ballot(top > m[rt] + kLag)) {
         const float now = fmaxf(m[rt], top);
         const float f = now == -INFINITY ? 1.f : exp2_fast(m[rt] - now);
         m[rt] = now;
@@ -408,12 +404,14 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
           p = e == at ? w : p;
         }
         p = __shfl(p, 16 * (key % 16 / 4) + c, kWave);
-        const int kp = pos + key;
-        if (kp <= qpos[rt] && (a.window == 0 || kp > qpos[rt] - a.window || kp < a.sinks)) {
+        if (seen_bits(a, 1ull, pos + key, qpos[rt])) {
 #pragma unroll
           for (int v = 0; v < 2 * NB; ++v)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[rt][v][e] += p * value_of<T>(row, 16 * v + 4 * g + e);
+            for (int e = 0; e < 4; ++e) {
+              o[rt][v][e] += p * value_of<T>(row, 16 * v + 4 * g + e);
+              asm volatile("" ::: "memory");  // one value at a time: no registers for this path
+            }
         }
       }
     }

@@ -1,0 +1,447 @@
+// Attention of many query rows a kv head: prompts and chunks.
+//
+// Bound by the matrix pipe and the softmax beside it.  A workgroup owns 128 rows,
+// 32 a wave, and walks the keys in steps of 64 (heads of 256: 32, for the
+// registers' sake) that all waves share: the records
+// are loaded into registers a step ahead, converted to 16-bit values once for the
+// 128 rows, and written to one of two LDS buffers, one barrier a step.  Two
+// workgroups fit a CU, so one's products run beside the other's softmax.
+//
+// As for few rows the scores are formed transposed (S^T = K Q^T, here with
+// 32x32x16 products): a lane holds 32 keys of one query, the maximum needs one
+// lane exchange, the accumulators' scale is one number a lane, and the weights
+// are the right operand of O^T = V^T P^T without leaving their registers, V^T
+// read by the transposing LDS read in the weights' key order.
+//
+// Numbers: queries, values of quantized keys and values, and weights are each
+// rounded once to 16 bits (a second part of each would cost the matrix pipe as
+// much again); products, maximum, sum and accumulators are in 32 bits.
+#include "attention.h"
+#include "runtime.h"
+
+namespace weft {
+namespace {
+
+constexpr int kWaves = 4, kThreads = kWaves * kWave, kRows = 32;  // rows a wave
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int T, int NB>
+struct Tile {
+  static constexpr int kStep = many_step(32 * NB);
+  static constexpr int kUnit = T == kKvF16 ? 4 * NB : T == kKvQ8_0 ? 2 * NB : NB;  // 16-byte units a row
+  static constexpr int kUnits = (kUnit * kStep + kThreads - 1) / kThreads;          // a thread
+  static constexpr bool kEven = kUnit * kStep % kThreads == 0;
+  // rows in LDS: K's on different banks for 16 lanes' 16 bytes, V's for eight rows' 32
+  static constexpr int kKRow = 64 * NB + 16, kVRow = 64 * NB + 32;
+  static constexpr int kV = kStep * kKRow, kBytes = kV + kStep * kVRow;
+};
+
+template <int T, int NB>
+__global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(AttendArgs a) {
+  using L = Tile<T, NB>;
+  constexpr int D = 32 * NB, kStep = L::kStep, kPart = kStep / 32;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two steps' tiles
+  __shared__ unsigned long long spoiled_of[2][kWaves];
+
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, tid = threadIdx.x;
+  const int c = lane & 31, h = lane >> 5;  // query column (or key, value) and half
+  const int kvh = (int)blockIdx.x % a.kv_heads;
+  const int split = (int)blockIdx.y;
+  int tile;
+  // a causal call's last tiles are its longest: they start first
+  const int seq = find_tile(a, (int)(gridDim.x / a.kv_heads) - 1 - (int)blockIdx.x / a.kv_heads, tile);
+  TileRows t;
+  if (seq < 0 || !tile_rows(a, seq, tile, t)) return;
+  int step0 = 0, step1 = t.range.steps;
+  bool whole = true;
+  if (a.part != nullptr) {
+    const int n = split_steps(a);
+    whole = n >= step1;
+    step0 = min(split * n, step1);
+    step1 = min(step0 + n, step1);
+    if (split > 0 && step0 >= step1) return;
+  }
+
+  // this wave's queries, as right operands: lane c's row, values 16 b + 8 h + j
+  f16x8 qf[2 * NB];
+  const int wrow0 = t.row0 + min(kRows * wave, t.rows - 1), wrow1 = t.row0 + min(kRows * wave + kRows, t.rows) - 1;
+  const bool idle = kRows * wave >= t.rows;  // no row of this wave
+  const int row = t.row0 + min(kRows * wave + c, t.rows - 1);
+  const int tok = row / a.share, head = kvh * a.share + row % a.share;
+  const int qpos = (int)max(-1ll, t.pos0 + tok);
+  const int first_pos = (int)max(-1ll, t.pos0 + wrow0 / a.share), last_pos = (int)max(-1ll, t.pos0 + wrow1 / a.share);
+  // of the whole tile
+  const int first_all = (int)max(-1ll, t.pos0 + t.row0 / a.share);
+  const int last_all = (int)max(-1ll, t.pos0 + (t.row0 + t.rows - 1) / a.share);
+  {
+    const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
+    if (a.half_q) {
+#pragma unroll
+      for (int b = 0; b < 2 * NB; ++b)
+        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h));
+    } else {
+#pragma unroll
+      for (int b = 0; b < 2 * NB; ++b) {
+        const float* x = reinterpret_cast<const float*>(src) + 16 * b + 8 * h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)x[j];
+      }
+    }
+  }
+
+  f32x16 o[NB] = {};
+  float m = -INFINITY, l = 0.f;
+
+  // page of a step's key `lane` (of 32: keys twice), -1 where it is absent or no row of the tile sees it
+  auto pages_of = [&](int step) {
+    int page = -1, slot;
+    if (step < step1) {
+      const int pos = step_position<kStep>(t.range, step) + (lane & (kStep - 1));
+      const bool seen = pos < t.range.end && (a.window == 0 || pos > first_all - a.window || pos < a.sinks);
+      if (!kv_place(a.seqs, seq, pos, page, slot) || !seen) page = -1;
+    }
+    return page;
+  };
+  Bytes16 rk[L::kUnits], rv[L::kUnits];
+  uint32_t sk[L::kUnits], sv[L::kUnits];
+  auto slot_of = [&](int at) {
+    return a.seqs.page_shift >= 0 ? at & (a.seqs.page_size - 1) : (int)((uint32_t)at % (uint32_t)a.seqs.page_size);
+  };
+  // a unit of a row: 16 bytes of values or codes, and their step
+  auto fetch = [&](const uint8_t* r, int e, Bytes16& b, uint32_t& s) {
+    if constexpr (T == kKvF16) {
+      b = *reinterpret_cast<const Bytes16*>(r + 16 * e);
+    } else if constexpr (T == kKvQ8_0) {
+      b = *reinterpret_cast<const Bytes16*>(r + 34 * (e / 2) + 2 + 16 * (e & 1));
+      s = ld_u16(r + 34 * (e / 2));
+    } else {
+      b = *reinterpret_cast<const Bytes16*>(r + 18 * e + 2);
+      s = ld_u16(r + 18 * e);
+    }
+  };
+  // the thread's number behind a barrier to the optimizer, which would keep every
+  // unit's address and mask in registers across the loop
+  auto opaque_tid = [&] {
+    int x = tid;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  auto load = [&](int step, int page) {
+    const int tid = opaque_tid();
+    const int pos = step_position<kStep>(t.range, step);
+    const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
+    const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
+    if (a.whole32) {
+      const unsigned long long there = __ballot(page >= 0);
+      const uint8_t *kb[2], *vb[2];
+#pragma unroll
+      for (int i = 0; i < kPart; ++i) {
+        // 32 keys lie in one page: that of any key that is there
+        const uint32_t some = (uint32_t)(there >> (32 * i));
+        const int p = some ? __builtin_amdgcn_readlane(page, 32 * i + __builtin_ctz(some)) : 0;
+        const int slot = slot_of(pos + 32 * i);
+        kb[i] = kh + p * a.k.page + slot * a.k.slot;
+        vb[i] = vh + p * a.v.page + slot * a.v.slot;
+      }
+      const int ks = (int)a.k.slot, vs = (int)a.v.slot;
+#pragma unroll
+      for (int i = 0; i < L::kUnits; ++i) {
+        const int u = i * kThreads + tid, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
+        fetch((kPart > 1 && key & 32 ? kb[1] : kb[0]) + (key & 31) * ks, e, rk[i], sk[i]);
+        fetch((kPart > 1 && key & 32 ? vb[1] : vb[0]) + (key & 31) * vs, e, rv[i], sv[i]);
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < L::kUnits; ++i) {
+      const int u = i * kThreads + tid, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
+      const int p = __shfl(page, key, kWave);
+      const long long slot = p < 0 ? 0 : slot_of(pos + key);
+      fetch(kh + (long long)max(p, 0) * a.k.page + slot * a.k.slot, e, rk[i], sk[i]);
+      fetch(vh + (long long)max(p, 0) * a.v.page + slot * a.v.slot, e, rv[i], sv[i]);
+    }
+  };
+  // a unit's values, in 16 bits, into a row in LDS
+  auto put = [&](const Bytes16& b, uint32_t step16, bool zero, uint8_t* dst, int e) {
+    if constexpr (T == kKvF16) {
+      uint4 x = make_uint4(b.w[0], b.w[1], b.w[2], b.w[3]);
+      if (zero) x = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(dst + 16 * e) = x;
+    } else {
+      const _Float16 s1 = zero ? (_Float16)0.f : __builtin_bit_cast(_Float16, (uint16_t)step16);
+      const f16x2 s = {s1, s1};
+      f16x2 x[2][8];
+      if constexpr (T == kKvQ8_0) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) codes4<128>(b.w[w] ^ 0x80808080u, x[0][2 * w], x[0][2 * w + 1]);
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          codes4<8>(b.w[w] & 0x0f0f0f0fu, x[0][2 * w], x[0][2 * w + 1]);
+          codes4<8>(b.w[w] >> 4 & 0x0f0f0f0fu, x[1][2 * w], x[1][2 * w + 1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < (T == kKvQ8_0 ? 1 : 2); ++i) {
+        uint32_t y[8];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) y[w] = __builtin_bit_cast(uint32_t, x[i][w] * s);
+        uint4* to = reinterpret_cast<uint4*>(dst + (T == kKvQ8_0 ? 32 * e : 64 * e + 32 * i));
+        to[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        to[1] = make_uint4(y[4], y[5], y[6], y[7]);
+      }
+    }
+  };
+  // a step in which the tile's rows see different keys, or not all of them
+  auto is_edge = [&](int pos, unsigned long long present) {
+    return pos + kStep - 1 > first_all || (a.window > 0 && pos <= last_all - a.window && pos + kStep - 1 >= a.sinks) ||
+           present != ~0ull;
+  };
+  // the loaded step into LDS buffer `buf`; V of a key that no row sees is zeros
+  auto store = [&](int step, int page, int buf) {
+    const int tid = opaque_tid();
+    const unsigned long long present = __ballot(page >= 0);
+    const bool edge = is_edge(step_position<kStep>(t.range, step), present);
+    uint8_t* base = lds + buf * L::kBytes;
+    unsigned long long spoiled = 0;
+#pragma unroll
+    for (int i = 0; i < L::kUnits; ++i) {
+      const int u = i * kThreads + tid, key = u / L::kUnit, e = u % L::kUnit;
+      if (!L::kEven && key >= kStep) continue;
+      put(rk[i], sk[i], false, base + key * L::kKRow, e);
+      bool zero = false;
+      if (edge) {
+        zero = !((uint32_t)(key & 32 ? present >> 32 : present) >> (key & 31) & 1u);
+        bool bad = false;
+        if constexpr (T == kKvF16) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) bad = bad || half_not_finite(rv[i].w[w]) || half_not_finite(rv[i].w[w] >> 16);
+        } else {
+          bad = half_not_finite(sv[i]);
+        }
+        if (bad && !zero) spoiled |= 1ull << key;
+        zero = zero || bad;
+      }
+      put(rv[i], sv[i], zero, base + L::kV + key * L::kVRow, e);
+    }
+    if (edge) {
+      if (__ballot(spoiled != 0)) {  // hardly ever
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1)
+          spoiled |= (unsigned long long)__shfl_xor((long long)spoiled, s, kWave);
+      }
+      if (lane == 0) spoiled_of[buf][wave] = spoiled;
+    }
+  };
+
+  int page = pages_of(step0), next_page = pages_of(step0 + 1);
+  if (step0 < step1) {
+    load(step0, page);
+    store(step0, page, 0);
+  }
+  __syncthreads();
+  for (int step = step0; step < step1; ++step) {
+    const int buf = (step - step0) & 1;
+    const int pos = step_position<kStep>(t.range, step);
+    const unsigned long long present = __ballot(page >= 0);
+    if (step + 1 < step1) load(step + 1, next_page);
+
+    // rows of this wave see none, different, or all of the step's keys
+    const bool none = idle || pos > last_pos ||
+                      (a.window > 0 && pos + kStep - 1 <= first_pos - a.window && pos >= a.sinks);
+    const bool masked = pos + kStep - 1 > first_pos ||
+                        (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks) || present != ~0ull;
+    if (!none) {
+      const uint8_t* base = lds + buf * L::kBytes;
+      f32x16 s[kPart] = {};
+      // operands come two blocks ahead of their products; the barriers keep the
+      // scheduler from fetching them all at once, which the registers would not hold
+      constexpr int kAhead = 2;
+      f16x8 kf[kAhead][kPart];
+      auto k_at = [&](int b, int i) {
+        return *reinterpret_cast<const f16x8*>(base + (32 * i + c) * L::kKRow + 32 * b + 16 * h);
+      };
+#pragma unroll
+      for (int b = 0; b < kAhead; ++b)
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) kf[b][i] = k_at(b, i);
+#pragma unroll
+      for (int b = 0; b < 2 * NB; ++b) {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) {
+          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b % kAhead][i], qf[b], s[i], 0, 0, 0);
+          if (b + kAhead < 2 * NB) kf[b % kAhead][i] = k_at(b + kAhead, i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      float top;
+      if (masked) {
+        // value e of half i: key 32 i + 8 (e / 4) + 4 h + e % 4
+        const unsigned long long seen = seen_bits(a, present, pos, qpos) >> (4 * h);
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) {
+          const uint32_t bits = (uint32_t)(seen >> (32 * i));
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[i][e] = bits & 1u << (8 * (e / 4) + e % 4) ? s[i][e] * a.scale : -INFINITY;
+            top = fmaxf(top, s[i][e]);
+          }
+        }
+      } else {
+        top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kPart; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            s[i][e] *= a.scale;
+            top = fmaxf(top, s[i][e]);
+          }
+      }
+      {
+        typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+        const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      }
+      if (__ballot(top > m + kLag)) {
+        const float now = fmaxf(m, top);
+        const float f = now == -INFINITY ? 1.f : exp2_fast(m - now);
+        m = now;
+        l *= f;
+#pragma unroll
+        for (int v = 0; v < NB; ++v) o[v] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      f16x8 p[2 * kPart];
+#pragma unroll
+      for (int i = 0; i < kPart; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float w = exp2_fast(s[i][e] - ref);
+          l += w;
+          p[2 * i + e / 8][e % 8] = (_Float16)w;
+        }
+      // O^T += V^T P^T: 16 keys a product, four of a quarter's and four 8 on
+      {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* LdsPtr;
+        const int i = lane & 15;
+        uint8_t* const vbase = lds + buf * L::kBytes + L::kV + (4 * h + i / 4) * L::kVRow + 32 * (lane >> 4 & 1) + 8 * (i & 3);
+        auto v_at = [&](int n) {  // product n: keys 16 (n / NB), values 32 (n % NB)
+          uint8_t* at = vbase + 16 * (n / NB) * L::kVRow + 64 * (n % NB);
+          const f16x4 lo = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at)));
+          const f16x4 hi = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 8 * L::kVRow)));
+          return f16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        };
+        constexpr int kAheadV = 4;
+        f16x8 vf[kAheadV];
+#pragma unroll
+        for (int n = 0; n < kAheadV; ++n) vf[n] = v_at(n);
+#pragma unroll
+        for (int n = 0; n < 2 * kPart * NB; ++n) {
+          o[n % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n % kAheadV], p[n / NB], o[n % NB], 0, 0, 0);
+          if (n + kAheadV < 2 * kPart * NB) vf[n % kAheadV] = v_at(n + kAheadV);
+          if (n % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (is_edge(pos, present)) {
+        // values that are not finite reach the rows that see their key, and no other
+        unsigned long long spoiled = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) spoiled |= spoiled_of[buf][w];
+        while (spoiled) {
+          const int key = __builtin_ctzll(spoiled);
+          spoiled &= spoiled - 1;
+          int pg, slot;
+          if (!kv_place(a.seqs, seq, pos + key, pg, slot)) continue;
+          const uint8_t* vr = a.v.data + (long long)kvh * a.v.head + pg * a.v.page + slot * a.v.slot;
+          const int want = 16 * (key / 32) + 4 * (key % 32 / 8) + key % 4;
+          float w = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16 * kPart; ++e) w = e == want ? (float)p[e / 8][e % 8] : w;
+          w = __shfl(w, 32 * (key / 4 & 1) + c, kWave);
+          if (seen_bits(a, 1ull, pos + key, qpos)) {
+#pragma unroll
+            for (int v = 0; v < NB; ++v)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                o[v][e] += w * value_of<T>(vr, 32 * v + 8 * (e / 4) + 4 * h + e % 4);
+                asm volatile("" ::: "memory");  // one value at a time: no registers for this path
+              }
+          }
+        }
+      }
+    }
+    page = next_page;
+    if (step + 1 < step1) store(step + 1, page, buf ^ 1);
+    next_page = pages_of(step + 2);
+    __syncthreads();
+  }
+
+  // a lane has value 32 v + 8 (e / 4) + 4 h + e % 4 of its row
+  if (kRows * wave + c >= t.rows) return;
+  {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  if (!whole) {
+    // the item's number in the sequences' order, as the join counts it
+    const long long item = (long long)(gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads) * a.kv_heads + kvh;
+    float* part = a.part + (item * a.splits + split) * (kWaves * kRows) * (D + 2) + (kRows * wave + c) * (D + 2);
+#pragma unroll
+    for (int v = 0; v < NB; ++v)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) part[32 * v + 8 * (e / 4) + 4 * h + e % 4] = o[v][e];
+    if (h == 0) part[D] = m, part[D + 1] = l;
+    return;
+  }
+  const float f = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
+  uint8_t* dst = a.o + (long long)(t.token0 + tok) * a.o_token + (long long)head * a.o_head;
+#pragma unroll
+  for (int v = 0; v < NB; ++v)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int e = 32 * v + 8 * g + 4 * h;
+      const float x[4] = {o[v][4 * g] * f, o[v][4 * g + 1] * f, o[v][4 * g + 2] * f, o[v][4 * g + 3] * f};
+      if (a.half_o) {
+        const f16x4 y = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+        *reinterpret_cast<Bytes8*>(dst + 2 * e) = __builtin_bit_cast(Bytes8, y);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(dst)[e + i] = x[i];
+      }
+    }
+}
+
+template <int T, int NB>
+void launch(const AttendArgs& a, dim3 grid, hipStream_t st) {
+  constexpr size_t kLds = 2 * Tile<T, NB>::kBytes;
+  attend_many_kernel<T, NB><<<grid, kThreads, kLds, st>>>(a);
+}
+
+template <int T>
+void launch_d(int d, const AttendArgs& a, dim3 grid, hipStream_t st) {
+  switch (d) {
+    case 64: launch<T, 2>(a, grid, st); break;
+    case 96: launch<T, 3>(a, grid, st); break;
+    case 128: launch<T, 4>(a, grid, st); break;
+    case 192: launch<T, 6>(a, grid, st); break;
+    default: launch<T, 8>(a, grid, st); break;
+  }
+}
+
+}  // namespace
+
+void attend_many(int type, int d, const AttendArgs& a, int items, hipStream_t st) {
+  const dim3 grid((unsigned)items, (unsigned)a.splits);
+  switch (type) {
+    case kKvF16: launch_d<kKvF16>(d, a, grid, st); break;
+    case kKvQ8_0: launch_d<kKvQ8_0>(d, a, grid, st); break;
+    default: launch_d<kKvQ4_0>(d, a, grid, st); break;
+  }
+  check_launch("attend_many_kernel");
+}
+
+}  // namespace weft
