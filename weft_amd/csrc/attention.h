@@ -24,7 +24,8 @@ struct AttendArgs {
   int step;        // keys a step, 32 or 64
   int splits;      // the most splits of a tile's steps
   int least;       // the fewest steps a split is made for
-  float scale;     // times log2 e
+  float scale;     // its magnitude times log2 e, > 0; the queries take its sign (0: they are zeros)
+  float sign;
   bool half_q, half_o;
   bool whole16;    // pages hold whole groups of 16 slots, strides below 2^26
   bool whole32;    // of 32
@@ -40,6 +41,12 @@ struct __attribute__((packed, aligned(2))) Bytes8 {
 struct __attribute__((packed, aligned(2))) Bytes16 {
   uint32_t w[4];
 };
+
+// a value that all lanes share, known to the compiler as such
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long uniform(long long x) {
+  return (long long)(((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
+}
 
 // the new tokens of a sequence, whatever its starts hold
 __device__ __forceinline__ int seq_tokens(const KvSeqs& s, int seq, int& first) {
@@ -101,7 +108,7 @@ __device__ __forceinline__ int split_steps(const AttendArgs& a) {
     for (int o = 32; o > 0; o >>= 1) steps = max(steps, __shfl_xor(steps, o, kWave));
     longest = max(longest, steps);
   }
-  return max(a.least, (longest + a.splits - 1) / a.splits);
+  return uniform(max(a.least, (longest + a.splits - 1) / a.splits));
 }
 
 // Tile t of the call's tiles in the sequences' order -> its sequence (-1: there
@@ -125,8 +132,8 @@ __device__ __forceinline__ int find_tile(const AttendArgs& a, int t, int& tile) 
     const int all = __builtin_amdgcn_readlane(sum, kWave - 1);
     if (t < all) {
       const int at = __popcll(__ballot(sum <= t));
-      tile = t - __shfl(sum - n, at, kWave);
-      return i + at;
+      tile = uniform(t - __shfl(sum - n, at, kWave));
+      return uniform(i + at);
     }
     t -= all;
   }
@@ -149,12 +156,12 @@ struct TileRows {
 
 __device__ __forceinline__ bool tile_rows(const AttendArgs& a, int seq, int tile, TileRows& t) {
   int first;
-  const int n = seq_tokens(a.seqs, seq, first);
+  const int n = uniform(seq_tokens(a.seqs, seq, first));
   t.seq = seq;
-  t.token0 = first;
+  t.token0 = uniform(first);
   t.row0 = tile * a.tile;
   t.rows = min(a.tile, n * a.share - t.row0);
-  t.pos0 = (long long)a.seqs.lengths[seq] - n;
+  t.pos0 = (long long)uniform(a.seqs.lengths[seq]) - n;
   if (tile < 0 || t.rows <= 0) return false;
   t.range = visible_range(a, t.pos0 + t.row0 / a.share, t.pos0 + (t.row0 + t.rows - 1) / a.share);
   return true;

@@ -8,6 +8,7 @@
 // attention_few.hip has tiles of 16 query rows, attention_many.hip of 128; this
 // file checks calls, chooses tiles and splits, and joins the splits.
 #include <algorithm>
+#include <cmath>
 
 #include "attention.h"
 #include "runtime.h"
@@ -16,9 +17,38 @@ namespace weft {
 namespace {
 
 // The splits of a (token, head) row, each with its maximum, sum and weighted
-// values: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.  One workgroup a row;
-// groups of lanes take every so-many-th split, four values a lane.
+// values: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 constexpr int kJoinThreads = 256, kMaxSplits = 256;
+
+__device__ __forceinline__ void store_row4(const AttendArgs& a, int t, int head, int e, f32x4 x, float all) {
+  x *= all == 0.f ? 0.f : 1.f / all;  // a row that saw nothing: zeros
+  uint8_t* dst = a.o + (long long)t * a.o_token + (long long)head * a.o_head;
+  if (a.half_o) {
+    const f16x4 h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+    *reinterpret_cast<Bytes8*>(dst + 2 * e) = __builtin_bit_cast(Bytes8, h);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(dst)[e + i] = x[i];
+  }
+}
+
+// where a row's partial results begin, and how many splits it has (0: none to join)
+__device__ __forceinline__ int row_splits(const AttendArgs& a, int d, int seq, int t, int head, const float*& part,
+                                          long long& stride) {
+  int first;
+  seq_tokens(a.seqs, seq, first);
+  const int kvh = head / a.share, row = (t - first) * a.share + head - kvh * a.share;
+  TileRows rows;
+  const int before = tiles_before(a, seq), each = split_steps(a);
+  if (!tile_rows(a, seq, row / a.tile, rows)) return 0;
+  const int n = (rows.range.steps + each - 1) / each;
+  stride = (long long)a.tile * (d + 2);
+  part = a.part + ((long long)(before + row / a.tile) * a.kv_heads + kvh) * a.splits * stride + (row % a.tile) * (d + 2);
+  return n > 1 ? n : 0;  // one: written by its only split
+}
+
+// Few rows, many splits: a workgroup a row, groups of lanes taking every
+// so-many-th split, four values a lane.
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttendArgs a) {
   constexpr int kLanes = D <= 128 ? 32 : 64;  // of which D / 4 work
@@ -27,19 +57,12 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttendArgs a)
   __shared__ float wave_top[kJoinThreads / kWave], wave_sums[kJoinThreads / kWave];
   __shared__ f32x4 sums[kGroups][kLanes];
   const int t = (int)blockIdx.x, head = (int)blockIdx.y, tid = threadIdx.x;
-  const int kvh = head / a.share;
   const int seq = kv_sequence_of(a.seqs, t);
   if (seq < 0) return;
-  int first;
-  seq_tokens(a.seqs, seq, first);
-  const int row = (t - first) * a.share + head - kvh * a.share;
-  TileRows rows;
-  if (!tile_rows(a, seq, row / a.tile, rows)) return;
-  const int each = split_steps(a), n = (rows.range.steps + each - 1) / each;
-  if (n <= 1) return;  // written by its only split
-  const int item = (tiles_before(a, seq) + row / a.tile) * a.kv_heads + kvh;
-  const float* part = a.part + (long long)item * a.splits * a.tile * (D + 2) + (row % a.tile) * (D + 2);
-  const long long stride = (long long)a.tile * (D + 2);
+  const float* part;
+  long long stride;
+  const int n = row_splits(a, D, seq, t, head, part, stride);
+  if (n == 0) return;
   float m = -INFINITY, l = 0.f;
   if (tid < n) m = part[tid * stride + D], l = part[tid * stride + D + 1];
   const float wt = wave_max(m);
@@ -70,27 +93,56 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttendArgs a)
   if (group != 0 || 4 * lane >= D) return;
 #pragma unroll
   for (int i = 1; i < kGroups; ++i) x += sums[i][lane];
-  x *= all == 0.f ? 0.f : 1.f / all;
-  uint8_t* dst = a.o + (long long)t * a.o_token + (long long)head * a.o_head;
-  if (a.half_o) {
-    const f16x4 h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-    *reinterpret_cast<Bytes8*>(dst + 8 * lane) = __builtin_bit_cast(Bytes8, h);
+  store_row4(a, t, head, 4 * lane, x, all);
+}
+
+// Many rows, few splits: a group of lanes a row, several heads of a token a
+// workgroup.
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) attend_join_rows_kernel(AttendArgs a) {
+  constexpr int kLanes = D <= 128 ? 32 : 64;
+  constexpr int kGroups = kJoinThreads / kLanes;
+  const int t = (int)blockIdx.x, tid = threadIdx.x, lane = tid % kLanes;
+  const int heads = a.kv_heads * a.share, head = (int)blockIdx.y * kGroups + tid / kLanes;
+  const int seq = kv_sequence_of(a.seqs, t);
+  if (seq < 0) return;
+  const float* part;
+  long long stride;
+  const int n = row_splits(a, D, seq, t, min(head, heads - 1), part, stride);
+  if (n == 0 || head >= heads || 4 * lane >= D) return;
+  float top = -INFINITY, all = 0.f;
+  for (int i = 0; i < n; ++i) top = fmaxf(top, part[i * stride + D]);
+  f32x4 x = {};
+  for (int i = 0; i < n; ++i) {
+    const float* p = part + i * stride;
+    const float w = top == -INFINITY ? 0.f : exp2_fast(p[D] - top);
+    const f32x4 v = {p[4 * lane], p[4 * lane + 1], p[4 * lane + 2], p[4 * lane + 3]};
+    x += w * v;
+    all += w * p[D + 1];
+  }
+  store_row4(a, t, head, 4 * lane, x, all);
+}
+
+template <int D>
+void launch_join(const AttendArgs& a, bool rows, hipStream_t st) {
+  const unsigned tokens = (unsigned)a.seqs.n_tokens, heads = (unsigned)(a.kv_heads * a.share);
+  if (rows) {
+    constexpr unsigned kGroups = kJoinThreads / (D <= 128 ? 32 : 64);
+    attend_join_rows_kernel<D><<<dim3(tokens, (heads + kGroups - 1) / kGroups), kJoinThreads, 0, st>>>(a);
   } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(dst)[4 * lane + i] = x[i];
+    attend_join_kernel<D><<<dim3(tokens, heads), kJoinThreads, 0, st>>>(a);
   }
 }
 
-void join(int d, const AttendArgs& a, int heads, hipStream_t st) {
-  const dim3 grid((unsigned)a.seqs.n_tokens, (unsigned)heads);
+void join(int d, const AttendArgs& a, bool rows, hipStream_t st) {
   switch (d) {
-    case 64: attend_join_kernel<64><<<grid, kJoinThreads, 0, st>>>(a); break;
-    case 96: attend_join_kernel<96><<<grid, kJoinThreads, 0, st>>>(a); break;
-    case 128: attend_join_kernel<128><<<grid, kJoinThreads, 0, st>>>(a); break;
-    case 192: attend_join_kernel<192><<<grid, kJoinThreads, 0, st>>>(a); break;
-    default: attend_join_kernel<256><<<grid, kJoinThreads, 0, st>>>(a); break;
+    case 64: launch_join<64>(a, rows, st); break;
+    case 96: launch_join<96>(a, rows, st); break;
+    case 128: launch_join<128>(a, rows, st); break;
+    case 192: launch_join<192>(a, rows, st); break;
+    default: launch_join<256>(a, rows, st); break;
   }
-  check_launch("attend_join_kernel");
+  check_launch(rows ? "attend_join_rows_kernel" : "attend_join_kernel");
 }
 
 // Tiles and splits of a call, from what the host knows of it.
@@ -181,12 +233,13 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.share = (int)(q->ne[1] / w.heads);
   a.window = (int)std::min<int64_t>(window, INT32_MAX);
   a.sinks = (int)std::min<int64_t>(sinks, INT32_MAX);
-  a.scale = scale * 1.44269504f;  // weights are powers of two
+  a.scale = scale == 0.f ? 1.f : std::fabs(scale) * 1.44269504f;  // weights are powers of two
+  a.sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : 0.f;
   a.half_q = q->type == WEFT_GGML_TYPE_F16;
   a.half_o = dst->type == WEFT_GGML_TYPE_F16;
   const hipStream_t st = current_stream();
   (p.many ? attend_many : attend_few)(w.type, w.d, a, p.tiles * w.heads, st);
-  if (p.splits > 1) join(w.d, a, (int)q->ne[1], st);
+  if (p.splits > 1) join(w.d, a, p.many, st);
   return pending_error();
 }
 

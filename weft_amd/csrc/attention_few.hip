@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
   __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves][L::kBytes];
   __shared__ float ml[kWaves][16][2];
 
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;  // query column (or key, value) and quarter
   const int kvh = (int)blockIdx.x % a.kv_heads;
   const int split = (int)blockIdx.y;
@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int e = 32 * b + (T == kKvQ4_0 ? 4 * g + (j & 3) + 4 * (j & 4) : 8 * g + j);
-        const float x = a.half_q ? (float)*reinterpret_cast<const _Float16*>(src + 2 * e)
-                                 : *reinterpret_cast<const float*>(src + 4 * e);
+        const float x = a.sign * (a.half_q ? (float)*reinterpret_cast<const _Float16*>(src + 2 * e)
+                                           : *reinterpret_cast<const float*>(src + 4 * e));
         qh[rt][b][j] = (_Float16)x;
         ql[rt][b][j] = (_Float16)(x - (float)qh[rt][b][j]);
       }

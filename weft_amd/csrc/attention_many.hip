@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two steps' tiles
   __shared__ unsigned long long spoiled_of[2][kWaves];
 
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, tid = threadIdx.x;
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave), tid = threadIdx.x;
   const int c = lane & 31, h = lane >> 5;  // query column (or key, value) and half
   const int kvh = (int)blockIdx.x % a.kv_heads;
   const int split = (int)blockIdx.y;
@@ -79,13 +79,13 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     if (a.half_q) {
 #pragma unroll
       for (int b = 0; b < 2 * NB; ++b)
-        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h));
+        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h)) * (_Float16)a.sign;
     } else {
 #pragma unroll
       for (int b = 0; b < 2 * NB; ++b) {
         const float* x = reinterpret_cast<const float*>(src) + 16 * b + 8 * h;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)x[j];
+        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)(x[j] * a.sign);
       }
     }
   }
@@ -109,26 +109,31 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     return a.seqs.page_shift >= 0 ? at & (a.seqs.page_size - 1) : (int)((uint32_t)at % (uint32_t)a.seqs.page_size);
   };
   // a unit of a row: 16 bytes of values or codes, and their step
-  auto fetch = [&](const uint8_t* r, int e, Bytes16& b, uint32_t& s) {
+  auto fetch = [&](const uint8_t* base, uint32_t off, int e, Bytes16& b, uint32_t& s) {
     if constexpr (T == kKvF16) {
-      b = *reinterpret_cast<const Bytes16*>(r + 16 * e);
+      b = *reinterpret_cast<const Bytes16*>(base + (off + 16 * e));
     } else if constexpr (T == kKvQ8_0) {
-      b = *reinterpret_cast<const Bytes16*>(r + 34 * (e / 2) + 2 + 16 * (e & 1));
-      s = ld_u16(r + 34 * (e / 2));
+      b = *reinterpret_cast<const Bytes16*>(base + (off + 34 * (e / 2) + 2 + 16 * (e & 1)));
+      s = ld_u16(base + (off + 34 * (e / 2)));
     } else {
-      b = *reinterpret_cast<const Bytes16*>(r + 18 * e + 2);
-      s = ld_u16(r + 18 * e);
+      b = *reinterpret_cast<const Bytes16*>(base + (off + 18 * e + 2));
+      s = ld_u16(base + (off + 18 * e));
     }
   };
-  // the thread's number behind a barrier to the optimizer, which would keep every
-  // unit's address and mask in registers across the loop
+  // Units per row a power of two: unit i of a thread is its unit 0 some whole rows
+  // on, in the wave's half of the step, so one offset a thread serves them all.
+  // Else (heads of 96 and 192) each unit's place is computed at each step, behind a
+  // barrier to the optimizer, which would keep them all in registers.
+  constexpr bool kSame = (L::kUnit & (L::kUnit - 1)) == 0;
+  constexpr int kRowsOn = kThreads / L::kUnit;  // rows between a thread's units
+  const int key0 = tid / L::kUnit, e0 = tid % L::kUnit;
   auto opaque_tid = [&] {
     int x = tid;
     asm volatile("" : "+v"(x));
     return x;
   };
+  const uint32_t koff = (uint32_t)(key0 & 31) * (uint32_t)a.k.slot, voff = (uint32_t)(key0 & 31) * (uint32_t)a.v.slot;
   auto load = [&](int step, int page) {
-    const int tid = opaque_tid();
     const int pos = step_position<kStep>(t.range, step);
     const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
     const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
@@ -144,22 +149,38 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         kb[i] = kh + p * a.k.page + slot * a.k.slot;
         vb[i] = vh + p * a.v.page + slot * a.v.slot;
       }
-      const int ks = (int)a.k.slot, vs = (int)a.v.slot;
+      if constexpr (kSame) {
 #pragma unroll
-      for (int i = 0; i < L::kUnits; ++i) {
-        const int u = i * kThreads + tid, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
-        fetch((kPart > 1 && key & 32 ? kb[1] : kb[0]) + (key & 31) * ks, e, rk[i], sk[i]);
-        fetch((kPart > 1 && key & 32 ? vb[1] : vb[0]) + (key & 31) * vs, e, rv[i], sv[i]);
+        for (int i = 0; i < L::kUnits; ++i) {
+          // a wave's units lie in one half: those past the step read its last rows again
+          const int at = min(i * kRowsOn + __builtin_amdgcn_readfirstlane(key0), kStep - 1);
+          const bool half = kPart > 1 && at >= 32;
+          const int on = i * kRowsOn & 31 & ~(kRowsOn - 1);  // whole rows on, inside the half
+          const uint8_t* kr = (half ? kb[1] : kb[0]) + on * a.k.slot;
+          const uint8_t* vr = (half ? vb[1] : vb[0]) + on * a.v.slot;
+          fetch(kr, koff, e0, rk[i], sk[i]);
+          fetch(vr, voff, e0, rv[i], sv[i]);
+        }
+      } else {
+        const int x = opaque_tid();
+        const uint32_t ks = (uint32_t)a.k.slot, vs = (uint32_t)a.v.slot;
+#pragma unroll
+        for (int i = 0; i < L::kUnits; ++i) {
+          const int u = i * kThreads + x, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
+          fetch(kPart > 1 && key & 32 ? kb[1] : kb[0], (key & 31) * ks, e, rk[i], sk[i]);
+          fetch(kPart > 1 && key & 32 ? vb[1] : vb[0], (key & 31) * vs, e, rv[i], sv[i]);
+        }
       }
       return;
     }
+    const int x = opaque_tid();
 #pragma unroll
     for (int i = 0; i < L::kUnits; ++i) {
-      const int u = i * kThreads + tid, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
+      const int u = i * kThreads + x, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
       const int p = __shfl(page, key, kWave);
       const long long slot = p < 0 ? 0 : slot_of(pos + key);
-      fetch(kh + (long long)max(p, 0) * a.k.page + slot * a.k.slot, e, rk[i], sk[i]);
-      fetch(vh + (long long)max(p, 0) * a.v.page + slot * a.v.slot, e, rv[i], sv[i]);
+      fetch(kh + (long long)max(p, 0) * a.k.page + slot * a.k.slot, 0, e, rk[i], sk[i]);
+      fetch(vh + (long long)max(p, 0) * a.v.page + slot * a.v.slot, 0, e, rv[i], sv[i]);
     }
   };
   // a unit's values, in 16 bits, into a row in LDS
@@ -200,14 +221,15 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   };
   // the loaded step into LDS buffer `buf`; V of a key that no row sees is zeros
   auto store = [&](int step, int page, int buf) {
-    const int tid = opaque_tid();
+    const int x = kSame ? tid : opaque_tid();
     const unsigned long long present = __ballot(page >= 0);
     const bool edge = is_edge(step_position<kStep>(t.range, step), present);
     uint8_t* base = lds + buf * L::kBytes;
     unsigned long long spoiled = 0;
 #pragma unroll
     for (int i = 0; i < L::kUnits; ++i) {
-      const int u = i * kThreads + tid, key = u / L::kUnit, e = u % L::kUnit;
+      const int u = i * kThreads + x;
+      const int key = kSame ? i * kRowsOn + key0 : u / L::kUnit, e = kSame ? e0 : u % L::kUnit;
       if (!L::kEven && key >= kStep) continue;
       put(rk[i], sk[i], false, base + key * L::kKRow, e);
       bool zero = false;
@@ -285,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
           const uint32_t bits = (uint32_t)(seen >> (32 * i));
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            s[i][e] = bits & 1u << (8 * (e / 4) + e % 4) ? s[i][e] * a.scale : -INFINITY;
+            s[i][e] = bits & 1u << (8 * (e / 4) + e % 4) ? s[i][e] : -INFINITY;
             top = fmaxf(top, s[i][e]);
           }
         }
@@ -294,15 +316,12 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
 #pragma unroll
         for (int i = 0; i < kPart; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            s[i][e] *= a.scale;
-            top = fmaxf(top, s[i][e]);
-          }
+          for (int e = 0; e < 16; ++e) top = fmaxf(top, s[i][e]);
       }
       {
         typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
         const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale;  // a.scale > 0
       }
       if (__ballot(top > m + kLag)) {
         const float now = fmaxf(m, top);
@@ -318,10 +337,11 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       for (int i = 0; i < kPart; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float w = exp2_fast(s[i][e] - ref);
+          const float w = exp2_fast(fmaf(s[i][e], a.scale, -ref));
           l += w;
           p[2 * i + e / 8][e % 8] = (_Float16)w;
         }
+      asm volatile("" : "+v"(l));  // summed here: 32 weights more in registers would not fit
       // O^T += V^T P^T: 16 keys a product, four of a quarter's and four 8 on
       {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -359,7 +379,12 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
           const int want = 16 * (key / 32) + 4 * (key % 32 / 8) + key % 4;
           float w = 0.f;
 #pragma unroll
-          for (int e = 0; e < 16 * kPart; ++e) w = e == want ? (float)p[e / 8][e % 8] : w;
+          for (int k = 0; k < 2 * kPart; ++k) {
+            f16x8 pk = p[k];
+            asm volatile("" : "+v"(pk));  // converted here, not beside every step's weights
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w = 8 * k + e == want ? (float)pk[e] : w;
+          }
           w = __shfl(w, 32 * (key / 4 & 1) + c, kWave);
           if (seen_bits(a, 1ull, pos + key, qpos)) {
 #pragma unroll
