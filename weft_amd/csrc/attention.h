@@ -27,8 +27,9 @@ struct AttendArgs {
   float scale;     // its magnitude times log2 e, > 0; the queries take its sign (0: they are zeros)
   float sign;
   bool half_q, half_o;
-  bool whole16;    // pages hold whole groups of 16 slots, strides below 2^26
-  bool whole32;    // of 32
+  // pages of a power of two >= 16 (32) slots, none longer than 2^31 bytes, so that
+  // 16 (32) keys lie in one page and offsets in a page in 32 bits
+  bool whole16, whole32;
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));

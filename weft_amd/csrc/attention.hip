@@ -219,9 +219,14 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.splits = p.splits;
   a.least = p.least;
   a.kv_heads = w.heads;
-  const bool near = w.k.slot >= 0 && w.k.slot < 1 << 26 && w.v.slot >= 0 && w.v.slot < 1 << 26;
-  a.whole16 = near && w.seqs.page_size % 16 == 0;
-  a.whole32 = near && w.seqs.page_size % 32 == 0;
+  // a page's slots span less than 2^31 bytes, and so do two pages' starts
+  const auto near = [&](const KvPool& c) {
+    return c.slot >= 0 && c.page >= 0 && c.page < (long long)1 << 31 &&
+           c.slot < ((long long)1 << 31) / w.seqs.page_size;
+  };
+  const bool fits = near(w.k) && near(w.v) && w.seqs.page_shift >= 0;
+  a.whole16 = fits && w.seqs.page_size >= 16;
+  a.whole32 = fits && w.seqs.page_size >= 32;
   a.k = w.k;
   a.v = w.v;
   a.q = static_cast<const uint8_t*>(q->data);

@@ -119,14 +119,10 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
   uint8_t* const vrow = lds[wave];
   float* const ksteps = reinterpret_cast<float*>(lds[wave] + L::kSteps);
 
-  // page of a step's key `lane & 31`, -1 where it is absent or no row sees it
+  // page of a step's key `lane & 31`, -1 where it is absent
   auto pages_of = [&](int step) {
     int page = -1, slot;
-    if (step < step1) {
-      const int pos = step_position<kStep>(t.range, step) + (lane & 31);
-      const bool seen = pos < t.range.end && (a.window == 0 || pos > first_pos - a.window || pos < a.sinks);
-      if (!kv_place(a.seqs, seq, pos, page, slot) || !seen) page = -1;
-    }
+    if (step < step1 && !kv_place(a.seqs, seq, step_position<kStep>(t.range, step) + (lane & 31), page, slot)) page = -1;
     return page;
   };
   // addresses: key's row in a pool, absent keys at the pool's first row
@@ -137,13 +133,10 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
       const uint8_t *kb[2], *vb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        // a group of 16 keys lies in one page: that of any key that is there
-        const uint32_t there = (uint32_t)__ballot(page >= 0) >> (16 * i) & 0xffffu;
-        const int p = there ? __builtin_amdgcn_readlane(page, 16 * i + __builtin_ctz(there)) : 0;
-        const int at = pos + 16 * i;
-        const int slot = a.seqs.page_shift >= 0 ? at & (a.seqs.page_size - 1) : at % a.seqs.page_size;
-        kb[i] = a.k.data + kh + p * a.k.page + slot * a.k.slot;
-        vb[i] = a.v.data + vh + p * a.v.page + slot * a.v.slot;
+        const uint32_t p = (uint32_t)max(__builtin_amdgcn_readlane(page, 16 * i), 0);
+        const uint32_t slot = (uint32_t)(pos + 16 * i) & (uint32_t)(a.seqs.page_size - 1);
+        kb[i] = a.k.data + kh + ((unsigned long long)p * (uint32_t)a.k.page + slot * (uint32_t)a.k.slot);
+        vb[i] = a.v.data + vh + ((unsigned long long)p * (uint32_t)a.v.page + slot * (uint32_t)a.v.slot);
       }
       const int ks = (int)a.k.slot, vs = (int)a.v.slot;
 #pragma unroll
@@ -217,7 +210,11 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
   if (step < step1) load(step, page, raw);
   for (; step < step1; step += kWaves) {
     const int pos = step_position<kStep>(t.range, step);
-    const uint32_t present = (uint32_t)__ballot(page >= 0);  // key i: bit i
+    // the keys that are there and that some row sees, key i as bit i
+    uint32_t present = (uint32_t)__ballot(page >= 0);
+    if (pos + kStep > t.range.end) present &= (uint32_t)first_bits(t.range.end - pos);
+    if (a.window > 0 && pos <= first_pos - a.window)
+      present &= (uint32_t)(~first_bits(first_pos - a.window - pos + 1) | first_bits(a.sinks - pos));
     // rows see different keys of this step
     const bool mixed = pos + kStep - 1 > first_pos ||
                        (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks);

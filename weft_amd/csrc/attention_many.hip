@@ -93,15 +93,22 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   f32x16 o[NB] = {};
   float m = -INFINITY, l = 0.f;
 
-  // page of a step's key `lane` (of 32: keys twice), -1 where it is absent or no row of the tile sees it
+  // page of a step's key `lane` (of 32: keys twice), -1 where it is absent
   auto pages_of = [&](int step) {
     int page = -1, slot;
-    if (step < step1) {
-      const int pos = step_position<kStep>(t.range, step) + (lane & (kStep - 1));
-      const bool seen = pos < t.range.end && (a.window == 0 || pos > first_all - a.window || pos < a.sinks);
-      if (!kv_place(a.seqs, seq, pos, page, slot) || !seen) page = -1;
-    }
+    if (step < step1 && !kv_place(a.seqs, seq, step_position<kStep>(t.range, step) + (lane & (kStep - 1)), page, slot))
+      page = -1;
     return page;
+  };
+  // the keys of a step that are there and that some row of the tile sees
+  auto present_of = [&](int pos, int page) {
+    unsigned long long present = __ballot(page >= 0);
+    if (pos + kStep > t.range.end || (a.window > 0 && pos <= first_all - a.window)) {
+      unsigned long long seen = first_bits(t.range.end - pos);
+      if (a.window > 0) seen &= ~first_bits(first_all - a.window - pos + 1) | first_bits(a.sinks - pos);
+      present &= seen;
+    }
+    return present;
   };
   Bytes16 rk[L::kUnits], rv[L::kUnits];
   uint32_t sk[L::kUnits], sv[L::kUnits];
@@ -138,26 +145,25 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
     const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
     if (a.whole32) {
-      const unsigned long long there = __ballot(page >= 0);
+      // 32 keys lie in one page
       const uint8_t *kb[2], *vb[2];
 #pragma unroll
       for (int i = 0; i < kPart; ++i) {
-        // 32 keys lie in one page: that of any key that is there
-        const uint32_t some = (uint32_t)(there >> (32 * i));
-        const int p = some ? __builtin_amdgcn_readlane(page, 32 * i + __builtin_ctz(some)) : 0;
-        const int slot = slot_of(pos + 32 * i);
-        kb[i] = kh + p * a.k.page + slot * a.k.slot;
-        vb[i] = vh + p * a.v.page + slot * a.v.slot;
+        const uint32_t p = (uint32_t)max(__builtin_amdgcn_readlane(page, 32 * i), 0);
+        const uint32_t slot = (uint32_t)(pos + 32 * i) & (uint32_t)(a.seqs.page_size - 1);
+        kb[i] = kh + ((unsigned long long)p * (uint32_t)a.k.page + slot * (uint32_t)a.k.slot);
+        vb[i] = vh + ((unsigned long long)p * (uint32_t)a.v.page + slot * (uint32_t)a.v.slot);
       }
       if constexpr (kSame) {
 #pragma unroll
         for (int i = 0; i < L::kUnits; ++i) {
-          // a wave's units lie in one half: those past the step read its last rows again
-          const int at = min(i * kRowsOn + __builtin_amdgcn_readfirstlane(key0), kStep - 1);
-          const bool half = kPart > 1 && at >= 32;
-          const int on = i * kRowsOn & 31 & ~(kRowsOn - 1);  // whole rows on, inside the half
-          const uint8_t* kr = (half ? kb[1] : kb[0]) + on * a.k.slot;
-          const uint8_t* vr = (half ? vb[1] : vb[0]) + on * a.v.slot;
+          // a wave's units lie in one half, whole rows on in it; those past the step
+          // read its last rows again
+          const bool half = kPart > 1 && (kRowsOn <= 32 ? i * kRowsOn >= 32 : uniform(key0) >= 32);
+          constexpr int kOn = kRowsOn <= 32 ? kRowsOn : 32;
+          const uint32_t on = (uint32_t)(i * kOn & 31);
+          const uint8_t* kr = (half ? kb[1] : kb[0]) + on * (uint32_t)a.k.slot;
+          const uint8_t* vr = (half ? vb[1] : vb[0]) + on * (uint32_t)a.v.slot;
           fetch(kr, koff, e0, rk[i], sk[i]);
           fetch(vr, voff, e0, rv[i], sv[i]);
         }
@@ -222,8 +228,9 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   // the loaded step into LDS buffer `buf`; V of a key that no row sees is zeros
   auto store = [&](int step, int page, int buf) {
     const int x = kSame ? tid : opaque_tid();
-    const unsigned long long present = __ballot(page >= 0);
-    const bool edge = is_edge(step_position<kStep>(t.range, step), present);
+    const int pos = step_position<kStep>(t.range, step);
+    const unsigned long long present = present_of(pos, page);
+    const bool edge = is_edge(pos, present);
     uint8_t* base = lds + buf * L::kBytes;
     unsigned long long spoiled = 0;
 #pragma unroll
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   for (int step = step0; step < step1; ++step) {
     const int buf = (step - step0) & 1;
     const int pos = step_position<kStep>(t.range, step);
-    const unsigned long long present = __ballot(page >= 0);
+    const unsigned long long present = present_of(pos, page);
     if (step + 1 < step1) load(step + 1, next_page);
 
     // rows of this wave see none, different, or all of the step's keys
