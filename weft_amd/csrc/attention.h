@@ -21,7 +21,7 @@ struct AttendArgs {
   long long q_head, q_token, o_head, o_token;  // byte strides
   int share, kv_heads, window, sinks;
   int tile;        // rows a tile
-  int step;        // keys a step, 32 or 64
+  int step_shift;  // log2 of the keys a step, 5 or 6
   int splits;      // the most splits of a tile's steps
   int least;       // the fewest steps a split is made for
   float scale;     // its magnitude times log2 e, > 0; the queries take its sign (0: they are zeros)
@@ -30,8 +30,10 @@ struct AttendArgs {
   // pages of a power of two >= 16 (32) slots, none longer than 2^31 bytes, so that
   // 16 (32) keys lie in one page and offsets in a page in 32 bits
   bool whole16, whole32;
+  bool dense;  // and a page's slots follow each other, 16 rows beginning at multiples of 16 bytes
 };
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -43,17 +45,8 @@ struct __attribute__((packed, aligned(2))) Bytes16 {
   uint32_t w[4];
 };
 
-// a value that all lanes share, known to the compiler as such
+// a value that all lanes share, known to the compiler as one
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long long uniform(long long x) {
-  return (long long)(((unsigned long long)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x));
-}
-
-// the new tokens of a sequence, whatever its starts hold
-__device__ __forceinline__ int seq_tokens(const KvSeqs& s, int seq, int& first) {
-  first = max(0, min(s.starts[seq], s.n_tokens));
-  return max(0, max(0, min(s.starts[seq + 1], s.n_tokens)) - first);
-}
 
 struct Range {
   int sink_steps;   // steps at positions 0, step, ..
@@ -68,9 +61,9 @@ __device__ __forceinline__ Range visible_range(const AttendArgs& a, long long p0
   const long long table = (long long)a.seqs.max_pages * a.seqs.page_size;
   r.end = (int)max(0ll, min(min(p1 + 1, table), (long long)INT32_MAX - 128));
   const long long first = a.window > 0 ? max(0ll, p0 - a.window + 1) : 0;
-  r.begin = (int)min(first, (long long)r.end) & -a.step;
-  r.sink_steps = (min(a.sinks, r.begin) + a.step - 1) / a.step;
-  r.steps = r.sink_steps + (r.end - r.begin + a.step - 1) / a.step;
+  r.begin = (int)min(first, (long long)r.end) & -(1 << a.step_shift);
+  r.sink_steps = (min(a.sinks, r.begin) + (1 << a.step_shift) - 1) >> a.step_shift;
+  r.steps = r.sink_steps + ((r.end - r.begin + (1 << a.step_shift) - 1) >> a.step_shift);
   return r;
 }
 
@@ -91,79 +84,81 @@ __device__ __forceinline__ unsigned long long seen_bits(const AttendArgs& a, uns
   return present;
 }
 
-// Steps a split takes, the same for every tile of the call, so that a batch of
-// uneven sequences makes splits of even work: the longest sequence's steps over
-// the most splits.  The whole wave calls it.
-__device__ __forceinline__ int split_steps(const AttendArgs& a) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int longest = 0;
-  for (int i = 0; i < a.seqs.n_seqs; i += kWave) {
-    int steps = 0;
-    if (i + lane < a.seqs.n_seqs) {
-      int first;
-      const int n = seq_tokens(a.seqs, i + lane, first);
-      const long long len = a.seqs.lengths[i + lane];
-      if (n > 0) steps = visible_range(a, len - n, len - 1).steps;
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) steps = max(steps, __shfl_xor(steps, o, kWave));
-    longest = max(longest, steps);
-  }
-  return uniform(max(a.least, (longest + a.splits - 1) / a.splits));
-}
-
-// Tile t of the call's tiles in the sequences' order -> its sequence (-1: there
-// is none) and its tile in it; tile_of the other way round: the tiles of the
-// sequences before `seq`.  The whole wave calls both.
-__device__ __forceinline__ int seq_tiles(const AttendArgs& a, int seq) {
-  int first;
-  return seq < a.seqs.n_seqs ? (seq_tokens(a.seqs, seq, first) * a.share + a.tile - 1) / a.tile : 0;
-}
-
-__device__ __forceinline__ int find_tile(const AttendArgs& a, int t, int& tile) {
-  const int lane = threadIdx.x & (kWave - 1);
-  for (int i = 0; i < a.seqs.n_seqs; i += kWave) {
-    const int n = seq_tiles(a, i + lane);
-    int sum = n;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int up = __shfl_up(sum, o, kWave);
-      if (lane >= o) sum += up;
-    }
-    const int all = __builtin_amdgcn_readlane(sum, kWave - 1);
-    if (t < all) {
-      const int at = __popcll(__ballot(sum <= t));
-      tile = uniform(t - __shfl(sum - n, at, kWave));
-      return uniform(i + at);
-    }
-    t -= all;
-  }
-  return -1;
-}
-
-__device__ __forceinline__ int tiles_before(const AttendArgs& a, int seq) {
-  const int lane = threadIdx.x & (kWave - 1);
-  int n = 0;
-  for (int i = 0; i < seq; i += kWave) n += i + lane < seq ? seq_tiles(a, i + lane) : 0;
-  return wave_sum(n);
-}
-
-// One tile's rows: its first, how many, their first token and its position.
+// A tile of query rows: its sequence, rows and keys.
 struct TileRows {
-  int seq, row0, rows, token0;
-  long long pos0;  // of the sequence's first new token
+  int seq, row0, rows, token0;  // token0: the sequence's first new token
+  long long pos0;               // and its position
   Range range;
+  int each;    // steps a split takes
+  int before;  // tiles of the sequences before
 };
 
-__device__ __forceinline__ bool tile_rows(const AttendArgs& a, int seq, int tile, TileRows& t) {
-  int first;
-  const int n = uniform(seq_tokens(a.seqs, seq, first));
-  t.seq = seq;
-  t.token0 = uniform(first);
-  t.row0 = tile * a.tile;
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += dpp<kDppBcast15, 0xA>(v);
+  return v + dpp<kDppBcast31, 0xC>(v);
+}
+__device__ __forceinline__ int wave_max_count(int v) {  // of values >= 0
+  v = max(v, dpp<kDppXor1>(v));
+  v = max(v, dpp<kDppXor2>(v));
+  v = max(v, dpp<kDppHalfMirror>(v));
+  v = max(v, dpp<kDppMirror>(v));
+  v = max(v, dpp<kDppBcast15, 0xA>(v));
+  v = max(v, dpp<kDppBcast31, 0xC>(v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
+// Where a tile of the call lies: tile number `tile` in the sequences' order, or
+// with `row` >= 0 the tile of that new token's row (token, head in its group).
+// Also the steps a split takes: the longest sequence's over the most splits, the
+// same for every tile, so that a batch of uneven sequences makes splits of even
+// work.  The whole wave calls it; 64 sequences are looked at at once, so a call's
+// starts and lengths cost one trip to memory.
+__device__ __forceinline__ bool locate(const AttendArgs& a, int tile, int token, int head, TileRows& t) {
+  const int lane = threadIdx.x & (kWave - 1);
+  int longest = 0, before = 0, found = -1, first = 0, n = 0, in = 0;
+  long long len = 0;
+  for (int i = 0; i < a.seqs.n_seqs; i += kWave) {
+    int f = 0, count = 0, length = 0;
+    if (i + lane < a.seqs.n_seqs) {
+      f = max(0, min(a.seqs.starts[i + lane], a.seqs.n_tokens));
+      count = max(0, max(0, min(a.seqs.starts[i + lane + 1], a.seqs.n_tokens)) - f);
+      length = a.seqs.lengths[i + lane];
+    }
+    int steps = 0;
+    if (count > 0) steps = visible_range(a, (long long)length - count, (long long)length - 1).steps;
+    longest = max(longest, wave_max_count(steps));
+    const int tiles = (count * a.share + a.tile - 1) / a.tile;
+    const int sum = wave_scan(tiles), all = __builtin_amdgcn_readlane(sum, kWave - 1);
+    if (found < 0) {
+      const unsigned long long hit = token < 0 ? __ballot(before + sum > tile)
+                                               : __ballot(count > 0 && token >= f && token < f + count);
+      if (hit) {
+        const int at = __builtin_ctzll(hit);
+        found = i + at;
+        first = __builtin_amdgcn_readlane(f, at);
+        n = __builtin_amdgcn_readlane(count, at);
+        len = __builtin_amdgcn_readlane(length, at);
+        before += __builtin_amdgcn_readlane(sum - tiles, at);
+        in = tile - before;
+      } else {
+        before += all;
+      }
+    }
+  }
+  if (found < 0) return false;
+  if (token >= 0) in = ((token - first) * a.share + head) / a.tile;
+  t.seq = found;
+  t.token0 = first;
+  t.row0 = in * a.tile;
   t.rows = min(a.tile, n * a.share - t.row0);
-  t.pos0 = (long long)uniform(a.seqs.lengths[seq]) - n;
-  if (tile < 0 || t.rows <= 0) return false;
+  t.pos0 = len - n;
+  t.before = before;
+  t.each = max(a.least, (longest + a.splits - 1) / a.splits);
+  if (in < 0 || t.rows <= 0) return false;
   t.range = visible_range(a, t.pos0 + t.row0 / a.share, t.pos0 + (t.row0 + t.rows - 1) / a.share);
   return true;
 }

@@ -33,17 +33,15 @@ __device__ __forceinline__ void store_row4(const AttendArgs& a, int t, int head,
 }
 
 // where a row's partial results begin, and how many splits it has (0: none to join)
-__device__ __forceinline__ int row_splits(const AttendArgs& a, int d, int seq, int t, int head, const float*& part,
+__device__ __forceinline__ int row_splits(const AttendArgs& a, int d, int token, int head, const float*& part,
                                           long long& stride) {
-  int first;
-  seq_tokens(a.seqs, seq, first);
-  const int kvh = head / a.share, row = (t - first) * a.share + head - kvh * a.share;
-  TileRows rows;
-  const int before = tiles_before(a, seq), each = split_steps(a);
-  if (!tile_rows(a, seq, row / a.tile, rows)) return 0;
-  const int n = (rows.range.steps + each - 1) / each;
+  const int kvh = head / a.share;
+  TileRows t;
+  if (!locate(a, 0, token, head - kvh * a.share, t)) return 0;
+  const int n = (t.range.steps + t.each - 1) / t.each;
+  const int row = (token - t.token0) * a.share + head - kvh * a.share;
   stride = (long long)a.tile * (d + 2);
-  part = a.part + ((long long)(before + row / a.tile) * a.kv_heads + kvh) * a.splits * stride + (row % a.tile) * (d + 2);
+  part = a.part + ((long long)(t.before + row / a.tile) * a.kv_heads + kvh) * a.splits * stride + (row % a.tile) * (d + 2);
   return n > 1 ? n : 0;  // one: written by its only split
 }
 
@@ -57,11 +55,9 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttendArgs a)
   __shared__ float wave_top[kJoinThreads / kWave], wave_sums[kJoinThreads / kWave];
   __shared__ f32x4 sums[kGroups][kLanes];
   const int t = (int)blockIdx.x, head = (int)blockIdx.y, tid = threadIdx.x;
-  const int seq = kv_sequence_of(a.seqs, t);
-  if (seq < 0) return;
   const float* part;
   long long stride;
-  const int n = row_splits(a, D, seq, t, head, part, stride);
+  const int n = row_splits(a, D, t, head, part, stride);
   if (n == 0) return;
   float m = -INFINITY, l = 0.f;
   if (tid < n) m = part[tid * stride + D], l = part[tid * stride + D + 1];
@@ -104,11 +100,9 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_rows_kernel(AttendAr
   constexpr int kGroups = kJoinThreads / kLanes;
   const int t = (int)blockIdx.x, tid = threadIdx.x, lane = tid % kLanes;
   const int heads = a.kv_heads * a.share, head = (int)blockIdx.y * kGroups + tid / kLanes;
-  const int seq = kv_sequence_of(a.seqs, t);
-  if (seq < 0) return;
   const float* part;
   long long stride;
-  const int n = row_splits(a, D, seq, t, min(head, heads - 1), part, stride);
+  const int n = row_splits(a, D, t, min(head, heads - 1), part, stride);
   if (n == 0 || head >= heads || 4 * lane >= D) return;
   float top = -INFINITY, all = 0.f;
   for (int i = 0; i < n; ++i) top = fmaxf(top, part[i * stride + D]);
@@ -162,9 +156,12 @@ Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
   p.tile = p.many ? 128 : 16;
   p.step = p.many ? many_step(w.d) : 32;
   p.tiles = (int)std::min(tokens * ((share + p.tile - 1) / p.tile), rows / p.tile + std::min(tokens, seqs));
-  p.least = p.many ? 4 : 8;
-  // as many workgroups as run at once, unless there are that many tiles
-  const int64_t items = (int64_t)p.tiles * w.heads, want = (p.many ? 2 : 3) * (int64_t)cu_count();
+  p.least = 4;
+  // as many workgroups as run at once, unless there are that many tiles: more of
+  // them cost 10 % (131072 keys, Q8_0: 70 us at three a CU, 80 at six), as their
+  // first steps and joins add up
+  const int64_t resident = w.d > 128 ? 1 : p.many || w.type == kKvF16 ? 2 : 3;
+  const int64_t items = (int64_t)p.tiles * w.heads, want = resident * (int64_t)cu_count();
   const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + p.step - 1) / p.step;
   p.splits = (int)std::max<int64_t>(
       1, std::min({(want + items - 1) / items, (steps + p.least - 1) / p.least, (int64_t)kMaxSplits}));
@@ -215,7 +212,7 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.seqs.n_tokens = (int)q->ne[2];
   a.part = p.splits > 1 ? static_cast<float*>(work) : nullptr;
   a.tile = p.tile;
-  a.step = p.step;
+  a.step_shift = p.step == 64 ? 6 : 5;
   a.splits = p.splits;
   a.least = p.least;
   a.kv_heads = w.heads;
@@ -227,6 +224,10 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   const bool fits = near(w.k) && near(w.v) && w.seqs.page_shift >= 0;
   a.whole16 = fits && w.seqs.page_size >= 16;
   a.whole32 = fits && w.seqs.page_size >= 32;
+  const auto packed = [&](const KvPool& c) {
+    return c.slot == (long long)kv_row_bytes(w.type, w.d) && c.head % 16 == 0 && c.page % 16 == 0 && aligned(c.data, 16);
+  };
+  a.dense = a.whole16 && packed(w.k) && packed(w.v);
   a.k = w.k;
   a.v = w.v;
   a.q = static_cast<const uint8_t*>(q->data);

@@ -24,6 +24,8 @@
 // step); against them the weights are two parts as well, so that V's rounding is
 // all that the sum carries.  A 16-bit V is exact and takes rounded weights.
 // Maximum, sum and accumulators are in 32 bits.
+#include <type_traits>
+
 #include "attention.h"
 #include "runtime.h"
 
@@ -32,12 +34,19 @@ namespace {
 
 constexpr int kWaves = 4, kStep = 32;
 
-template <int T, int NB>
-struct Raw {  // a step's records: K as operands, V as rows
+// A step's records as they are loaded.  kDense: whole 16-byte lines of them, 32
+// rows one after the other, which LDS hands out as operands and units.
+template <int T, int NB, bool kDense>
+struct Raw {
   static constexpr int kVUnit = T == kKvF16 ? 4 * NB : T == kKvQ8_0 ? 2 * NB : NB;  // 16-byte units a row
   static constexpr int kV = (kVUnit * kStep + kWave - 1) / kWave;                  // units a lane
   static constexpr int kS = T == kKvF16 ? 1 : (NB + 3) / 4;                        // K steps a lane and 16 keys
   static constexpr int kKWords = T == kKvF16 ? 4 : T == kKvQ8_0 ? 2 : 1;
+  static constexpr int kRowBytes = KvRecord<T>::kBytes * NB;
+  static constexpr int kLines = kStep * kRowBytes / 16;  // a step's
+  // those of a last part of at most 32 of K and V go together: lanes 0.. and 32..
+  static constexpr int kRest = kLines % kWave <= 32 ? kLines % kWave : 0;
+  static constexpr int kLine = (kLines - kRest + kWave - 1) / kWave;  // a lane's besides
   uint32_t k[2][NB][kKWords];
   uint32_t ks[2][kS];
   Bytes16 v[kV];
@@ -52,7 +61,8 @@ struct Lds {
   static constexpr int kSteps = kStep * kRow;
   static constexpr int kBytes = kSteps + NB * kStep * 4;
   static constexpr int kORow = 32 * NB + 4;  // floats
-  static_assert(16 * kORow * 4 <= kBytes, "a group of rows' sums fit");
+  static_assert(16 * kORow * 4 <= kBytes && 2 * kStep * 34 * NB <= kSteps && 16 * kRow + kStep * 34 * NB <= kSteps,
+                "the rows' sums, and a step's records beside half its V rows");
 };
 
 __device__ __forceinline__ void wave_sync() {
@@ -61,153 +71,208 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int T, int NB, int RT>
-__global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_kernel(AttendArgs a) {
+template <int T, int NB, bool kDense>
+__global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_kernel(AttendArgs a) {
   using L = Lds<NB>;
-  using R = Raw<T, NB>;
+  using R = Raw<T, NB, kDense>;
   constexpr int D = 32 * NB;
   __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves][L::kBytes];
+  constexpr int kQRow = 64 * NB + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t qs[2][16 * kQRow];
   __shared__ float ml[kWaves][16][2];
 
   const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;  // query column (or key, value) and quarter
   const int kvh = (int)blockIdx.x % a.kv_heads;
   const int split = (int)blockIdx.y;
-  int tile;
-  const int seq = find_tile(a, (int)blockIdx.x / a.kv_heads, tile);
   TileRows t;
-  if (seq < 0 || !tile_rows(a, seq, tile, t)) return;
+  if (!locate(a, (int)blockIdx.x / a.kv_heads, -1, 0, t)) return;
+  const int seq = t.seq;
   int step0 = 0, step1 = t.range.steps;
   bool whole = true;  // the tile has one split
   if (a.part != nullptr) {
-    const int n = split_steps(a);
+    const int n = t.each;
     whole = n >= step1;
     step0 = min(split * n, step1);
     step1 = min(step0 + n, step1);
     if (split > 0 && step0 >= step1) return;
   }
 
-  // the queries, as right operands: lane c's row, values 8 g + j of each block
-  // (Q4_0: 4 g + j and 16 + 4 g + j)
-  f16x8 qh[RT][NB], ql[RT][NB];
-  int qpos[RT];  // -1: before the sequence
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int row = t.row0 + min(16 * rt + c, t.rows - 1);
+  // The queries into LDS, as right operands: lane (c, g) reads row c's values
+  // 8 g .. 8 g + 7 of a block (Q4_0: 4 g + j and 16 + 4 g + j) as 16 bytes; two
+  // parts of 16 bits where they have 32.
+  for (int i = threadIdx.x; i < 16 * 8 * NB; i += kWaves * kWave) {
+    const int r = i / (8 * NB), e = i % (8 * NB), b = e / 8, four = e % 8;
+    const int row = t.row0 + min(r, t.rows - 1);
     const int tok = row / a.share, head = kvh * a.share + row % a.share;
-    qpos[rt] = (int)max(-1ll, t.pos0 + tok);
     const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
+    f16x4 hi, lo;
+    if (a.half_q) {
+      hi = __builtin_bit_cast(f16x4, *reinterpret_cast<const Bytes8*>(src + 8 * e)) * (_Float16)a.sign;
+      lo = f16x4{};
+    } else {
+      const float* x = reinterpret_cast<const float*>(src) + 4 * e;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int e = 32 * b + (T == kKvQ4_0 ? 4 * g + (j & 3) + 4 * (j & 4) : 8 * g + j);
-        const float x = a.sign * (a.half_q ? (float)*reinterpret_cast<const _Float16*>(src + 2 * e)
-                                           : *reinterpret_cast<const float*>(src + 4 * e));
-        qh[rt][b][j] = (_Float16)x;
-        ql[rt][b][j] = (_Float16)(x - (float)qh[rt][b][j]);
+      for (int j = 0; j < 4; ++j) {
+        const float v = x[j] * a.sign;
+        hi[j] = (_Float16)v;
+        lo[j] = (_Float16)(v - (float)hi[j]);
       }
+    }
+    uint8_t* dst = qs[0] + r * kQRow + 64 * b + (T != kKvQ4_0 ? 8 * four : four < 4 ? 16 * four : 16 * (four - 4) + 8);
+    *reinterpret_cast<f16x4*>(dst) = hi;
+    *reinterpret_cast<f16x4*>(dst + 16 * kQRow) = lo;
   }
+  int qpos;  // of lane c's row; -1: before the sequence
+  {
+    const int row = t.row0 + min(c, t.rows - 1);
+    qpos = (int)max(-1ll, t.pos0 + row / a.share);
+  }
+  int qoff = c * kQRow + 16 * g;
   const int first_pos = (int)max(-1ll, t.pos0 + t.row0 / a.share);
   const int last_pos = (int)max(-1ll, t.pos0 + (t.row0 + t.rows - 1) / a.share);
 
-  f32x4 o[RT][2 * NB] = {};
-  float m[RT], l[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) m[rt] = -INFINITY, l[rt] = 0.f;
+  f32x4 o[2 * NB] = {};
+  float m = -INFINITY, l = 0.f;
 
   uint8_t* const vrow = lds[wave];
   float* const ksteps = reinterpret_cast<float*>(lds[wave] + L::kSteps);
 
-  // page of a step's key `lane & 31`, -1 where it is absent
-  auto pages_of = [&](int step) {
-    int page = -1, slot;
-    if (step < step1 && !kv_place(a.seqs, seq, step_position<kStep>(t.range, step) + (lane & 31), page, slot)) page = -1;
-    return page;
+  // The table's entry for a step's key `lane` (32 keys), looked up two steps
+  // ahead and not looked at before it is needed: a check here would wait for the
+  // load, and for the records loaded before it.  Past the table its last entry
+  // stands in; no key there is present.
+  auto entry_of = [&](int step) {
+    if (step >= step1) return -1;
+    const uint32_t pos = (uint32_t)(step_position<kStep>(t.range, step) + (lane & 31));
+    const uint32_t entry = a.seqs.page_shift >= 0 ? pos >> a.seqs.page_shift : pos / (uint32_t)a.seqs.page_size;
+    return a.seqs.pages[(long long)seq * a.seqs.pages_row + min(entry, (uint32_t)a.seqs.max_pages - 1)];
   };
-  // addresses: key's row in a pool, absent keys at the pool's first row
-  auto load = [&](int step, int page, R& r) {
+  // -1 where that is no page
+  auto page_of = [&](int entry) { return (uint32_t)entry < (uint32_t)a.seqs.n_pages ? entry : -1; };
+  // A step's records: K as operands (lane c's key of each 16, quarter g's values),
+  // V as rows of 16-byte units.  With whole groups of 16 keys in a page the bases
+  // are scalars and a lane's offsets constants; where a row's units are a power of
+  // two (>= 4), unit i of a lane is its unit 0 some whole rows on.  Else places are
+  // computed at each step, behind a barrier to the optimizer, which would keep them
+  // all in registers.  Absent keys read the pool's first row.
+  constexpr bool kSame = R::kVUnit >= 4 && (R::kVUnit & (R::kVUnit - 1)) == 0;
+  constexpr int kRowsOn = kWave / R::kVUnit;
+  // where a lane's part of a row begins: K's values and steps, V's unit and its step
+  auto k_part = [&](int quarter) { return T == kKvF16 ? 16 * quarter : T == kKvQ8_0 ? 2 + 8 * quarter : 2 + 4 * quarter; };
+  auto v_part = [&](int e) { return T == kKvF16 ? 16 * e : T == kKvQ8_0 ? 34 * (e / 2) + 2 + 16 * (e & 1) : 18 * e + 2; };
+  auto v_step = [&](int e) { return T == kKvQ8_0 ? 34 * (e / 2) : 18 * e; };
+  const uint32_t krow = (uint32_t)c * (uint32_t)a.k.slot, vrow_off = (uint32_t)(lane / R::kVUnit) * (uint32_t)a.v.slot;
+  const int e0 = lane % R::kVUnit;
+  const uint32_t koff = krow + k_part(g), voff = vrow_off + v_part(e0), vsoff = vrow_off + v_step(e0);
+  auto fetch_k = [&](const uint8_t* row, const uint8_t* part, R& r, int i) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+      __builtin_memcpy(r.k[i][b], __builtin_assume_aligned(part + b * KvRecord<T>::kBytes, 2), 4 * R::kKWords);
+    if constexpr (T != kKvF16) {
+#pragma unroll
+      for (int s = 0; s < R::kS; ++s) r.ks[i][s] = ld_u16(row + KvRecord<T>::kBytes * min(4 * s + g, NB - 1));
+    }
+  };
+  auto fetch_v = [&](const uint8_t* part, const uint8_t* step, R& r, int i) {
+    r.v[i] = *reinterpret_cast<const Bytes16*>(part);
+    if constexpr (T != kKvF16) r.vs[i] = ld_u16(step);
+  };
+  auto opaque_lane = [&] {
+    int x = lane;
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  u32x4 klines[kDense ? R::kLine : 1], vlines[kDense ? R::kLine : 1], rest;
+  auto load = [&](int step, int page, R& r, bool keys, bool values) {
     const int pos = step_position<kStep>(t.range, step);
-    const long long kh = (long long)kvh * a.k.head, vh = (long long)kvh * a.v.head;
-    if (a.whole16) {
+    const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
+    const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
+    if (kDense || a.whole16) {
       const uint8_t *kb[2], *vb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint32_t p = (uint32_t)max(__builtin_amdgcn_readlane(page, 16 * i), 0);
         const uint32_t slot = (uint32_t)(pos + 16 * i) & (uint32_t)(a.seqs.page_size - 1);
-        kb[i] = a.k.data + kh + ((unsigned long long)p * (uint32_t)a.k.page + slot * (uint32_t)a.k.slot);
-        vb[i] = a.v.data + vh + ((unsigned long long)p * (uint32_t)a.v.page + slot * (uint32_t)a.v.slot);
+        kb[i] = kh + ((unsigned long long)p * (uint32_t)a.k.page + slot * (uint32_t)a.k.slot);
+        vb[i] = vh + ((unsigned long long)p * (uint32_t)a.v.page + slot * (uint32_t)a.v.slot);
       }
-      const int ks = (int)a.k.slot, vs = (int)a.v.slot;
+      if constexpr (kDense) {
+        // 16 rows are kHalf lines, the second 16 rows' may lie elsewhere
+        constexpr int kHalf = R::kLines / 2, kWhole = R::kLines - R::kRest;
+        static_assert(R::kRest == 0 || kWhole >= kHalf, "");
+        auto lines = [&](const uint8_t* b0, const uint8_t* b1, u32x4 (&to)[kDense ? R::kLine : 1]) {
+          b1 -= 16 * kHalf;
+#pragma unroll
+          for (int i = 0; i < R::kLine; ++i) {
+            const int n0 = i * kWave, u = n0 + kWave <= kWhole ? n0 + lane : min(n0 + lane, kWhole - 1);
+            const uint8_t* from = n0 + kWave <= kHalf ? b0 : n0 >= kHalf ? b1 : u < kHalf ? b0 : b1;
+            to[i] = *reinterpret_cast<const u32x4*>(from + (uint32_t)(16 * u));
+          }
+        };
+        if (values && R::kRest > 0)
+          rest = *reinterpret_cast<const u32x4*>((lane < 32 ? kb[1] : vb[1]) +
+                                                 (uint32_t)(16 * (kWhole - kHalf + min(lane & 31, R::kRest - 1))));
+        if (keys) lines(kb[0], kb[1], klines);
+        if (values) lines(vb[0], vb[1], vlines);
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
+        if (keys) fetch_k(kb[i] + krow, kb[i] + koff, r, i);
+      }
+      if (!values) return;
+      if constexpr (kSame) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const int off = c * ks + (T == kKvF16 ? 64 * b + 16 * g : T == kKvQ8_0 ? 34 * b + 2 + 8 * g : 18 * b + 2 + 4 * g);
-          __builtin_memcpy(r.k[i][b], __builtin_assume_aligned(kb[i] + off, 2), 4 * R::kKWords);
+        for (int i = 0; i < R::kV; ++i) {
+          const uint8_t* base = vb[i * kRowsOn >= 16 ? 1 : 0] + (uint32_t)(i * kRowsOn & 15) * (uint32_t)a.v.slot;
+          fetch_v(base + voff, base + vsoff, r, i);
         }
-        if constexpr (T != kKvF16) {
+      } else {
+        const int x = opaque_lane();
 #pragma unroll
-          for (int s = 0; s < R::kS; ++s)
-            r.ks[i][s] = ld_u16(kb[i] + c * ks + KvRecord<T>::kBytes * min(4 * s + g, NB - 1));
+        for (int i = 0; i < R::kV; ++i) {
+          const int u = i * kWave + x, key = min(u / R::kVUnit, kStep - 1), e = u % R::kVUnit;
+          const uint8_t* row = (key & 16 ? vb[1] : vb[0]) + (uint32_t)(key & 15) * (uint32_t)a.v.slot;
+          fetch_v(row + v_part(e), row + v_step(e), r, i);
         }
       }
-#pragma unroll
-      for (int i = 0; i < R::kV; ++i) {
-        const int u = i * kWave + lane, key = min(u / R::kVUnit, kStep - 1), e = u % R::kVUnit;
-        const uint8_t* row = (key & 16 ? vb[1] : vb[0]) + (key & 15) * vs;
-        if constexpr (T == kKvF16) {
-          r.v[i] = *reinterpret_cast<const Bytes16*>(row + 16 * e);
-        } else if constexpr (T == kKvQ8_0) {
-          r.v[i] = *reinterpret_cast<const Bytes16*>(row + 34 * (e / 2) + 2 + 16 * (e & 1));
-          r.vs[i] = ld_u16(row + 34 * (e / 2));
-        } else {
-          r.v[i] = *reinterpret_cast<const Bytes16*>(row + 18 * e + 2);
-          r.vs[i] = ld_u16(row + 18 * e);
-        }
-      }
+      asm volatile("; whole groups");  // kept apart: merged with those below, the loads' addresses would all be kept
       return;
     }
     auto slot_of = [&](int at) {
       return a.seqs.page_shift >= 0 ? at & (a.seqs.page_size - 1) : (int)((uint32_t)at % (uint32_t)a.seqs.page_size);
     };
+    const int x = opaque_lane();
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int p = __shfl(page, 16 * i + c, kWave);
-      const uint8_t* row = a.k.data + kh + (long long)max(p, 0) * a.k.page +
-                           (long long)(p < 0 ? 0 : slot_of(pos + 16 * i + c)) * a.k.slot;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int off = T == kKvF16 ? 64 * b + 16 * g : T == kKvQ8_0 ? 34 * b + 2 + 8 * g : 18 * b + 2 + 4 * g;
-        __builtin_memcpy(r.k[i][b], __builtin_assume_aligned(row + off, 2), 4 * R::kKWords);
-      }
-      if constexpr (T != kKvF16) {
-#pragma unroll
-        for (int s = 0; s < R::kS; ++s) r.ks[i][s] = ld_u16(row + KvRecord<T>::kBytes * min(4 * s + g, NB - 1));
-      }
+      const int key = 16 * i + (x & 15), p = __shfl(page, key, kWave);
+      const long long slot = p < 0 ? 0 : slot_of(pos + key);
+      const uint8_t* row = kh + (long long)max(p, 0) * a.k.page + slot * a.k.slot;
+      if (keys) fetch_k(row, row + k_part(g), r, i);
     }
 #pragma unroll
-    for (int i = 0; i < R::kV; ++i) {
-      const int u = i * kWave + lane, key = min(u / R::kVUnit, kStep - 1), e = u % R::kVUnit;
+    for (int i = 0; values && i < R::kV; ++i) {
+      const int u = i * kWave + x, key = min(u / R::kVUnit, kStep - 1), e = u % R::kVUnit;
       const int p = __shfl(page, key, kWave);
-      const uint8_t* row = a.v.data + vh + (long long)max(p, 0) * a.v.page +
-                           (long long)(p < 0 ? 0 : slot_of(pos + key)) * a.v.slot;
-      if constexpr (T == kKvF16) {
-        r.v[i] = *reinterpret_cast<const Bytes16*>(row + 16 * e);
-      } else if constexpr (T == kKvQ8_0) {
-        r.v[i] = *reinterpret_cast<const Bytes16*>(row + 34 * (e / 2) + 2 + 16 * (e & 1));
-        r.vs[i] = ld_u16(row + 34 * (e / 2));
-      } else {
-        r.v[i] = *reinterpret_cast<const Bytes16*>(row + 18 * e + 2);
-        r.vs[i] = ld_u16(row + 18 * e);
-      }
+      const long long slot = p < 0 ? 0 : slot_of(pos + key);
+      const uint8_t* row = vh + (long long)max(p, 0) * a.v.page + slot * a.v.slot;
+      fetch_v(row + v_part(e), row + v_step(e), r, i);
     }
   };
 
+  __syncthreads();
+  // heads up to 128: three waves a SIMD leave no registers for the next step's keys
+  // beside this step's, which are loaded when its scores are done
+  constexpr bool kLate = NB <= 4;
+  // dense: V's lines in LDS; records lie at odd halfwords, but whole words are read
+  // (LDS stalls on others) and shifted
+  constexpr int kVRaw = L::kSteps - kStep * R::kRowBytes;
+  auto word = [&](const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(__builtin_assume_aligned(p, 4)); };
   R raw;
   int step = step0 + wave;
-  int page = pages_of(step), next_page = pages_of(step + kWaves);
-  if (step < step1) load(step, page, raw);
+  int page = page_of(entry_of(step)), next = entry_of(step + kWaves);
+  if (step < step1) load(step, page, raw, true, true);
   for (; step < step1; step += kWaves) {
     const int pos = step_position<kStep>(t.range, step);
     // the keys that are there and that some row sees, key i as bit i
@@ -220,11 +285,90 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
                        (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks);
     const bool masked = mixed || present != 0xffffffffu;
 
+    if constexpr (kDense) {
+      // the lines into the place of the V rows, V's at its end, and out as operands
+      // and units
+      constexpr int kWhole = R::kLines - R::kRest;
+#pragma unroll
+      for (int i = 0; i < R::kLine; ++i) {
+        const int u = i * kWave + lane;
+        if (u < kWhole) {
+          *reinterpret_cast<u32x4*>(vrow + 16 * u) = klines[i];
+          *reinterpret_cast<u32x4*>(vrow + kVRaw + 16 * u) = vlines[i];
+        }
+      }
+      const int z = opaque_lane();
+      if ((z & 31) < R::kRest)
+        *reinterpret_cast<u32x4*>(vrow + (z < 32 ? 0 : kVRaw) + 16 * (kWhole + (z & 31))) = rest;
+      wave_sync();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = (16 * i + c) * R::kRowBytes;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int at = row + b * KvRecord<T>::kBytes + k_part(g);
+          if (R::kRowBytes % 4 == 0 && (b * KvRecord<T>::kBytes + 2) % 4 == 0) {
+#pragma unroll
+            for (int j = 0; j < R::kKWords; ++j) raw.k[i][b][j] = word(vrow + at + 4 * j);
+            continue;
+          }
+          const uint8_t* from = vrow + (at & ~3);
+          uint32_t w[R::kKWords + 1];
+#pragma unroll
+          for (int j = 0; j <= R::kKWords; ++j) w[j] = word(from + 4 * j);
+#pragma unroll
+          for (int j = 0; j < R::kKWords; ++j) raw.k[i][b][j] = __builtin_amdgcn_alignbyte(w[j + 1], w[j], at & 3);
+        }
+#pragma unroll
+        for (int s = 0; s < R::kS; ++s) raw.ks[i][s] = ld_u16(vrow + row + KvRecord<T>::kBytes * min(4 * s + g, NB - 1));
+      }
+    }
+    // a V unit out of the lines
+    auto unit = [&](int i) {
+      if constexpr (kDense) {
+        int row, at, shift;
+        if constexpr (kSame) {  // whole rows on, a multiple of four bytes
+          constexpr int kOn = kRowsOn * R::kRowBytes;
+          static_assert(kOn % 4 == 0, "");
+          const int first = kVRaw + lane / R::kVUnit * R::kRowBytes;
+          row = first + i * kOn;
+          at = ((first + v_part(e0)) & ~3) + i * kOn;
+          shift = (first + v_part(e0)) & 3;
+          row += v_step(e0);
+        } else {
+          const int u = i * kWave + opaque_lane(), key = min(u / R::kVUnit, kStep - 1), e = u % R::kVUnit;
+          row = kVRaw + key * R::kRowBytes;
+          at = (row + v_part(e)) & ~3;
+          shift = (row + v_part(e)) & 3;
+          row += v_step(e);
+        }
+        const uint8_t* from = vrow + at;
+        uint32_t w[5];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) w[j] = word(from + 4 * j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) raw.v[i].w[j] = __builtin_amdgcn_alignbyte(w[j + 1], w[j], shift);
+        raw.vs[i] = ld_u16(vrow + row);
+      }
+    };
+    // The rows overwrite the lines: those of the first 16 keys lie before V's (and
+    // over K's, which are read), so units that come in halves take half the registers.
+    constexpr bool kHalves = kSame && R::kV % 2 == 0;
     // V into LDS rows; a key that no row sees is zeros (its memory may hold anything)
     uint32_t spoiled = 0;  // keys some rows see whose values are not all finite
+    const int x0 = kSame ? lane : opaque_lane();
 #pragma unroll
     for (int i = 0; i < R::kV; ++i) {
-      const int u = i * kWave + lane, key = u / R::kVUnit, e = u % R::kVUnit;
+      if constexpr (kDense) {
+        constexpr int kEach = kHalves ? R::kV / 2 : R::kV;
+        if (i % kEach == 0) {
+#pragma unroll
+          for (int j = 0; j < kEach; ++j) unit(i + j);
+          wave_sync();
+        }
+      }
+      const int u = i * kWave + x0;
+      const int key = kSame ? i * kRowsOn + lane / R::kVUnit : u / R::kVUnit, e = kSame ? e0 : u % R::kVUnit;
       const bool live = R::kVUnit * kStep % kWave == 0 || key < kStep;
       bool zero = masked && !(present >> (key & 31) & 1u);
       if (masked) {
@@ -277,111 +421,129 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
         }
       }
     }
-    // K's steps, times the scale, as [block][key]; K as operands
-    f16x8 kf[2][NB];
+    // K's steps, times the scale, as [block][key]
+    if constexpr (T != kKvF16) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (T != kKvF16) {
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int s = 0; s < R::kS; ++s)
           if (4 * s + g < NB) ksteps[(4 * s + g) * kStep + 16 * i + c] = fp16_to_fp32(raw.ks[i][s]) * a.scale;
-      }
+    }
+    // K as operands
+    auto k_operand = [&](int i, int b) {
+      if constexpr (T == kKvF16) {
+        return __builtin_bit_cast(f16x8, make_uint4(raw.k[i][b][0], raw.k[i][b][1], raw.k[i][b][2], raw.k[i][b][3]));
+      } else {
+        uint32_t w[R::kKWords];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        if constexpr (T == kKvF16) {
-          kf[i][b] = __builtin_bit_cast(f16x8, make_uint4(raw.k[i][b][0], raw.k[i][b][1], raw.k[i][b][2], raw.k[i][b][3]));
-        } else {
-          f16x2 x[4];
-          if constexpr (T == kKvQ8_0) {
-            codes4<128>(raw.k[i][b][0] ^ 0x80808080u, x[0], x[1]);
-            codes4<128>(raw.k[i][b][1] ^ 0x80808080u, x[2], x[3]);
-          } else {
-            codes4<8>(raw.k[i][b][0] & 0x0f0f0f0fu, x[0], x[1]);
-            codes4<8>(raw.k[i][b][0] >> 4 & 0x0f0f0f0fu, x[2], x[3]);
-          }
-          kf[i][b] = f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
+        for (int j = 0; j < R::kKWords; ++j) {
+          w[j] = raw.k[i][b][j];
+          if constexpr (kLate) asm volatile("" : "+v"(w[j]));  // converted where it is used, not all at once before
         }
+        f16x2 x[4];
+        if constexpr (T == kKvQ8_0) {
+          codes4<128>(w[0] ^ 0x80808080u, x[0], x[1]);
+          codes4<128>(w[1] ^ 0x80808080u, x[2], x[3]);
+        } else {
+          codes4<8>(w[0] & 0x0f0f0f0fu, x[0], x[1]);
+          codes4<8>(w[0] >> 4 & 0x0f0f0f0fu, x[2], x[3]);
+        }
+        return f16x8{x[0][0], x[0][1], x[1][0], x[1][1], x[2][0], x[2][1], x[3][0], x[3][1]};
       }
+    };
+    f16x8 kf[2][NB];
+    if constexpr (!kLate) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) kf[i][b] = k_operand(i, b);
     }
     wave_sync();
     // the next step's records are on their way while this one is worked on
-    page = next_page;
-    if (step + kWaves < step1) load(step + kWaves, page, raw);
-    next_page = pages_of(step + 2 * kWaves);
+    page = page_of(next);
+    if (step + kWaves < step1) load(step + kWaves, page, raw, !kLate, true);
+    next = entry_of(step + 2 * kWaves);
 
-    f32x4 s[RT][2] = {};
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
+    // scores: key 16 i + 4 g + e of the lane's query
+    f32x4 s[2] = {};
+    asm volatile("" : "+v"(qoff));  // read at every step: in registers they would halve the waves
+    auto scores = [&](auto two) {  // two: queries of two parts
+      constexpr bool kTwo = decltype(two)::value;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        f32x4 step4;
-        if constexpr (T != kKvF16) step4 = *reinterpret_cast<const f32x4*>(ksteps + b * kStep + 16 * i + 4 * g);
+        const f16x8 qh = *reinterpret_cast<const f16x8*>(qs[0] + qoff + 64 * b);
+        f16x8 ql;
+        if constexpr (kTwo) ql = *reinterpret_cast<const f16x8*>(qs[1] + qoff + 64 * b);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int i = 0; i < 2; ++i) {
+          const f16x8 kx = kLate ? k_operand(i, b) : kf[i][b];
           f32x4 x = {};
-          if constexpr (T == kKvF16) x = s[rt][i];
-          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i][b], qh[rt][b], x, 0, 0, 0);
-          if (!a.half_q) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[i][b], ql[rt][b], x, 0, 0, 0);
+          if constexpr (T == kKvF16) x = s[i];
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, qh, x, 0, 0, 0);
+          if constexpr (kTwo) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kx, ql, x, 0, 0, 0);
           if constexpr (T == kKvF16) {
-            s[rt][i] = x;
+            s[i] = x;
           } else {
+            const f32x4 step4 = *reinterpret_cast<const f32x4*>(ksteps + b * kStep + 16 * i + 4 * g);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[rt][i][e] = fmaf(x[e], step4[e], s[rt][i][e]);
+            for (int e = 0; e < 4; ++e) s[i][e] = fmaf(x[e], step4[e], s[i][e]);
           }
         }
       }
+    };
+    if (a.half_q)
+      scores(std::false_type{});
+    else
+      scores(std::true_type{});
+    if (kLate && step + kWaves < step1) load(step + kWaves, page, raw, true, false);
 
-    f16x8 ph[RT], pl[RT];
+    float x[8];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float x[8];
+    for (int e = 0; e < 8; ++e) {
+      x[e] = s[e / 4][e % 4];
+      if constexpr (T == kKvF16) x[e] *= a.scale;
+    }
+    if (masked) {
+      // value e: key 16 (e / 4) + 4 g + e % 4
+      const uint32_t seen = (uint32_t)seen_bits(a, present, pos, qpos) >> (4 * g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = s[rt][e / 4][e % 4];
-        if constexpr (T == kKvF16) x[e] *= a.scale;
-      }
-      if (masked) {
-        // value e: key 16 (e / 4) + 4 g + e % 4
-        const uint32_t seen = (uint32_t)seen_bits(a, present, pos, qpos[rt]) >> (4 * g);
+      for (int e = 0; e < 8; ++e) x[e] = seen & 1u << (16 * (e / 4) + e % 4) ? x[e] : -INFINITY;
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    top = quarters_max(top);
+    if (__ballot(top > m + kLag)) {
+      const float now = fmaxf(m, top);
+      const float f = now == -INFINITY ? 1.f : exp2_fast(m - now);
+      m = now;
+      l *= f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = seen & 1u << (16 * (e / 4) + e % 4) ? x[e] : -INFINITY;
-      }
-      float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-      top = quarters_max(top);
-      if (__ballot(top > m[rt] + kLag)) {
-        const float now = fmaxf(m[rt], top);
-        const float f = now == -INFINITY ? 1.f : exp2_fast(m[rt] - now);
-        m[rt] = now;
-        l[rt] *= f;
+      for (int v = 0; v < 2 * NB; ++v) o[v] *= f;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    f16x8 ph, pl;
 #pragma unroll
-        for (int v = 0; v < 2 * NB; ++v) o[rt][v] *= f;
-      }
-      const float base = m[rt] == -INFINITY ? 0.f : m[rt];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = exp2_fast(x[e] - base);
-        l[rt] += p;
-        ph[rt][e] = (_Float16)p;
-        if constexpr (T != kKvF16) pl[rt][e] = (_Float16)(p - (float)ph[rt][e]);
-      }
+    for (int e = 0; e < 8; ++e) {
+      const float p = exp2_fast(x[e] - ref);
+      l += p;
+      ph[e] = (_Float16)p;
+      if constexpr (T != kKvF16) pl[e] = (_Float16)(p - (float)ph[e]);
     }
 
     // O^T += V^T P^T
+    const int y = opaque_lane();  // addresses made here: kept, they would be one register too many
+    uint8_t* const vfrom = vrow + (4 * (y >> 4) + (y & 15) / 4) * L::kRow + 8 * (y & 3);
 #pragma unroll
     for (int v = 0; v < 2 * NB; ++v) {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4* LdsPtr;
       // a quarter's lane i: key 4 g + i / 4, values 4 (i % 4) .. of the 16 columns
-      uint8_t* at = vrow + (4 * g + c / 4) * L::kRow + 32 * v + 8 * (c & 3);
+      uint8_t* at = vfrom + 32 * v;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(at + 16 * L::kRow));
       const f16x4 lo4 = __builtin_bit_cast(f16x4, lo), hi4 = __builtin_bit_cast(f16x4, hi);
       const f16x8 vf = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        o[rt][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[rt], o[rt][v], 0, 0, 0);
-        if constexpr (T != kKvF16) o[rt][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[rt], o[rt][v], 0, 0, 0);
-      }
+      o[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[v], 0, 0, 0);
+      if constexpr (T != kKvF16) o[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[v], 0, 0, 0);
     }
     // values that are not finite reach the rows that see their key, and no other
     while (spoiled) {
@@ -391,82 +553,85 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 2 : 1) attend_few_ker
       if (!kv_place(a.seqs, seq, pos + key, pg, slot)) continue;
       const uint8_t* row = a.v.data + (long long)kvh * a.v.head + pg * a.v.page + slot * a.v.slot;
       const int at = 4 * (key / 16) + key % 4;  // among the lane's weights
+      float p = 0.f;
+      f16x8 wh = ph, wl = pl;
+      asm volatile("" : "+v"(wh), "+v"(wl));  // converted here, not beside every step's weights
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float p = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        float w = (float)wh[e];
+        if constexpr (T != kKvF16) w += (float)wl[e];
+        p = e == at ? w : p;
+      }
+      p = __shfl(p, 16 * (key % 16 / 4) + c, kWave);
+      if (seen_bits(a, 1ull, pos + key, qpos)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float w = (float)ph[rt][e];
-          if constexpr (T != kKvF16) w += (float)pl[rt][e];
-          p = e == at ? w : p;
-        }
-        p = __shfl(p, 16 * (key % 16 / 4) + c, kWave);
-        if (seen_bits(a, 1ull, pos + key, qpos[rt])) {
+        for (int v = 0; v < 2 * NB; ++v)
 #pragma unroll
-          for (int v = 0; v < 2 * NB; ++v)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              o[rt][v][e] += p * value_of<T>(row, 16 * v + 4 * g + e);
-              asm volatile("" ::: "memory");  // one value at a time: no registers for this path
-            }
-        }
+          for (int e = 0; e < 4; ++e) {
+            o[v][e] += p * value_of<T>(row, 16 * v + 4 * g + e);
+            asm volatile("" ::: "memory");  // one value at a time: no registers for this path
+          }
       }
     }
     wave_sync();
   }
 
-  // join the waves: sixteen rows at a time through LDS
+  // join the waves through LDS
+  __syncthreads();
+  const float sum = quarters_sum(l);
+  const int last = opaque_lane(), col = last & 15;
+  float* mine = reinterpret_cast<float*>(lds[wave]) + col * L::kORow + last / 16 * 4;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    __syncthreads();
-    const float sum = quarters_sum(l[rt]);
-    float* mine = reinterpret_cast<float*>(lds[wave]) + c * L::kORow;
+  for (int v = 0; v < 2 * NB; ++v) *reinterpret_cast<f32x4*>(mine + 16 * v) = o[v];
+  if (last < 16) ml[wave][col][0] = m, ml[wave][col][1] = sum;
+  __syncthreads();
+  const int row = threadIdx.x / 16;
+  if (row >= t.rows) return;
+  float top = -INFINITY, w[kWaves], all = 0.f;
 #pragma unroll
-    for (int v = 0; v < 2 * NB; ++v) *reinterpret_cast<f32x4*>(mine + 16 * v + 4 * g) = o[rt][v];
-    if (g == 0) ml[wave][c][0] = m[rt], ml[wave][c][1] = sum;
-    __syncthreads();
-    const int row = threadIdx.x / 16;
-    if (16 * rt + row >= t.rows) continue;
-    float top = -INFINITY, w[kWaves], all = 0.f;
+  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[i][row][0]);
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) top = fmaxf(top, ml[i][row][0]);
+  for (int i = 0; i < kWaves; ++i) {
+    w[i] = top == -INFINITY ? 0.f : exp2_fast(ml[i][row][0] - top);
+    all += w[i] * ml[i][row][1];
+  }
+  const int r = t.row0 + row;
+  const float f = !whole ? 1.f : all == 0.f ? 0.f : 1.f / all;  // a row that sees nothing: zeros
+  float* part = nullptr;
+  if (!whole) {
+    part = a.part + ((long long)blockIdx.x * a.splits + split) * 16 * (D + 2) + row * (D + 2);
+    if (threadIdx.x % 16 == 0) part[D] = top, part[D + 1] = all;
+  }
+  uint8_t* dst =
+      a.o + (long long)(t.token0 + r / a.share) * a.o_token + (long long)(kvh * a.share + r % a.share) * a.o_head;
+  for (int e = 4 * (threadIdx.x % 16); e < D; e += 64) {
+    f32x4 x = {};
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      w[i] = top == -INFINITY ? 0.f : exp2_fast(ml[i][row][0] - top);
-      all += w[i] * ml[i][row][1];
-    }
-    const int r = t.row0 + 16 * rt + row;
-    const float f = !whole ? 1.f : all == 0.f ? 0.f : 1.f / all;  // a row that sees nothing: zeros
-    float* part = nullptr;
-    if (!whole) {
-      part = a.part + ((long long)blockIdx.x * a.splits + split) * (16 * RT) * (D + 2) + (16 * rt + row) * (D + 2);
-      if (threadIdx.x % 16 == 0) part[D] = top, part[D + 1] = all;
-    }
-    uint8_t* dst = a.o + (long long)(t.token0 + r / a.share) * a.o_token +
-                   (long long)(kvh * a.share + r % a.share) * a.o_head;
-    for (int e = 4 * (threadIdx.x % 16); e < D; e += 64) {
-      f32x4 x = {};
+    for (int i = 0; i < kWaves; ++i)
+      x += w[i] * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[i]) + row * L::kORow + e);
+    x *= f;
+    if (part != nullptr) {
 #pragma unroll
-      for (int i = 0; i < kWaves; ++i)
-        x += w[i] * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[i]) + row * L::kORow + e);
-      x *= f;
-      if (part != nullptr) {
+      for (int i = 0; i < 4; ++i) part[e + i] = x[i];
+    } else if (a.half_o) {
+      const f16x4 h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+      *reinterpret_cast<Bytes8*>(dst + 2 * e) = __builtin_bit_cast(Bytes8, h);
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) part[e + i] = x[i];
-      } else if (a.half_o) {
-        const f16x4 h = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-        *reinterpret_cast<Bytes8*>(dst + 2 * e) = __builtin_bit_cast(Bytes8, h);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(dst)[e + i] = x[i];
-      }
+      for (int i = 0; i < 4; ++i) reinterpret_cast<float*>(dst)[e + i] = x[i];
     }
   }
 }
 
 template <int T, int NB>
 void launch(const AttendArgs& a, dim3 grid, hipStream_t st) {
-  attend_few_kernel<T, NB, 1><<<grid, kWaves * kWave, 0, st>>>(a);
+  if constexpr (T != kKvF16) {
+    if (a.dense) {
+      attend_few_kernel<T, NB, true><<<grid, kWaves * kWave, 0, st>>>(a);
+      return;
+    }
+  }
+  attend_few_kernel<T, NB, false><<<grid, kWaves * kWave, 0, st>>>(a);
 }
 
 template <int T>

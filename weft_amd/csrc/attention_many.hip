@@ -48,15 +48,14 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   const int c = lane & 31, h = lane >> 5;  // query column (or key, value) and half
   const int kvh = (int)blockIdx.x % a.kv_heads;
   const int split = (int)blockIdx.y;
-  int tile;
   // a causal call's last tiles are its longest: they start first
-  const int seq = find_tile(a, (int)(gridDim.x / a.kv_heads) - 1 - (int)blockIdx.x / a.kv_heads, tile);
   TileRows t;
-  if (seq < 0 || !tile_rows(a, seq, tile, t)) return;
+  if (!locate(a, (int)(gridDim.x / a.kv_heads) - 1 - (int)blockIdx.x / a.kv_heads, -1, 0, t)) return;
+  const int seq = t.seq;
   int step0 = 0, step1 = t.range.steps;
   bool whole = true;
   if (a.part != nullptr) {
-    const int n = split_steps(a);
+    const int n = t.each;
     whole = n >= step1;
     step0 = min(split * n, step1);
     step1 = min(step0 + n, step1);
@@ -93,13 +92,18 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   f32x16 o[NB] = {};
   float m = -INFINITY, l = 0.f;
 
-  // page of a step's key `lane` (of 32: keys twice), -1 where it is absent
-  auto pages_of = [&](int step) {
-    int page = -1, slot;
-    if (step < step1 && !kv_place(a.seqs, seq, step_position<kStep>(t.range, step) + (lane & (kStep - 1)), page, slot))
-      page = -1;
-    return page;
+  // The table's entry for a step's key `lane` (of 32: keys twice), looked up two steps
+  // ahead and not looked at before it is needed: a check here would wait for the
+  // load, and for the records loaded before it.  Past the table its last entry
+  // stands in; no key there is present.
+  auto entry_of = [&](int step) {
+    if (step >= step1) return -1;
+    const uint32_t pos = (uint32_t)(step_position<kStep>(t.range, step) + (lane & (kStep - 1)));
+    const uint32_t entry = a.seqs.page_shift >= 0 ? pos >> a.seqs.page_shift : pos / (uint32_t)a.seqs.page_size;
+    return a.seqs.pages[(long long)seq * a.seqs.pages_row + min(entry, (uint32_t)a.seqs.max_pages - 1)];
   };
+  // -1 where that is no page
+  auto page_of = [&](int entry) { return (uint32_t)entry < (uint32_t)a.seqs.n_pages ? entry : -1; };
   // the keys of a step that are there and that some row of the tile sees
   auto present_of = [&](int pos, int page) {
     unsigned long long present = __ballot(page >= 0);
@@ -116,16 +120,11 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     return a.seqs.page_shift >= 0 ? at & (a.seqs.page_size - 1) : (int)((uint32_t)at % (uint32_t)a.seqs.page_size);
   };
   // a unit of a row: 16 bytes of values or codes, and their step
-  auto fetch = [&](const uint8_t* base, uint32_t off, int e, Bytes16& b, uint32_t& s) {
-    if constexpr (T == kKvF16) {
-      b = *reinterpret_cast<const Bytes16*>(base + (off + 16 * e));
-    } else if constexpr (T == kKvQ8_0) {
-      b = *reinterpret_cast<const Bytes16*>(base + (off + 34 * (e / 2) + 2 + 16 * (e & 1)));
-      s = ld_u16(base + (off + 34 * (e / 2)));
-    } else {
-      b = *reinterpret_cast<const Bytes16*>(base + (off + 18 * e + 2));
-      s = ld_u16(base + (off + 18 * e));
-    }
+  auto part_of = [&](int e) { return T == kKvF16 ? 16 * e : T == kKvQ8_0 ? 34 * (e / 2) + 2 + 16 * (e & 1) : 18 * e + 2; };
+  auto step_of = [&](int e) { return T == kKvQ8_0 ? 34 * (e / 2) : 18 * e; };
+  auto fetch = [&](const uint8_t* part, const uint8_t* step, Bytes16& b, uint32_t& s) {
+    b = *reinterpret_cast<const Bytes16*>(part);
+    if constexpr (T != kKvF16) s = ld_u16(step);
   };
   // Units per row a power of two: unit i of a thread is its unit 0 some whole rows
   // on, in the wave's half of the step, so one offset a thread serves them all.
@@ -139,7 +138,9 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     asm volatile("" : "+v"(x));
     return x;
   };
-  const uint32_t koff = (uint32_t)(key0 & 31) * (uint32_t)a.k.slot, voff = (uint32_t)(key0 & 31) * (uint32_t)a.v.slot;
+  const uint32_t krow = (uint32_t)(key0 & 31) * (uint32_t)a.k.slot, vrow = (uint32_t)(key0 & 31) * (uint32_t)a.v.slot;
+  const uint32_t koff = krow + part_of(e0), voff = vrow + part_of(e0);
+  const uint32_t ksoff = krow + step_of(e0), vsoff = vrow + step_of(e0);
   auto load = [&](int step, int page) {
     const int pos = step_position<kStep>(t.range, step);
     const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
           const uint32_t on = (uint32_t)(i * kOn & 31);
           const uint8_t* kr = (half ? kb[1] : kb[0]) + on * (uint32_t)a.k.slot;
           const uint8_t* vr = (half ? vb[1] : vb[0]) + on * (uint32_t)a.v.slot;
-          fetch(kr, koff, e0, rk[i], sk[i]);
-          fetch(vr, voff, e0, rv[i], sv[i]);
+          fetch(kr + koff, kr + ksoff, rk[i], sk[i]);
+          fetch(vr + voff, vr + vsoff, rv[i], sv[i]);
         }
       } else {
         const int x = opaque_tid();
@@ -173,8 +174,10 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
 #pragma unroll
         for (int i = 0; i < L::kUnits; ++i) {
           const int u = i * kThreads + x, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
-          fetch(kPart > 1 && key & 32 ? kb[1] : kb[0], (key & 31) * ks, e, rk[i], sk[i]);
-          fetch(kPart > 1 && key & 32 ? vb[1] : vb[0], (key & 31) * vs, e, rv[i], sv[i]);
+          const uint8_t* kr = (kPart > 1 && key & 32 ? kb[1] : kb[0]) + (key & 31) * ks;
+          const uint8_t* vr = (kPart > 1 && key & 32 ? vb[1] : vb[0]) + (key & 31) * vs;
+          fetch(kr + part_of(e), kr + step_of(e), rk[i], sk[i]);
+          fetch(vr + part_of(e), vr + step_of(e), rv[i], sv[i]);
         }
       }
       return;
@@ -185,8 +188,10 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       const int u = i * kThreads + x, key = min(u / L::kUnit, kStep - 1), e = u % L::kUnit;
       const int p = __shfl(page, key, kWave);
       const long long slot = p < 0 ? 0 : slot_of(pos + key);
-      fetch(kh + (long long)max(p, 0) * a.k.page + slot * a.k.slot, 0, e, rk[i], sk[i]);
-      fetch(vh + (long long)max(p, 0) * a.v.page + slot * a.v.slot, 0, e, rv[i], sv[i]);
+      const uint8_t* kr = kh + (long long)max(p, 0) * a.k.page + slot * a.k.slot;
+      const uint8_t* vr = vh + (long long)max(p, 0) * a.v.page + slot * a.v.slot;
+      fetch(kr + part_of(e), kr + step_of(e), rk[i], sk[i]);
+      fetch(vr + part_of(e), vr + step_of(e), rv[i], sv[i]);
     }
   };
   // a unit's values, in 16 bits, into a row in LDS
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     }
   };
 
-  int page = pages_of(step0), next_page = pages_of(step0 + 1);
+  int page = page_of(entry_of(step0)), next = entry_of(step0 + 1);
   if (step0 < step1) {
     load(step0, page);
     store(step0, page, 0);
@@ -274,7 +279,9 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     const int buf = (step - step0) & 1;
     const int pos = step_position<kStep>(t.range, step);
     const unsigned long long present = present_of(pos, page);
+    const int next_page = page_of(next);
     if (step + 1 < step1) load(step + 1, next_page);
+    next = entry_of(step + 2);
 
     // rows of this wave see none, different, or all of the step's keys
     const bool none = idle || pos > last_pos ||
@@ -407,7 +414,6 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     }
     page = next_page;
     if (step + 1 < step1) store(step + 1, page, buf ^ 1);
-    next_page = pages_of(step + 2);
     __syncthreads();
   }
 
