@@ -9,7 +9,6 @@
 // file checks calls, chooses tiles and splits, and joins the splits.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "attention.h"
 #include "runtime.h"
@@ -162,7 +161,7 @@ Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
   // them cost 10 % (131072 keys, Q8_0: 70 us at three a CU, 80 at six), as their
   // first steps and joins add up
   const int64_t resident = w.d > 128 ? 1 : p.many || w.type == kKvF16 ? 2 : 3;
-  const int64_t items = (int64_t)p.tiles * w.heads, want = (getenv("W") ? atoi(getenv("W")) : resident) * (int64_t)cu_count();
+  const int64_t items = (int64_t)p.tiles * w.heads, want = resident * (int64_t)cu_count();
   const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + p.step - 1) / p.step;
   p.splits = (int)std::max<int64_t>(
       1, std::min({(want + items - 1) / items, (steps + p.least - 1) / p.least, (int64_t)kMaxSplits}));
