@@ -84,63 +84,6 @@ __device__ __forceinline__ unsigned long long seen_bits(const AttendArgs& a, uns
   return present;
 }
 
-// Steps first .. end - 1 of a tile in which every row sees every key that is
-// there, so that nothing is masked (steps at sinks may be such too; they are few
-// and take the general way).
-struct CleanSteps {
-  int first, end;
-};
-template <int kStep>
-__device__ __forceinline__ CleanSteps clean_steps(const AttendArgs& a, const Range& r, int first_pos, int last_pos) {
-  CleanSteps c;
-  c.first = r.sink_steps;
-  if (a.window > 0) c.first += (max(0, last_pos - a.window + 1 - r.begin) + kStep - 1) / kStep;
-  c.end = r.sink_steps + max(0, min(first_pos + 1, r.end) - r.begin) / kStep;
-  return c;
-}
-
-// Where the rows of the next steps' groups of kGroup keys begin, a group a lane:
-// looked up and multiplied out for many steps at once, because a step that did it
-// alone spent longer in that chain of scalar instructions than in its products.
-// A group that is not there has the pool's first page's address.
-template <int kStep, int kGroup>
-struct Groups {
-  static constexpr int kParts = kStep / kGroup, kSteps = kWave / kParts;  // groups a step, steps held
-  unsigned long long k, v;      // lane: step lane / kParts, part lane % kParts
-  unsigned long long there;     // lanes whose group is there
-  __device__ __forceinline__ void fill(const AttendArgs& a, const Range& r, int seq, int kvh, int step, int stride,
-                                       int end) {
-    const int lane = threadIdx.x & (kWave - 1);
-    const int at = step + lane / kParts * stride;
-    const uint32_t pos = (uint32_t)(step_position<kStep>(r, min(at, end - 1)) + lane % kParts * kGroup);
-    // past the table its last entry stands in: no key there is visible
-    const uint32_t entry = min(pos >> a.seqs.page_shift, (uint32_t)a.seqs.max_pages - 1);
-    const int page = a.seqs.pages[(long long)seq * a.seqs.pages_row + entry];
-    const bool is = (uint32_t)page < (uint32_t)a.seqs.n_pages;
-    const uint32_t p = is ? (uint32_t)page : 0u, slot = pos & (uint32_t)(a.seqs.page_size - 1);
-    k = (unsigned long long)(a.k.data + (long long)kvh * a.k.head) + (unsigned long long)p * (uint32_t)a.k.page +
-        slot * (uint32_t)a.k.slot;
-    v = (unsigned long long)(a.v.data + (long long)kvh * a.v.head) + (unsigned long long)p * (uint32_t)a.v.page +
-        slot * (uint32_t)a.v.slot;
-    there = __ballot(is);
-  }
-  static __device__ __forceinline__ const uint8_t* of(unsigned long long x, int lane) {
-    const uint32_t lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
-    return reinterpret_cast<const uint8_t*>((unsigned long long)hi << 32 | lo);
-  }
-  // the keys of held step n that are there, key i as bit i
-  __device__ __forceinline__ unsigned long long present(int n) const {
-    unsigned long long keys = 0;
-#pragma unroll
-    for (int i = 0; i < 64 / kGroup; ++i)  // steps of fewer than 64 keys: again in the upper half
-      if (there >> (n * kParts + i % kParts) & 1ull) keys |= ((1ull << kGroup) - 1) << (kGroup * i);
-    return keys;
-  }
-  __device__ __forceinline__ bool all(int n) const {
-    return (there >> (n * kParts) & ((1u << kParts) - 1)) == (1u << kParts) - 1;
-  }
-};
-
 // A tile of query rows: its sequence, rows and keys.
 struct TileRows {
   int seq, row0, rows, token0;  // token0: the sequence's first new token

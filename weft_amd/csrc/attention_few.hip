@@ -72,7 +72,7 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 template <int T, int NB, bool kDense>
-__global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB == 4 ? 2 : 3) attend_few_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_kernel(AttendArgs a) {
   using L = Lds<NB>;
   using R = Raw<T, NB, kDense>;
   constexpr int D = 32 * NB;
@@ -98,6 +98,31 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
     if (split > 0 && step0 >= step1) return;
   }
 
+  // The queries into LDS, as right operands: lane (c, g) reads row c's values
+  // 8 g .. 8 g + 7 of a block (Q4_0: 4 g + j and 16 + 4 g + j) as 16 bytes; two
+  // parts of 16 bits where they have 32.
+  for (int i = threadIdx.x; i < 16 * 8 * NB; i += kWaves * kWave) {
+    const int r = i / (8 * NB), e = i % (8 * NB), b = e / 8, four = e % 8;
+    const int row = t.row0 + min(r, t.rows - 1);
+    const int tok = row / a.share, head = kvh * a.share + row % a.share;
+    const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
+    f16x4 hi, lo;
+    if (a.half_q) {
+      hi = __builtin_bit_cast(f16x4, *reinterpret_cast<const Bytes8*>(src + 8 * e)) * (_Float16)a.sign;
+      lo = f16x4{};
+    } else {
+      const float* x = reinterpret_cast<const float*>(src) + 4 * e;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float v = x[j] * a.sign;
+        hi[j] = (_Float16)v;
+        lo[j] = (_Float16)(v - (float)hi[j]);
+      }
+    }
+    uint8_t* dst = qs[0] + r * kQRow + 64 * b + (T != kKvQ4_0 ? 8 * four : four < 4 ? 16 * four : 16 * (four - 4) + 8);
+    *reinterpret_cast<f16x4*>(dst) = hi;
+    *reinterpret_cast<f16x4*>(dst + 16 * kQRow) = lo;
+  }
   int qpos;  // of lane c's row; -1: before the sequence
   {
     const int row = t.row0 + min(c, t.rows - 1);
@@ -113,13 +138,10 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
   uint8_t* const vrow = lds[wave];
   float* const ksteps = reinterpret_cast<float*>(lds[wave] + L::kSteps);
 
-  // Pages of a power of two >= 16 slots: the steps' groups of 16 keys, some steps
-  // held.  Else the table's entry for a step's key `lane` (32 keys), looked up two
-  // steps ahead and not looked at before it is needed: a check would wait for the
+  // The table's entry for a step's key `lane` (32 keys), looked up two steps
+  // ahead and not looked at before it is needed: a check here would wait for the
   // load, and for the records loaded before it.  Past the table its last entry
-  // stands in; no key there is visible.
-  Groups<kStep, 16> groups;
-  int held = step0 + wave;  // the first step that groups has
+  // stands in; no key there is present.
   auto entry_of = [&](int step) {
     if (step >= step1) return -1;
     const uint32_t pos = (uint32_t)(step_position<kStep>(t.range, step) + (lane & 31));
@@ -163,13 +185,17 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
   };
   u32x4 klines[kDense ? R::kLine : 1], vlines[kDense ? R::kLine : 1], rest;
   auto load = [&](int step, int page, R& r, bool keys, bool values) {
+    const int pos = step_position<kStep>(t.range, step);
+    const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
+    const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
     if (kDense || a.whole16) {
       const uint8_t *kb[2], *vb[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int n = (step - held) / kWaves * 2 + i;
-        kb[i] = groups.of(groups.k, n);
-        vb[i] = groups.of(groups.v, n);
+        const uint32_t p = (uint32_t)max(__builtin_amdgcn_readlane(page, 16 * i), 0);
+        const uint32_t slot = (uint32_t)(pos + 16 * i) & (uint32_t)(a.seqs.page_size - 1);
+        kb[i] = kh + ((unsigned long long)p * (uint32_t)a.k.page + slot * (uint32_t)a.k.slot);
+        vb[i] = vh + ((unsigned long long)p * (uint32_t)a.v.page + slot * (uint32_t)a.v.slot);
       }
       if constexpr (kDense) {
         // 16 rows are kHalf lines, the second 16 rows' may lie elsewhere
@@ -214,9 +240,6 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
       asm volatile("; whole groups");  // kept apart: merged with those below, the loads' addresses would all be kept
       return;
     }
-    const int pos = step_position<kStep>(t.range, step);
-    const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
-    const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
     auto slot_of = [&](int at) {
       return a.seqs.page_shift >= 0 ? at & (a.seqs.page_size - 1) : (int)((uint32_t)at % (uint32_t)a.seqs.page_size);
     };
@@ -238,6 +261,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
     }
   };
 
+  __syncthreads();
   // heads up to 128: three waves a SIMD leave no registers for the next step's keys
   // beside this step's, which are loaded when its scores are done
   constexpr bool kLate = NB <= 4;
@@ -246,72 +270,20 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
   constexpr int kVRaw = L::kSteps - kStep * R::kRowBytes;
   auto word = [&](const uint8_t* p) { return *reinterpret_cast<const uint32_t*>(__builtin_assume_aligned(p, 4)); };
   R raw;
-  int step = step0 + wave, next = -1, page = -1;
-  const CleanSteps clean = clean_steps<kStep>(a, t.range, first_pos, last_pos);
-  constexpr bool kGeneral = !kDense;  // the general way is compiled in
-  // what is known of a step when its records are loaded: whether all rows see all
-  // its keys, and else the keys that are there and that some row sees, key i as bit i
-  bool masked = false;
-  uint32_t present = ~0u;
-  auto look_up = [&](int step) {
-    bool all;
-    if (!kGeneral || a.whole16) {
-      if (step - held >= Groups<kStep, 16>::kSteps * kWaves || step == step0 + wave) {
-        held = step;
-        groups.fill(a, t.range, seq, kvh, step, kWaves, step1);
-      }
-      const int n = (step - held) / kWaves;
-      all = groups.all(n);
-      present = all ? ~0u : (uint32_t)groups.present(n);
-    } else {
-      page = page_of(next);
-      next = entry_of(step + kWaves);
-      present = (uint32_t)__ballot(page >= 0);
-      all = present == ~0u;
-    }
-    masked = !all || step < clean.first || step >= clean.end;
-    if (masked) {
-      const int pos = step_position<kStep>(t.range, step);
-      if (pos + kStep > t.range.end) present &= (uint32_t)first_bits(t.range.end - pos);
-      if (a.window > 0 && pos <= first_pos - a.window)
-        present &= (uint32_t)(~first_bits(first_pos - a.window - pos + 1) | first_bits(a.sinks - pos));
-    }
-  };
-  if (step < step1) {
-    if (kGeneral && !a.whole16) next = entry_of(step);
-    look_up(step);
-    load(step, page, raw, true, true);
-  }
-  // The queries into LDS while the first records are on their way, as right operands: lane (c, g) reads row c's values
-  // 8 g .. 8 g + 7 of a block (Q4_0: 4 g + j and 16 + 4 g + j) as 16 bytes; two
-  // parts of 16 bits where they have 32.
-  for (int i = threadIdx.x; i < 16 * 8 * NB; i += kWaves * kWave) {
-    const int r = i / (8 * NB), e = i % (8 * NB), b = e / 8, four = e % 8;
-    const int row = t.row0 + min(r, t.rows - 1);
-    const int tok = row / a.share, head = kvh * a.share + row % a.share;
-    const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
-    f16x4 hi, lo;
-    if (a.half_q) {
-      hi = __builtin_bit_cast(f16x4, *reinterpret_cast<const Bytes8*>(src + 8 * e)) * (_Float16)a.sign;
-      lo = f16x4{};
-    } else {
-      const float* x = reinterpret_cast<const float*>(src) + 4 * e;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float v = x[j] * a.sign;
-        hi[j] = (_Float16)v;
-        lo[j] = (_Float16)(v - (float)hi[j]);
-      }
-    }
-    uint8_t* dst = qs[0] + r * kQRow + 64 * b + (T != kKvQ4_0 ? 8 * four : four < 4 ? 16 * four : 16 * (four - 4) + 8);
-    *reinterpret_cast<f16x4*>(dst) = hi;
-    *reinterpret_cast<f16x4*>(dst + 16 * kQRow) = lo;
-  }
-  __syncthreads();
+  int step = step0 + wave;
+  int page = page_of(entry_of(step)), next = entry_of(step + kWaves);
+  if (step < step1) load(step, page, raw, true, true);
   for (; step < step1; step += kWaves) {
     const int pos = step_position<kStep>(t.range, step);
-    const bool masked_now = masked;
-    const uint32_t present_now = present;
+    // the keys that are there and that some row sees, key i as bit i
+    uint32_t present = (uint32_t)__ballot(page >= 0);
+    if (pos + kStep > t.range.end) present &= (uint32_t)first_bits(t.range.end - pos);
+    if (a.window > 0 && pos <= first_pos - a.window)
+      present &= (uint32_t)(~first_bits(first_pos - a.window - pos + 1) | first_bits(a.sinks - pos));
+    // rows see different keys of this step
+    const bool mixed = pos + kStep - 1 > first_pos ||
+                       (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks);
+    const bool masked = mixed || present != 0xffffffffu;
 
     if constexpr (kDense) {
       // the lines into the place of the V rows, V's at its end, and out as operands
@@ -398,8 +370,8 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
       const int u = i * kWave + x0;
       const int key = kSame ? i * kRowsOn + lane / R::kVUnit : u / R::kVUnit, e = kSame ? e0 : u % R::kVUnit;
       const bool live = R::kVUnit * kStep % kWave == 0 || key < kStep;
-      bool zero = masked_now && !(present_now >> (key & 31) & 1u);
-      if (masked_now) {
+      bool zero = masked && !(present >> (key & 31) & 1u);
+      if (masked) {
         bool bad;
         if constexpr (T == kKvF16) {
           bad = false;
@@ -488,10 +460,9 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
     }
     wave_sync();
     // the next step's records are on their way while this one is worked on
-    if (step + kWaves < step1) {
-      look_up(step + kWaves);
-      load(step + kWaves, page, raw, !kLate, true);
-    }
+    page = page_of(next);
+    if (step + kWaves < step1) load(step + kWaves, page, raw, !kLate, true);
+    next = entry_of(step + 2 * kWaves);
 
     // scores: key 16 i + 4 g + e of the lane's query
     f32x4 s[2] = {};
@@ -532,9 +503,9 @@ __global__ void __launch_bounds__(kWaves* kWave, NB > 4 ? 1 : T == kKvF16 && NB 
       x[e] = s[e / 4][e % 4];
       if constexpr (T == kKvF16) x[e] *= a.scale;
     }
-    if (masked_now) {
+    if (masked) {
       // value e: key 16 (e / 4) + 4 g + e % 4
-      const uint32_t seen = (uint32_t)seen_bits(a, present_now, pos, qpos) >> (4 * g);
+      const uint32_t seen = (uint32_t)seen_bits(a, present, pos, qpos) >> (4 * g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = seen & 1u << (16 * (e / 4) + e % 4) ? x[e] : -INFINITY;
     }

@@ -74,16 +74,29 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   // of the whole tile
   const int first_all = (int)max(-1ll, t.pos0 + t.row0 / a.share);
   const int last_all = (int)max(-1ll, t.pos0 + (t.row0 + t.rows - 1) / a.share);
+  {
+    const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
+    if (a.half_q) {
+#pragma unroll
+      for (int b = 0; b < 2 * NB; ++b)
+        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h)) * (_Float16)a.sign;
+    } else {
+#pragma unroll
+      for (int b = 0; b < 2 * NB; ++b) {
+        const float* x = reinterpret_cast<const float*>(src) + 16 * b + 8 * h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)(x[j] * a.sign);
+      }
+    }
+  }
+
   f32x16 o[NB] = {};
   float m = -INFINITY, l = 0.f;
 
-  // Pages of a power of two >= 32 slots: the steps' groups of 32 keys, some steps
-  // held.  Else the table's entry for a step's key `lane` (of 32: keys twice), looked
-  // up two steps ahead and not looked at before it is needed: a check would wait for
-  // the load, and for the records loaded before it.  Past the table its last entry
-  // stands in; no key there is visible.
-  Groups<kStep, 32> groups;
-  int held = step0;  // the first step that groups has
+  // The table's entry for a step's key `lane` (of 32: keys twice), looked up two steps
+  // ahead and not looked at before it is needed: a check here would wait for the
+  // load, and for the records loaded before it.  Past the table its last entry
+  // stands in; no key there is present.
   auto entry_of = [&](int step) {
     if (step >= step1) return -1;
     const uint32_t pos = (uint32_t)(step_position<kStep>(t.range, step) + (lane & (kStep - 1)));
@@ -92,16 +105,16 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   };
   // -1 where that is no page
   auto page_of = [&](int entry) { return (uint32_t)entry < (uint32_t)a.seqs.n_pages ? entry : -1; };
-  // the keys of a step that some row of the tile sees, of those that are there
-  auto seen_of = [&](int pos, unsigned long long there) {
+  // the keys of a step that are there and that some row of the tile sees
+  auto present_of = [&](int pos, int page) {
+    unsigned long long present = __ballot(page >= 0);
     if (pos + kStep > t.range.end || (a.window > 0 && pos <= first_all - a.window)) {
       unsigned long long seen = first_bits(t.range.end - pos);
       if (a.window > 0) seen &= ~first_bits(first_all - a.window - pos + 1) | first_bits(a.sinks - pos);
-      there &= seen;
+      present &= seen;
     }
-    return there;
+    return present;
   };
-  const CleanSteps clean = clean_steps<kStep>(a, t.range, first_all, last_all);
   Bytes16 rk[L::kUnits], rv[L::kUnits];
   uint32_t sk[L::kUnits], sv[L::kUnits];
   auto slot_of = [&](int at) {
@@ -130,13 +143,18 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   const uint32_t koff = krow + part_of(e0), voff = vrow + part_of(e0);
   const uint32_t ksoff = krow + step_of(e0), vsoff = vrow + step_of(e0);
   auto load = [&](int step, int page) {
+    const int pos = step_position<kStep>(t.range, step);
+    const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
+    const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
     if (a.whole32) {
+      // 32 keys lie in one page
       const uint8_t *kb[2], *vb[2];
 #pragma unroll
       for (int i = 0; i < kPart; ++i) {
-        const int n = (step - held) * kPart + i;
-        kb[i] = groups.of(groups.k, n);
-        vb[i] = groups.of(groups.v, n);
+        const uint32_t p = (uint32_t)max(__builtin_amdgcn_readlane(page, 32 * i), 0);
+        const uint32_t slot = (uint32_t)(pos + 32 * i) & (uint32_t)(a.seqs.page_size - 1);
+        kb[i] = kh + ((unsigned long long)p * (uint32_t)a.k.page + slot * (uint32_t)a.k.slot);
+        vb[i] = vh + ((unsigned long long)p * (uint32_t)a.v.page + slot * (uint32_t)a.v.slot);
       }
       if constexpr (kSame) {
 #pragma unroll
@@ -163,12 +181,8 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
           fetch(vr + part_of(e), vr + step_of(e), rv[i], sv[i]);
         }
       }
-      asm volatile("; whole groups");  // kept apart: merged with those below, the loads' addresses would all be kept
       return;
     }
-    const int pos = step_position<kStep>(t.range, step);
-    const uint8_t* kh = a.k.data + (long long)kvh * a.k.head;
-    const uint8_t* vh = a.v.data + (long long)kvh * a.v.head;
     const int x = opaque_tid();
 #pragma unroll
     for (int i = 0; i < L::kUnits; ++i) {
@@ -212,10 +226,17 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       }
     }
   };
-  // the loaded step into LDS buffer `buf`; V of a key that no row sees is zeros.
-  // edge: the tile's rows see different keys of it, or not all
-  auto store = [&](bool edge, unsigned long long present, int buf) {
+  // a step in which the tile's rows see different keys, or not all of them
+  auto is_edge = [&](int pos, unsigned long long present) {
+    return pos + kStep - 1 > first_all || (a.window > 0 && pos <= last_all - a.window && pos + kStep - 1 >= a.sinks) ||
+           present != ~0ull;
+  };
+  // the loaded step into LDS buffer `buf`; V of a key that no row sees is zeros
+  auto store = [&](int step, int page, int buf) {
     const int x = kSame ? tid : opaque_tid();
+    const int pos = step_position<kStep>(t.range, step);
+    const unsigned long long present = present_of(pos, page);
+    const bool edge = is_edge(pos, present);
     uint8_t* base = lds + buf * L::kBytes;
     unsigned long long spoiled = 0;
 #pragma unroll
@@ -249,64 +270,25 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     }
   };
 
-  // what is known of a step when it is loaded: whether it is an edge, and its keys
-  auto is_edge = [&](int step, bool all) { return !all || step < clean.first || step >= clean.end; };
-  int next = -1, page = -1;
-  bool edge = false;
-  unsigned long long present = ~0ull;
-  auto look_up = [&](int step) {  // and load
-    bool all;
-    if (a.whole32) {
-      if (step - held >= Groups<kStep, 32>::kSteps || step == step0) {
-        held = step;
-        groups.fill(a, t.range, seq, kvh, step, 1, step1);
-      }
-      all = groups.all(step - held);
-      if (!all || is_edge(step, all)) present = groups.present(step - held);
-    } else {
-      page = page_of(next);
-      present = __ballot(page >= 0);
-      all = present == ~0ull;
-    }
-    load(step, page);
-    if (!a.whole32) next = entry_of(step + 1);
-    edge = is_edge(step, all);
-    if (edge) present = seen_of(step_position<kStep>(t.range, step), present);
-  };
-  if (!a.whole32) next = entry_of(step0);
-  if (step0 < step1) look_up(step0);
-  {
-    const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
-    if (a.half_q) {
-#pragma unroll
-      for (int b = 0; b < 2 * NB; ++b)
-        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h)) * (_Float16)a.sign;
-    } else {
-#pragma unroll
-      for (int b = 0; b < 2 * NB; ++b) {
-        const float* x = reinterpret_cast<const float*>(src) + 16 * b + 8 * h;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)(x[j] * a.sign);
-      }
-    }
+  int page = page_of(entry_of(step0)), next = entry_of(step0 + 1);
+  if (step0 < step1) {
+    load(step0, page);
+    store(step0, page, 0);
   }
-  if (step0 < step1) store(edge, present, 0);
   __syncthreads();
   for (int step = step0; step < step1; ++step) {
     const int buf = (step - step0) & 1;
-    const bool edge_now = edge;
-    const unsigned long long present_now = present;
-    if (step + 1 < step1) look_up(step + 1);
+    const int pos = step_position<kStep>(t.range, step);
+    const unsigned long long present = present_of(pos, page);
+    const int next_page = page_of(next);
+    if (step + 1 < step1) load(step + 1, next_page);
+    next = entry_of(step + 2);
 
     // rows of this wave see none, different, or all of the step's keys
-    const int pos = step_position<kStep>(t.range, step);
-    bool none = idle, masked = false;
-    if (edge_now) {
-      none = idle || pos > last_pos ||
-             (a.window > 0 && pos + kStep - 1 <= first_pos - a.window && pos >= a.sinks);
-      masked = pos + kStep - 1 > first_pos ||
-               (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks) || present_now != ~0ull;
-    }
+    const bool none = idle || pos > last_pos ||
+                      (a.window > 0 && pos + kStep - 1 <= first_pos - a.window && pos >= a.sinks);
+    const bool masked = pos + kStep - 1 > first_pos ||
+                        (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks) || present != ~0ull;
     if (!none) {
       const uint8_t* base = lds + buf * L::kBytes;
       f32x16 s[kPart] = {};
@@ -333,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       float top;
       if (masked) {
         // value e of half i: key 32 i + 8 (e / 4) + 4 h + e % 4
-        const unsigned long long seen = seen_bits(a, present_now, pos, qpos) >> (4 * h);
+        const unsigned long long seen = seen_bits(a, present, pos, qpos) >> (4 * h);
         top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kPart; ++i) {
@@ -398,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
           if (n % 2) __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (edge_now) {
+      if (is_edge(pos, present)) {
         // values that are not finite reach the rows that see their key, and no other
         unsigned long long spoiled = 0;
 #pragma unroll
@@ -431,7 +413,8 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         }
       }
     }
-    if (step + 1 < step1) store(edge, present, buf ^ 1);
+    page = next_page;
+    if (step + 1 < step1) store(step + 1, page, buf ^ 1);
     __syncthreads();
   }
 
