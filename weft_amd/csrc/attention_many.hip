@@ -295,6 +295,8 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       // operands come two blocks ahead of their products; the barriers keep the
       // scheduler from fetching them all at once, which the registers would not hold
       constexpr int kAhead = 2;
+      // the SIMD's other wave gets what the products leave: its softmax or its loads
+      __builtin_amdgcn_s_setprio(1);
       f16x8 kf[kAhead][kPart];
       auto k_at = [&](int b, int i) {
         return *reinterpret_cast<const f16x8*>(base + (32 * i + c) * L::kKRow + 32 * b + 16 * h);
@@ -312,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       float top;
       if (masked) {
         // value e of half i: key 32 i + 8 (e / 4) + 4 h + e % 4
@@ -348,16 +351,17 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       }
       const float ref = m == -INFINITY ? 0.f : m;
       f16x8 p[2 * kPart];
+      auto weigh = [&](int k, int from, int to) {  // weights [from, to) of p[k]
 #pragma unroll
-      for (int i = 0; i < kPart; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float w = exp2_fast(fmaf(s[i][e], a.scale, -ref));
+        for (int e = from; e < to; ++e) {
+          const float w = exp2_fast(fmaf(s[k / 2][8 * (k & 1) + e], a.scale, -ref));
           l += w;
-          p[2 * i + e / 8][e % 8] = (_Float16)w;
+          p[k][e] = (_Float16)w;
         }
-      asm volatile("" : "+v"(l));  // summed here: 32 weights more in registers would not fit
-      // O^T += V^T P^T: 16 keys a product, four of a quarter's and four 8 on
+      };
+      weigh(0, 0, 8);
+      // O^T += V^T P^T: 16 keys a product, four of a quarter's and four 8 on; the next
+      // products' weights are computed while these run
       {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4* LdsPtr;
@@ -377,8 +381,11 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         for (int n = 0; n < 2 * kPart * NB; ++n) {
           o[n % NB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[n % kAheadV], p[n / NB], o[n % NB], 0, 0, 0);
           if (n + kAheadV < 2 * kPart * NB) vf[n % kAheadV] = v_at(n + kAheadV);
-          if (n % 2) __builtin_amdgcn_sched_barrier(0);
+          const int k = n / NB + 1, v = n % NB;
+          if (k < 2 * kPart) weigh(k, 4 * v / NB * 2, 4 * (v + 1) / NB * 2);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        asm volatile("" : "+v"(l));  // summed here: 32 weights more in registers would not fit
       }
       if (is_edge(pos, present)) {
         // values that are not finite reach the rows that see their key, and no other
