@@ -76,6 +76,17 @@ def test_head_sizes_and_shared_heads(hip, kind, d, share):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_chunks_over_pages_of_whole_lines(hip, kind, d, page):
+    """Pages of a power of two slots that follow each other, every head size, and
+    the same with heads between the slots."""
+    for slots_first in (False, True):
+        check(hip, kind, [301, 77], [140, 77], page, 2, 4, d, slots_first=slots_first, seed=d + page)
+        check(hip, kind, [301, 77], [140, 77], page, 2, 4, d, 50, 3, slots_first=slots_first, seed=d + page)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("news", [2, 4, 5, 16, 17, 31, 32, 33, 63, 64, 65, 130])
 def test_chunks_of_every_size(hip, kind, news):
     for before in (0, 1, 97):
