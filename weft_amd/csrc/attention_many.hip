@@ -4,7 +4,7 @@
 // partly overlap: a prompt of 4096 16-bit tokens, 32 heads over 8 of 128 values,
 // takes 170 to 183 us (0.75 to 0.81 PFLOP/s; the matrix pipe is busy for 55 us of
 // it, the vector unit for 66); 512 tokens of 64 heads of 64 in a window of 4096
-// behind 32768 Q8_0 keys 78 us (0.44 PFLOP/s); a batch of nine chunks over 3000
+// behind 32768 Q8_0 keys 73 us with the join (0.47 PFLOP/s); a batch of nine chunks over 3000
 // Q4_0 keys with no shared heads 115 us (0.36 PFLOP/s: the longest tile's 47 steps,
 // of which each converts its records for 128 rows only).
 //
