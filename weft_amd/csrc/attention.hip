@@ -180,8 +180,10 @@ Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
   const int64_t resident = w.d > 128 ? 1 : p.many || w.type == kKvF16 ? 2 : 3;
   const int64_t items = (int64_t)p.tiles * w.heads, want = resident * (int64_t)cu_count();
   const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + p.step - 1) / p.step;
-  p.splits = (int)std::max<int64_t>(
-      1, std::min({(want + items - 1) / items, (steps + p.least - 1) / p.least, (int64_t)kMaxSplits}));
+  // two steps a wave cost less than a second launch that joins (one token, 256 keys:
+  // 9.5 us in one split, 11.6 in two; 512 keys: 14.0 and 11.6)
+  const int64_t most = !p.many && steps <= 2 * p.least ? 1 : (steps + p.least - 1) / p.least;
+  p.splits = (int)std::max<int64_t>(1, std::min({(want + items - 1) / items, most, (int64_t)kMaxSplits}));
   p.work = p.splits == 1 ? 0 : (size_t)items * p.splits * p.tile * (w.d + 2) * sizeof(float);
   return p;
 }
