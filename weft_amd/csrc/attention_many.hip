@@ -84,24 +84,33 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   // of the whole tile
   const int first_all = (int)max(-1ll, t.pos0 + t.row0 / a.share);
   const int last_all = (int)max(-1ll, t.pos0 + (t.row0 + t.rows - 1) / a.share);
+  // The scale (at most 1: queries stay in range) goes into the queries, and the scores'
+  // products begin at minus the row's reference, so that they end as the weights'
+  // exponents
+  const bool folded = a.scale <= 1.f;
   {
+    const float qscale = folded ? a.sign * a.scale : a.sign;
     const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
     if (a.half_q) {
 #pragma unroll
-      for (int b = 0; b < 2 * NB; ++b)
-        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h)) * (_Float16)a.sign;
+      for (int b = 0; b < 2 * NB; ++b) {
+        const f16x8 x = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)((float)x[j] * qscale);
+      }
     } else {
 #pragma unroll
       for (int b = 0; b < 2 * NB; ++b) {
         const float* x = reinterpret_cast<const float*>(src) + 16 * b + 8 * h;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)(x[j] * a.sign);
+        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)(x[j] * qscale);
       }
     }
   }
 
   f32x16 o[NB] = {};
   float m = -INFINITY, l = 0.f;
+  f32x16 minus = {};  // the reference, negative, in every place
 
   // The table's entry for a step's key `lane` (of 32: keys twice), looked up two steps
   // ahead and not looked at before it is needed: a check here would wait for the
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
                         (a.window > 0 && pos <= last_pos - a.window && pos + kStep - 1 >= a.sinks) || present != ~0ull;
     if (!none) {
       const uint8_t* base = lds + buf * L::kBytes;
-      f32x16 s[kPart] = {};
+      f32x16 s[kPart];
       // operands come two blocks ahead of their products; the barriers keep the
       // scheduler from fetching them all at once, which the registers would not hold
       constexpr int kAhead = 2;
@@ -319,12 +328,19 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       for (int b = 0; b < 2 * NB; ++b) {
 #pragma unroll
         for (int i = 0; i < kPart; ++i) {
-          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b % kAhead][i], qf[b], s[i], 0, 0, 0);
+          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[b % kAhead][i], qf[b], b == 0 ? minus : s[i], 0, 0, 0);
           if (b + kAhead < 2 * NB) kf[b % kAhead][i] = k_at(b + kAhead, i);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
+      const float ref0 = m == -INFINITY ? 0.f : m;
+      if (!folded) {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e] = fmaf(s[i][e], a.scale, -ref0);
+      }
       float top;
       if (masked) {
         // value e of half i: key 32 i + 8 (e / 4) + 4 h + e % 4
@@ -349,22 +365,30 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       {
         typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
         const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * a.scale;  // a.scale > 0
+        top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
       }
-      if (__ballot(top > m + kLag)) {
-        const float now = fmaxf(m, top);
+      if (__ballot(top + ref0 > m + kLag)) {
+        const float now = fmaxf(m, top + ref0);
         const float f = now == -INFINITY ? 1.f : exp2_fast(m - now);
         m = now;
         l *= f;
 #pragma unroll
         for (int v = 0; v < NB; ++v) o[v] *= f;
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < kPart; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e] += ref0 - ref;
+        if (folded) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) minus[e] = -ref;
+        }
       }
-      const float ref = m == -INFINITY ? 0.f : m;
       f16x8 p[2 * kPart];
       auto weigh = [&](int k, int from, int to) {  // weights [from, to) of p[k]
 #pragma unroll
         for (int e = from; e < to; ++e) {
-          const float w = exp2_fast(fmaf(s[k / 2][8 * (k & 1) + e], a.scale, -ref));
+          const float w = exp2_fast(s[k / 2][8 * (k & 1) + e]);
           l += w;
           p[k][e] = (_Float16)w;
         }
