@@ -1,12 +1,13 @@
 // Attention of many query rows a kv head: prompts and chunks.
 //
-// Bound by the matrix pipe and the softmax beside it, which two waves a SIMD only
-// partly overlap: a prompt of 4096 16-bit tokens, 32 heads over 8 of 128 values,
-// takes 170 to 183 us (0.75 to 0.81 PFLOP/s; the matrix pipe is busy for 55 us of
-// it, the vector unit for 66); 512 tokens of 64 heads of 64 in a window of 4096
-// behind 32768 Q8_0 keys 73 us with the join (0.47 PFLOP/s); a batch of nine chunks over 3000
-// Q4_0 keys with no shared heads 115 us (0.36 PFLOP/s: the longest tile's 47 steps,
-// of which each converts its records for 128 rows only).
+// Bound by the matrix pipe and the softmax beside it, which two waves a SIMD overlap
+// in part only: a prompt of 4096 16-bit tokens, 32 heads over 8 of 128 values, takes
+// 170 to 185 us (0.74 to 0.81 PFLOP/s; the matrix pipe is busy for 35 % of it, the
+// vector unit for 36 %, a quarter of a wave's time waits for records or the step's
+// barrier); 512 tokens of 64 heads of 64 in a window of 4096 behind 32768 Q8_0 keys
+// 71 to 79 us with the join (0.44 to 0.48 PFLOP/s); nine chunks of up to 640 tokens
+// over up to 3001 Q4_0 keys with no shared heads 111 to 114 us (0.37 PFLOP/s: the
+// longest tile's 47 steps; each workgroup converts the records for its 128 rows only).
 //
 // A workgroup owns 128 rows,
 // 32 a wave, and walks the keys in steps of 64 (heads of 256: 32, for the
@@ -84,20 +85,17 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   // of the whole tile
   const int first_all = (int)max(-1ll, t.pos0 + t.row0 / a.share);
   const int last_all = (int)max(-1ll, t.pos0 + (t.row0 + t.rows - 1) / a.share);
-  // The scale (at most 1: queries stay in range) goes into the queries, and the scores'
-  // products begin at minus the row's reference, so that they end as the weights'
-  // exponents
-  const bool folded = a.scale <= 1.f;
+  // The scale (at most 1: queries stay in range) goes into queries that are rounded
+  // here anyway, and the scores' products begin at minus the row's reference, so that
+  // they end as the weights' exponents.  16-bit queries stay exact.
+  const bool folded = a.scale <= 1.f && !a.half_q;
   {
     const float qscale = folded ? a.sign * a.scale : a.sign;
     const uint8_t* src = a.q + (long long)(t.token0 + tok) * a.q_token + (long long)head * a.q_head;
     if (a.half_q) {
 #pragma unroll
-      for (int b = 0; b < 2 * NB; ++b) {
-        const f16x8 x = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) qf[b][j] = (_Float16)((float)x[j] * qscale);
-      }
+      for (int b = 0; b < 2 * NB; ++b)
+        qf[b] = __builtin_bit_cast(f16x8, *reinterpret_cast<const Bytes16*>(src + 32 * b + 16 * h)) * (_Float16)a.sign;
     } else {
 #pragma unroll
       for (int b = 0; b < 2 * NB; ++b) {
