@@ -118,6 +118,22 @@ def test_strides_and_types(hip):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.125, 1.0), (1e-6, 1.0), (0.69, 0.2), (0.7, 0.2), (3.0, 0.05),
+                                          (-3.0, 0.05), (1000.0, 1e-4)])
+def test_scales(hip, kind, scale, spread):
+    """Zero, negative, tiny and large ones (past what queries of 16 bits could take)."""
+    for news in (1, 70):
+        for src in ("f32", "f16"):
+            cache = Cache(hip, kind, [150], [news], 16, 2, 64, seed=21)
+            q = np.random.default_rng(22).standard_normal((news, 8, 64)) * spread
+            q = q.astype(np.float16 if src == "f16" else np.float32).astype(np.float32)
+            print(f"attention {kind} scale={scale} news={news} {src}", flush=True)
+            got = call(hip, cache, q, scale, src=src)
+            want, mass, reach = attend(cache, q, scale)
+            assert not (np.abs(got - want) > attention_bound(mass, np.abs(reach), want, False)).any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_rows_that_see_nothing(hip, kind):
     """Lengths of zero and shorter than the new tokens, sequences without new
     tokens, and queries whose every visible page was given back."""
