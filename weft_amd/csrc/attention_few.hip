@@ -1,7 +1,7 @@
 // Attention of few query rows a kv head: decode steps and short chunks.
 //
 // Bound by reading the cache, 4-bit codes by converting them beside that: 48
-// sequences of up to 8192 Q8_0 tokens, 32 heads over 8 of 128 values, take 127 us
+// sequences of up to 8192 Q8_0 tokens, 32 heads over 8 of 128 values, take 125 us
 // (4.0 TB/s); one of 131072 Q4_0 tokens 52 us (2.9 TB/s, about 450 VALU
 // instructions a wave and step, 65 % of the busy cycles); 1023 Q8_0 tokens 11.8 us
 // with the join, both launches and a dozen dependent trips to memory.
@@ -60,6 +60,14 @@ struct Raw {
   Bytes16 v[kV];
   uint32_t vs[T == kKvF16 ? 1 : kV];
 };
+
+// A line of records, read once a tile, which the caches need not keep: one token
+// over 131072 Q8_0 keys takes 66 us instead of 70, 48 over up to 8192 124 instead of
+// 125; 32 heads over one kv head, two tiles on the same lines, 26.5 instead of 25.9.
+// (16-bit rows are not whole lines a load: eight chunks of 8 tokens would take 76 us instead of 64.)
+__device__ __forceinline__ u32x4 once(const uint8_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+}
 
 // a wave's place in LDS: V rows (padded by 32 bytes, so that eight rows of 32
 // bytes fall on different banks), K's steps; O at the end lies over them
@@ -215,12 +223,11 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
           for (int i = 0; i < R::kLine; ++i) {
             const int n0 = i * kWave, u = n0 + kWave <= kWhole ? n0 + lane : min(n0 + lane, kWhole - 1);
             const uint8_t* from = n0 + kWave <= kHalf ? b0 : n0 >= kHalf ? b1 : u < kHalf ? b0 : b1;
-            to[i] = *reinterpret_cast<const u32x4*>(from + (uint32_t)(16 * u));
+            to[i] = once(from + (uint32_t)(16 * u));
           }
         };
         if (values && R::kRest > 0)
-          rest = *reinterpret_cast<const u32x4*>((lane < 32 ? kb[1] : vb[1]) +
-                                                 (uint32_t)(16 * (kWhole - kHalf + min(lane & 31, R::kRest - 1))));
+          rest = once((lane < 32 ? kb[1] : vb[1]) + (uint32_t)(16 * (kWhole - kHalf + min(lane & 31, R::kRest - 1))));
         if (keys) lines(kb[0], kb[1], klines);
         if (values) lines(vb[0], vb[1], vlines);
         return;
