@@ -11,7 +11,7 @@
 // consecutive groups of four (write) or eight (read) values, keys and values
 // in one launch.  Writing 5500 tokens of 8 heads of 128 F32 values as Q4_0 takes
 // 17 us (3.0 TB/s); reading 32 sequences of up to 16384 Q8_0 tokens into F16
-// 580 us (5.0 TB/s, the zeros past their lengths with them); one token 3.3 us, and
+// 545 us (5.3 TB/s, the zeros past their lengths with them); one token 3.3 us, and
 // 131 tokens back 4.7 us: launches and the dependent loads of a row's place.
 #include <limits.h>
 
@@ -185,7 +185,10 @@ __device__ __forceinline__ void values8(const Bytes16& b, int part, uint32_t ste
 // blockIdx.x: kReadTokens positions, blockIdx.y: sequence, blockIdx.z: keys or
 // values; zeros where the sequence has no value.  The positions' rows are looked
 // up once; then a thread has four groups of eight values in flight, and a wave
-// writes 1 KiB of F16 in one store.
+// writes 1 KiB of F16 in one store, past the caches: 32 sequences of up to 16384
+// tokens take 545 us so and 584 through them, four of up to 8192 31 and 45.
+typedef _Float16 half8 __attribute__((ext_vector_type(8), aligned(2)));
+typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kReadTokens = 8;
 template <int T, bool kHalfOut>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvSeqs seqs, KvPool k, KvPool v, Rows ko, Rows vo,
@@ -231,13 +234,12 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvSeqs seqs, KvPool k
       float x[8] = {};
       if (there[u]) values8<T>(b[u], part[u], step[u], x);
       if constexpr (kHalfOut) {
-        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
         const half8 y = {(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3],
                          (_Float16)x[4], (_Float16)x[5], (_Float16)x[6], (_Float16)x[7]};
-        *reinterpret_cast<Bytes16*>(to[u]) = __builtin_bit_cast(Bytes16, y);
+        __builtin_nontemporal_store(y, reinterpret_cast<half8*>(to[u]));
       } else {
-        *reinterpret_cast<Floats4*>(to[u]) = Floats4{{x[0], x[1], x[2], x[3]}};
-        *reinterpret_cast<Floats4*>(to[u] + 16) = Floats4{{x[4], x[5], x[6], x[7]}};
+        __builtin_nontemporal_store(float4u{x[0], x[1], x[2], x[3]}, reinterpret_cast<float4u*>(to[u]));
+        __builtin_nontemporal_store(float4u{x[4], x[5], x[6], x[7]}, reinterpret_cast<float4u*>(to[u] + 16));
       }
     }
   }
