@@ -370,7 +370,8 @@ int weft_ggml_add_rms_norm(const weft_ggml_tensor *x, const weft_ggml_tensor *re
 
 /* A batch of sequences over a paged cache.  Sequence s has new tokens
  * starts[s] .. starts[s+1] - 1 of the call's token rows (in order; none is
- * fine), they are its last ones, and it is lengths[s] tokens long with them;
+ * fine; a start below one before it counts as that one, one past the rows as
+ * their number), they are its last ones, and it is lengths[s] tokens long with them;
  * its token at position p is in page pages[s][p / page size].  An entry that is
  * no page of the pool (-1) makes its positions absent. */
 typedef struct weft_ggml_kv_batch {

@@ -101,6 +101,14 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive
   v += dpp<kDppBcast15, 0xA>(v);
   return v + dpp<kDppBcast31, 0xC>(v);
 }
+__device__ __forceinline__ int wave_scan_max(int v) {  // inclusive, of values >= 0
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = max(v, dpp<kDppBcast15, 0xA>(v));
+  return max(v, dpp<kDppBcast31, 0xC>(v));
+}
 __device__ __forceinline__ int wave_max_count(int v) {  // of values >= 0
   v = max(v, dpp<kDppXor1>(v));
   v = max(v, dpp<kDppXor2>(v));
@@ -116,18 +124,24 @@ __device__ __forceinline__ int wave_max_count(int v) {  // of values >= 0
 // Also the steps a split takes: the longest sequence's over the most splits, the
 // same for every tile, so that a batch of uneven sequences makes splits of even
 // work.  The whole wave calls it; 64 sequences are looked at at once, so a call's
-// starts and lengths cost one trip to memory.
+// starts and lengths cost one trip to memory.  A start below one before it counts as
+// that one, so no row is in two sequences and a call has no more tiles than the host
+// planned for.
 __device__ __forceinline__ bool locate(const AttendArgs& a, int tile, int token, int head, TileRows& t) {
   const int lane = threadIdx.x & (kWave - 1);
-  int longest = 0, before = 0, found = -1, first = 0, n = 0, in = 0;
+  int longest = 0, before = 0, found = -1, first = 0, n = 0, in = 0, reached = 0;
   long long len = 0;
   for (int i = 0; i < a.seqs.n_seqs; i += kWave) {
-    int f = 0, count = 0, length = 0;
+    int f = 0, end = 0, length = 0;
     if (i + lane < a.seqs.n_seqs) {
       f = max(0, min(a.seqs.starts[i + lane], a.seqs.n_tokens));
-      count = max(0, max(0, min(a.seqs.starts[i + lane + 1], a.seqs.n_tokens)) - f);
+      end = max(0, min(a.seqs.starts[i + lane + 1], a.seqs.n_tokens));
       length = a.seqs.lengths[i + lane];
     }
+    f = max(reached, wave_scan_max(f));
+    end = max(f, end);  // past the last sequence: no rows
+    reached = __builtin_amdgcn_readlane(end, kWave - 1);
+    const int count = end - f;
     int steps = 0;
     if (count > 0) steps = visible_range(a, (long long)length - count, (long long)length - 1).steps;
     longest = max(longest, wave_max_count(steps));
