@@ -64,23 +64,26 @@ __device__ __forceinline__ bool kv_place(const KvSeqs& s, int seq, int pos, int&
 }
 
 // The sequence that new token t (wave-uniform) belongs to, -1 for none; the
-// whole wave calls it, 64 starts a step.
+// whole wave calls it, 64 starts a step.  Starts count as in the attention: one below
+// one before it as that one, so t's is the first sequence that ends past it.
 __device__ __forceinline__ int kv_sequence_of(const KvSeqs& s, int t) {
   const int lane = threadIdx.x & (kWave - 1);
   int n = 0;
   for (int i = 0; i < s.n_seqs; i += kWave) {
     const bool past = i + lane < s.n_seqs && s.starts[i + lane + 1] <= t;
-    n += __popcll(__ballot(past));
+    const unsigned long long left = ~__ballot(past);
+    n += left ? __builtin_ctzll(left) : kWave;
+    if (left) break;
   }
-  if (n >= s.n_seqs || s.starts[n] > t) return -1;
+  if (n >= s.n_seqs || s.starts[0] > t) return -1;
   return n;
 }
 
-// Position of new token t of sequence seq: its new tokens are its last ones.
-// Negative where a length is shorter than the new tokens; past the table where
-// a length says so (kv_place refuses it).
+// Position of new token t of its sequence: its new tokens are its last ones, those
+// past the call's rows left out.  Negative where a length is shorter than the new
+// tokens; past the table where a length says so (kv_place refuses it).
 __device__ __forceinline__ long long kv_position(const KvSeqs& s, int seq, int t) {
-  return (long long)s.lengths[seq] - s.starts[seq + 1] + t;
+  return (long long)s.lengths[seq] - min(s.starts[seq + 1], s.n_tokens) + t;
 }
 
 // ---------------------------------------------------------------- host side
