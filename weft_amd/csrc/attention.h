@@ -20,6 +20,7 @@ struct AttendArgs {
   float* part;  // the splits' partial results, nullptr where none are made
   long long q_head, q_token, o_head, o_token;  // byte strides
   int share, kv_heads, window, sinks;
+  int first, items;  // this launch's first (tile, kv head) and all of the call's
   int tile;        // rows a tile
   int step_shift;  // log2 of the keys a step, 5 or 6
   int splits;      // the most splits of a tile's steps
@@ -227,8 +228,10 @@ __device__ __forceinline__ bool half_not_finite(uint32_t h) { return (h & 0x7c00
 // the many-row kernel's keys a step
 __host__ __device__ constexpr int many_step(int d) { return d > 192 ? 32 : 64; }
 
-// launches of the kernels
-void attend_few(int type, int d, const AttendArgs& a, int items, hipStream_t st);   // tile 16, step 32
-void attend_many(int type, int d, const AttendArgs& a, int items, hipStream_t st);  // tile 128, step many_step
+// launches of the kernels, of a.items or (a launch has fewer than 2^32 threads: past
+// that the runtime starts the rest of the division, without an error) in parts
+constexpr int kMostItems = 1 << 23;
+void attend_few(int type, int d, AttendArgs a, hipStream_t st);   // tile 16, step 32
+void attend_many(int type, int d, AttendArgs a, hipStream_t st);  // tile 128, step many_step
 
 }  // namespace weft

@@ -230,6 +230,7 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.seqs = w.seqs;
   a.seqs.n_tokens = (int)q->ne[2];
   a.part = p.splits > 1 ? static_cast<float*>(work) : nullptr;
+  a.items = p.tiles * w.heads;
   a.tile = p.tile;
   a.step_shift = p.step == 64 ? 6 : 5;
   a.splits = p.splits;
@@ -263,7 +264,7 @@ hipError_t attention(const weft_ggml_tensor* q, const weft_ggml_tensor* kc, cons
   a.half_q = q->type == WEFT_GGML_TYPE_F16;
   a.half_o = dst->type == WEFT_GGML_TYPE_F16;
   const hipStream_t st = current_stream();
-  (p.many ? attend_many : attend_few)(w.type, w.d, a, p.tiles * w.heads, st);
+  (p.many ? attend_many : attend_few)(w.type, w.d, a, st);
   if (p.splits > 1) join(w.d, a, p.many, st);
   return pending_error();
 }

@@ -32,6 +32,7 @@
 // step); against them the weights are two parts as well, so that V's rounding is
 // all that the sum carries.  A 16-bit V is exact and takes rounded weights.
 // Maximum, sum and accumulators are in 32 bits.
+#include <algorithm>
 #include <type_traits>
 
 #include "attention.h"
@@ -99,10 +100,10 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
 
   const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave);
   const int c = lane & 15, g = lane >> 4;  // query column (or key, value) and quarter
-  const int kvh = (int)blockIdx.x % a.kv_heads;
+  const int item = a.first + (int)blockIdx.x, kvh = item % a.kv_heads;
   const int split = (int)blockIdx.y;
   TileRows t;
-  if (!locate(a, (int)blockIdx.x / a.kv_heads, -1, 0, t)) return;
+  if (!locate(a, item / a.kv_heads, -1, 0, t)) return;
   const int seq = t.seq;
   int step0 = 0, step1 = t.range.steps;
   bool whole = true;  // the tile has one split
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
   const float f = !whole ? 1.f : all == 0.f ? 0.f : 1.f / all;  // a row that sees nothing: zeros
   float* part = nullptr;
   if (!whole) {
-    part = a.part + ((long long)blockIdx.x * a.splits + split) * 16 * (D + 2) + row * (D + 2);
+    part = a.part + ((long long)item * a.splits + split) * 16 * (D + 2) + row * (D + 2);
     if (threadIdx.x % 16 == 0) part[D] = top, part[D + 1] = all;
   }
   uint8_t* dst =
@@ -662,14 +663,17 @@ void launch_d(int d, const AttendArgs& a, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
-void attend_few(int type, int d, const AttendArgs& a, int items, hipStream_t st) {
-  const dim3 grid((unsigned)items, (unsigned)a.splits);
-  switch (type) {
-    case kKvF16: launch_d<kKvF16>(d, a, grid, st); break;
-    case kKvQ8_0: launch_d<kKvQ8_0>(d, a, grid, st); break;
-    default: launch_d<kKvQ4_0>(d, a, grid, st); break;
+void attend_few(int type, int d, AttendArgs a, hipStream_t st) {
+  for (; a.first < a.items; a.first += kMostItems) {
+    const dim3 grid((unsigned)std::min(a.items - a.first, kMostItems), (unsigned)a.splits);
+    switch (type) {
+      case kKvF16: launch_d<kKvF16>(d, a, grid, st); break;
+      case kKvQ8_0: launch_d<kKvQ8_0>(d, a, grid, st); break;
+      default: launch_d<kKvQ4_0>(d, a, grid, st); break;
+    }
+    check_launch("attend_few_kernel");
+    if (a.items - a.first <= kMostItems) break;  // first stays in 32 bits
   }
-  check_launch("attend_few_kernel");
 }
 
 }  // namespace weft

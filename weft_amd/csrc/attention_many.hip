@@ -27,6 +27,8 @@
 // much again): against 64 bits the outputs are off by 3e-4 of their size over a
 // 16-bit cache and 5e-4 over a quantized one, whose values' own rounding is 5e-3 and
 // more.  Products, maximum, sum and accumulators are in 32 bits.
+#include <algorithm>
+
 #include "attention.h"
 #include "runtime.h"
 
@@ -58,11 +60,12 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
 
   const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave), tid = threadIdx.x;
   const int c = lane & 31, h = lane >> 5;  // query column (or key, value) and half
-  const int kvh = (int)blockIdx.x % a.kv_heads;
-  const int split = (int)blockIdx.y;
   // a causal call's last tiles are its longest: they start first
+  const int turn = a.first + (int)blockIdx.x, kvh = turn % a.kv_heads;
+  const int tile = a.items / a.kv_heads - 1 - turn / a.kv_heads;
+  const int split = (int)blockIdx.y;
   TileRows t;
-  if (!locate(a, (int)(gridDim.x / a.kv_heads) - 1 - (int)blockIdx.x / a.kv_heads, -1, 0, t)) return;
+  if (!locate(a, tile, -1, 0, t)) return;
   const int seq = t.seq;
   int step0 = 0, step1 = t.range.steps;
   bool whole = true;
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   }
   if (!whole) {
     // the item's number in the sequences' order, as the join counts it
-    const long long item = (long long)(gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads) * a.kv_heads + kvh;
+    const long long item = (long long)tile * a.kv_heads + kvh;
     float* part = a.part + (item * a.splits + split) * (kWaves * kRows) * (D + 2) + (kRows * wave + c) * (D + 2);
 #pragma unroll
     for (int v = 0; v < NB; ++v)
@@ -512,14 +515,17 @@ void launch_d(int d, const AttendArgs& a, dim3 grid, hipStream_t st) {
 
 }  // namespace
 
-void attend_many(int type, int d, const AttendArgs& a, int items, hipStream_t st) {
-  const dim3 grid((unsigned)items, (unsigned)a.splits);
-  switch (type) {
-    case kKvF16: launch_d<kKvF16>(d, a, grid, st); break;
-    case kKvQ8_0: launch_d<kKvQ8_0>(d, a, grid, st); break;
-    default: launch_d<kKvQ4_0>(d, a, grid, st); break;
+void attend_many(int type, int d, AttendArgs a, hipStream_t st) {
+  for (; a.first < a.items; a.first += kMostItems) {
+    const dim3 grid((unsigned)std::min(a.items - a.first, kMostItems), (unsigned)a.splits);
+    switch (type) {
+      case kKvF16: launch_d<kKvF16>(d, a, grid, st); break;
+      case kKvQ8_0: launch_d<kKvQ8_0>(d, a, grid, st); break;
+      default: launch_d<kKvQ4_0>(d, a, grid, st); break;
+    }
+    check_launch("attend_many_kernel");
+    if (a.items - a.first <= kMostItems) break;  // first stays in 32 bits
   }
-  check_launch("attend_many_kernel");
 }
 
 }  // namespace weft

@@ -24,6 +24,9 @@ namespace weft {
 namespace {
 
 constexpr int kThreads = 256;
+// A launch has fewer than 2^32 threads: past that the runtime starts the rest of the
+// division, without an error.
+constexpr int kMostBlocks = (int)(((int64_t)1 << 31) / kThreads);
 
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(2))) Bytes8 {
@@ -112,12 +115,12 @@ __device__ __forceinline__ void store_record(uint8_t* row, int block, int part, 
 // looked up (starts, length, page: three dependent loads, most of a small call).
 template <int T, bool kHalfSrc>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(KvSeqs seqs, KvPool k, KvPool v, Rows kx, Rows vx, int d,
-                                                            int heads, int waves) {
+                                                            int heads, int waves, int t0) {
   constexpr int U = 4;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const int t = (int)blockIdx.x * (kThreads / kWave / waves) + wave / waves;
+  const int t = t0 + (int)blockIdx.x * (kThreads / kWave / waves) + wave / waves;
   const int stride = waves * kWave, first = wave % waves * kWave;
-  if (t >= seqs.n_tokens) return;
+  if ((unsigned)t >= (unsigned)seqs.n_tokens) return;
   const KvPool pool = blockIdx.y ? v : k;
   const Rows rows = blockIdx.y ? vx : kx;
   const uint8_t* src = rows.data + t * rows.token;
@@ -193,12 +196,12 @@ constexpr int kReadTokens = 8;
 template <int T, bool kHalfOut>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(KvSeqs seqs, KvPool k, KvPool v, Rows ko, Rows vo,
                                                            long long k_seq, long long v_seq, int d, int heads,
-                                                           int n_pos) {
+                                                           int n_pos, int p_first) {
   __shared__ long long place[kReadTokens];
   const int seq = (int)blockIdx.y;
   const KvPool pool = blockIdx.z ? v : k;
   const Rows out = blockIdx.z ? vo : ko;
-  const int p0 = (int)blockIdx.x * kReadTokens;
+  const int p0 = p_first + (int)blockIdx.x * kReadTokens;
   const int n = min(kReadTokens, n_pos - p0);
   if ((int)threadIdx.x < n) {
     const int pos = p0 + (int)threadIdx.x;
@@ -285,17 +288,21 @@ hipError_t kv_write(const weft_ggml_tensor* kx, const weft_ggml_tensor* vx, cons
   // few tokens: a workgroup each, one group a lane (8 x 128 values, one token:
   // 2.8 us against 4.6); more than are resident at once: a wave each (6,500 tokens of
   // Q4_0: 16.9 us against 19.4)
-  const int waves = 2 * w.seqs.n_tokens <= 8 * cu_count() ? 4 : 1;
-  const dim3 grid((unsigned)((w.seqs.n_tokens + 4 / waves - 1) / (4 / waves)), 2);
+  const int waves = w.seqs.n_tokens <= 4 * cu_count() ? 4 : 1;
+  const int each = kThreads / kWave / waves;  // tokens a workgroup
   const bool half = kx->type == WEFT_GGML_TYPE_F16;
   const hipStream_t st = current_stream();
-#define WEFT_KV_WRITE(T)                                                                                         \
-  (half ? kv_write_kernel<T, true><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads, waves)     \
-        : kv_write_kernel<T, false><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads, waves))
-  switch (w.type) {
-    case kKvF16: WEFT_KV_WRITE(kKvF16); break;
-    case kKvQ8_0: WEFT_KV_WRITE(kKvQ8_0); break;
-    default: WEFT_KV_WRITE(kKvQ4_0); break;
+#define WEFT_KV_WRITE(T)                                                                                             \
+  (half ? kv_write_kernel<T, true><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads, waves, first)  \
+        : kv_write_kernel<T, false><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, w.d, w.heads, waves, first))
+  for (int64_t t0 = 0; t0 < w.seqs.n_tokens; t0 += (int64_t)kMostBlocks * each) {
+    const int first = (int)t0;
+    const dim3 grid((unsigned)std::min<int64_t>(kMostBlocks, (w.seqs.n_tokens - t0 + each - 1) / each), 2);
+    switch (w.type) {
+      case kKvF16: WEFT_KV_WRITE(kKvF16); break;
+      case kKvQ8_0: WEFT_KV_WRITE(kKvQ8_0); break;
+      default: WEFT_KV_WRITE(kKvQ4_0); break;
+    }
   }
 #undef WEFT_KV_WRITE
   check_launch("kv_write_kernel");
@@ -317,17 +324,23 @@ hipError_t kv_read(const weft_ggml_tensor* kc, const weft_ggml_tensor* vc, const
   const Rows kr{static_cast<uint8_t*>(ko->data), (long long)ko->nb[1], (long long)ko->nb[2]};
   const Rows vr{static_cast<uint8_t*>(vo->data), (long long)vo->nb[1], (long long)vo->nb[2]};
   const int n_pos = (int)ko->ne[2];
-  const dim3 grid((unsigned)((ko->ne[2] + kReadTokens - 1) / kReadTokens), (unsigned)w.seqs.n_seqs, 2);
   const bool half = ko->type == WEFT_GGML_TYPE_F16;
   const hipStream_t st = current_stream();
   const long long ks = (long long)ko->nb[3], vs = (long long)vo->nb[3];
-#define WEFT_KV_READ(T)                                                                                              \
-  (half ? kv_read_kernel<T, true><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, ks, vs, w.d, w.heads, n_pos)  \
-        : kv_read_kernel<T, false><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, ks, vs, w.d, w.heads, n_pos))
-  switch (w.type) {
-    case kKvF16: WEFT_KV_READ(kKvF16); break;
-    case kKvQ8_0: WEFT_KV_READ(kKvQ8_0); break;
-    default: WEFT_KV_READ(kKvQ4_0); break;
+#define WEFT_KV_READ(T)                                                                                            \
+  (half ? kv_read_kernel<T, true><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, ks, vs, w.d, w.heads,       \
+                                                             n_pos, first)                                         \
+        : kv_read_kernel<T, false><<<grid, kThreads, 0, st>>>(w.seqs, w.k, w.v, kr, vr, ks, vs, w.d, w.heads,      \
+                                                              n_pos, first))
+  for (int64_t p0 = 0; p0 < n_pos; p0 += (int64_t)kMostBlocks * kReadTokens) {
+    const int first = (int)p0;
+    const dim3 grid((unsigned)std::min<int64_t>(kMostBlocks, (n_pos - p0 + kReadTokens - 1) / kReadTokens),
+                    (unsigned)w.seqs.n_seqs, 2);
+    switch (w.type) {
+      case kKvF16: WEFT_KV_READ(kKvF16); break;
+      case kKvQ8_0: WEFT_KV_READ(kKvQ8_0); break;
+      default: WEFT_KV_READ(kKvQ4_0); break;
+    }
   }
 #undef WEFT_KV_READ
   check_launch("kv_read_kernel");

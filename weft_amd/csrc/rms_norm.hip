@@ -186,22 +186,31 @@ __global__ void __launch_bounds__(1024) add_rms_norm_kernel(NormArgs a) {
   }
 }
 
+// A launch has fewer than 2^32 threads; past that the runtime starts the rest of the
+// division, without an error.
 template <int Out>
-void launch(const NormArgs& a, int64_t rows, hipStream_t st) {
+void launch(NormArgs a, int64_t rows, hipStream_t st) {
   // threads: a lane's values stay in registers up to four groups of four
   const int groups = (a.k + 3) / 4;
   int threads = kWave;
   while (threads < 1024 && threads * 4 < groups) threads *= 2;
   const int v = (groups + threads - 1) / threads;
-  const dim3 grid((unsigned)rows);
-  if (v <= 1)
-    add_rms_norm_kernel<Out, 1><<<grid, threads, 0, st>>>(a);
-  else if (v <= 2)
-    add_rms_norm_kernel<Out, 2><<<grid, threads, 0, st>>>(a);
-  else if (v <= 4)
-    add_rms_norm_kernel<Out, 4><<<grid, threads, 0, st>>>(a);
-  else
-    add_rms_norm_kernel<Out, 0><<<grid, threads, 0, st>>>(a);
+  const int64_t most = ((int64_t)1 << 31) / threads;
+  for (; rows > 0; rows -= most) {
+    const dim3 grid((unsigned)std::min(rows, most));
+    if (v <= 1)
+      add_rms_norm_kernel<Out, 1><<<grid, threads, 0, st>>>(a);
+    else if (v <= 2)
+      add_rms_norm_kernel<Out, 2><<<grid, threads, 0, st>>>(a);
+    else if (v <= 4)
+      add_rms_norm_kernel<Out, 4><<<grid, threads, 0, st>>>(a);
+    else
+      add_rms_norm_kernel<Out, 0><<<grid, threads, 0, st>>>(a);
+    a.x += most * a.x_row;
+    if (a.r != nullptr) a.r += most * a.r_row;
+    if (a.s != nullptr) a.s += most * a.s_row;
+    a.y += most * a.y_row;
+  }
 }
 
 hipError_t fail(hipError_t e) {
