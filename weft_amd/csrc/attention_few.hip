@@ -396,14 +396,13 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
         } else {
           bad = half_not_finite(raw.vs[i]);
         }
-        bad = bad && !zero && live;
+        bad = bad && !zero && live;  // the row is cleared below
         if (__ballot(bad)) {  // hardly ever
           uint32_t mine = bad ? 1u << (key & 31) : 0u;
 #pragma unroll
           for (int s = 32; s > 0; s >>= 1) mine |= (uint32_t)__shfl_xor((int)mine, s, kWave);
           spoiled |= mine;
         }
-        zero = zero || bad;
       }
       if (live) {
         uint8_t* dst = vrow + key * L::kRow;
@@ -437,6 +436,11 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
         }
       }
     }
+    // whole rows: their finite values too are added with the others, at the end
+    if (spoiled != 0) wave_sync();
+    for (uint32_t left = spoiled; left != 0; left &= left - 1)
+      for (int i = opaque_lane(); i < 16 * NB; i += kWave)
+        *reinterpret_cast<uint32_t*>(vrow + (__ffs(left) - 1) * L::kRow + 4 * i) = 0;
     // K's steps, times the scale, as [block][key]
     if constexpr (T != kKvF16) {
 #pragma unroll
@@ -561,7 +565,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
       o[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[v], 0, 0, 0);
       if constexpr (T != kKvF16) o[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[v], 0, 0, 0);
     }
-    // values that are not finite reach the rows that see their key, and no other
+    // a key with values that are not finite reaches the rows that see it, and no other
     while (spoiled) {
       const int key = __ffs(spoiled) - 1;
       spoiled &= spoiled - 1;

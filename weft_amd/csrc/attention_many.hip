@@ -275,8 +275,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         } else {
           bad = half_not_finite(sv[i]);
         }
-        if (bad && !zero) spoiled |= 1ull << key;
-        zero = zero || bad;
+        if (bad && !zero) spoiled |= 1ull << key;  // the row is cleared before its products
       }
       put(rv[i], sv[i], zero, base + L::kV + key * L::kVRow, e);
     }
@@ -303,6 +302,21 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     const int next_page = page_of(next);
     if (step + 1 < step1) load(step + 1, next_page);
     next = entry_of(step + 2);
+
+    // Keys with values that are not finite: their whole rows are cleared, once every
+    // thread's part is there, and reach the rows that see them at the end.
+    unsigned long long spoiled = 0;
+    if (is_edge(pos, present)) {
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) spoiled |= spoiled_of[buf][w];
+      spoiled = (unsigned long long)(uint32_t)uniform((int)(spoiled >> 32)) << 32 | (uint32_t)uniform((int)spoiled);
+      if (spoiled != 0) {  // for all of the workgroup's threads, or none
+        for (unsigned long long left = spoiled; left != 0; left &= left - 1)
+          if (const int i = opaque_tid(); i < 16 * NB)
+            *reinterpret_cast<uint32_t*>(lds + buf * L::kBytes + L::kV + __builtin_ctzll(left) * L::kVRow + 4 * i) = 0;
+        __syncthreads();
+      }
+    }
 
     // rows of this wave see none, different, or all of the step's keys
     const bool none = idle || pos > last_pos ||
@@ -422,36 +436,30 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         }
         asm volatile("" : "+v"(l));  // summed here: 32 weights more in registers would not fit
       }
-      if (is_edge(pos, present)) {
-        // values that are not finite reach the rows that see their key, and no other
-        unsigned long long spoiled = 0;
+      while (spoiled) {
+        const int key = __builtin_ctzll(spoiled);
+        spoiled &= spoiled - 1;
+        int pg, slot;
+        if (!kv_place(a.seqs, seq, pos + key, pg, slot)) continue;
+        const uint8_t* vr = a.v.data + (long long)kvh * a.v.head + pg * a.v.page + slot * a.v.slot;
+        const int want = 16 * (key / 32) + 4 * (key % 32 / 8) + key % 4;
+        float w = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) spoiled |= spoiled_of[buf][w];
-        while (spoiled) {
-          const int key = __builtin_ctzll(spoiled);
-          spoiled &= spoiled - 1;
-          int pg, slot;
-          if (!kv_place(a.seqs, seq, pos + key, pg, slot)) continue;
-          const uint8_t* vr = a.v.data + (long long)kvh * a.v.head + pg * a.v.page + slot * a.v.slot;
-          const int want = 16 * (key / 32) + 4 * (key % 32 / 8) + key % 4;
-          float w = 0.f;
+        for (int k = 0; k < 2 * kPart; ++k) {
+          f16x8 pk = p[k];
+          asm volatile("" : "+v"(pk));  // converted here, not beside every step's weights
 #pragma unroll
-          for (int k = 0; k < 2 * kPart; ++k) {
-            f16x8 pk = p[k];
-            asm volatile("" : "+v"(pk));  // converted here, not beside every step's weights
+          for (int e = 0; e < 8; ++e) w = 8 * k + e == want ? (float)pk[e] : w;
+        }
+        w = __shfl(w, 32 * (key / 4 & 1) + c, kWave);
+        if (seen_bits(a, 1ull, pos + key, qpos)) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w = 8 * k + e == want ? (float)pk[e] : w;
-          }
-          w = __shfl(w, 32 * (key / 4 & 1) + c, kWave);
-          if (seen_bits(a, 1ull, pos + key, qpos)) {
+          for (int v = 0; v < NB; ++v)
 #pragma unroll
-            for (int v = 0; v < NB; ++v)
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                o[v][e] += w * value_of<T>(vr, 32 * v + 8 * (e / 4) + 4 * h + e % 4);
-                asm volatile("" ::: "memory");  // one value at a time: no registers for this path
-              }
-          }
+            for (int e = 0; e < 16; ++e) {
+              o[v][e] += w * value_of<T>(vr, 32 * v + 8 * (e / 4) + 4 * h + e % 4);
+              asm volatile("" ::: "memory");  // one value at a time: no registers for this path
+            }
         }
       }
     }
