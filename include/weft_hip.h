@@ -403,9 +403,10 @@ int weft_ggml_kv_read(const weft_ggml_tensor *k_cache, const weft_ggml_tensor *v
  * with window > 0 those of j > p - window or j < sinks, absent ones left out.
  * dst (D, heads, tokens): F32 or F16; a query that sees nothing gets zeros,
  * rows of no sequence stay as they are.  D: 64, 96, 128, 192 or 256.
- * Queries, keys and values pass through 16-bit floats: past 65504 they are
- * infinite, below 6e-5 they are rounded to multiples of 6e-8.  Sums, the
- * softmax's maximum and sum, and accumulators have 32 bits.
+ * Queries, keys and values pass through 16-bit floats: past 65504 queries and
+ * keys are infinite (quantized values stay as they are), below 6e-5 all are
+ * rounded to multiples of 6e-8.  Sums, the softmax's maximum and sum, and
+ * accumulators have 32 bits.
  * wdata: weft_ggml_attention_work_size bytes, 16-byte aligned (scratch; its
  * content need not be kept or cleared). */
 size_t weft_ggml_attention_work_size(const weft_ggml_tensor *q, const weft_ggml_tensor *k_cache,

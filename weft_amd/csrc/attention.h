@@ -225,6 +225,13 @@ __device__ __forceinline__ float value_of(const uint8_t* row, int i) {
 
 __device__ __forceinline__ bool half_not_finite(uint32_t h) { return (h & 0x7c00u) == 0x7c00u; }
 
+// Whether a record's values may be past 16 bits, by its step: infinite, NaN, or from
+// 65536 / 128 (8 for 4-bit codes) on.  kv_write makes such records of finite values.
+template <int T>
+__device__ __forceinline__ bool past_half(uint32_t step) {
+  return !(__builtin_fabsf16(__builtin_bit_cast(_Float16, (uint16_t)step)) < (_Float16)(T == kKvQ8_0 ? 512.f : 8192.f));
+}
+
 // the many-row kernel's keys a step
 __host__ __device__ constexpr int many_step(int d) { return d > 192 ? 32 : 64; }
 

@@ -30,7 +30,8 @@
 // too, and a record's step multiplies their 32-bit sum.  A query in 32 bits is
 // two 16-bit parts, two products.  V's values are rounded to 16 bits (code times
 // step); against them the weights are two parts as well, so that V's rounding is
-// all that the sum carries.  A 16-bit V is exact and takes rounded weights.
+// all that the sum carries.  A 16-bit V is exact and takes rounded weights.  A V whose
+// values may be past 16 bits is added apart, in 32.
 // Maximum, sum and accumulators are in 32 bits.
 #include <algorithm>
 #include <type_traits>
@@ -371,7 +372,10 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
     // over K's, which are read), so units that come in halves take half the registers.
     constexpr bool kHalves = kSame && R::kV % 2 == 0;
     // V into LDS rows; a key that no row sees is zeros (its memory may hold anything)
-    uint32_t spoiled = 0;  // keys some rows see whose values are not all finite
+    // keys that some rows see whose values are not all finite, in steps whose rows see
+    // different keys, or not all within 16 bits
+    uint32_t spoiled = 0;
+    unsigned long long past[R::kV];  // lanes whose unit i is past 16 bits
     const int x0 = kSame ? lane : opaque_lane();
 #pragma unroll
     for (int i = 0; i < R::kV; ++i) {
@@ -387,15 +391,11 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
       const int key = kSame ? i * kRowsOn + lane / R::kVUnit : u / R::kVUnit, e = kSame ? e0 : u % R::kVUnit;
       const bool live = R::kVUnit * kStep % kWave == 0 || key < kStep;
       bool zero = masked && !(present >> (key & 31) & 1u);
-      if (masked) {
-        bool bad;
-        if constexpr (T == kKvF16) {
-          bad = false;
+      if constexpr (T != kKvF16) past[i] = __ballot(past_half<T>(raw.vs[i]));
+      if (T == kKvF16 && masked) {
+        bool bad = false;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) bad = bad || half_not_finite(raw.v[i].w[w]) || half_not_finite(raw.v[i].w[w] >> 16);
-        } else {
-          bad = half_not_finite(raw.vs[i]);
-        }
+        for (int w = 0; w < 4; ++w) bad = bad || half_not_finite(raw.v[i].w[w]) || half_not_finite(raw.v[i].w[w] >> 16);
         bad = bad && !zero && live;  // the row is cleared below
         if (__ballot(bad)) {  // hardly ever
           uint32_t mine = bad ? 1u << (key & 31) : 0u;
@@ -434,6 +434,22 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
             to[1] = make_uint4(y[4], y[5], y[6], y[7]);
           }
         }
+      }
+    }
+    if constexpr (T != kKvF16) {
+      unsigned long long any = 0;
+#pragma unroll
+      for (int i = 0; i < R::kV; ++i) any |= past[i];
+      if (any) {  // hardly ever
+        uint32_t mine = 0;
+#pragma unroll
+        for (int i = 0; i < R::kV; ++i) {
+          const int u = i * kWave + opaque_lane();
+          if (u < R::kVUnit * kStep && past[i] >> (u % kWave) & 1) mine |= 1u << (u / R::kVUnit);
+        }
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) mine |= (uint32_t)__shfl_xor((int)mine, s, kWave);
+        spoiled = mine & present;
       }
     }
     // whole rows: their finite values too are added with the others, at the end
@@ -565,7 +581,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
       o[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph, o[v], 0, 0, 0);
       if constexpr (T != kKvF16) o[v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl, o[v], 0, 0, 0);
     }
-    // a key with values that are not finite reaches the rows that see it, and no other
+    // those keys reach the rows that see them, and no other
     while (spoiled) {
       const int key = __ffs(spoiled) - 1;
       spoiled &= spoiled - 1;

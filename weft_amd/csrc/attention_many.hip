@@ -26,7 +26,8 @@
 // rounded once to 16 bits (a second part of each would cost the matrix pipe as
 // much again): against 64 bits the outputs are off by 3e-4 of their size over a
 // 16-bit cache and 5e-4 over a quantized one, whose values' own rounding is 5e-3 and
-// more.  Products, maximum, sum and accumulators are in 32 bits.
+// more.  Records of V that may be past 16 bits are added apart, in 32.  Products, maximum,
+// sum and accumulators are in 32 bits.
 #include <algorithm>
 
 #include "attention.h"
@@ -57,6 +58,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   constexpr int D = 32 * NB, kStep = L::kStep, kPart = kStep / 32;
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // two steps' tiles
   __shared__ unsigned long long spoiled_of[2][kWaves];
+  __shared__ uint32_t met;  // whether any step had such a key, of quantized ones
 
   const int lane = threadIdx.x & (kWave - 1), wave = uniform((int)threadIdx.x / kWave), tid = threadIdx.x;
   const int c = lane & 31, h = lane >> 5;  // query column (or key, value) and half
@@ -258,7 +260,9 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     const unsigned long long present = present_of(pos, page);
     const bool edge = is_edge(pos, present);
     uint8_t* base = lds + buf * L::kBytes;
+    // keys whose rows (records, where there are some) stay out of the products
     unsigned long long spoiled = 0;
+    bool past = false;
 #pragma unroll
     for (int i = 0; i < L::kUnits; ++i) {
       const int u = i * kThreads + x;
@@ -268,27 +272,42 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
       bool zero = false;
       if (edge) {
         zero = !((uint32_t)(key & 32 ? present >> 32 : present) >> (key & 31) & 1u);
-        bool bad = false;
         if constexpr (T == kKvF16) {
+          bool bad = false;
 #pragma unroll
           for (int w = 0; w < 4; ++w) bad = bad || half_not_finite(rv[i].w[w]) || half_not_finite(rv[i].w[w] >> 16);
-        } else {
-          bad = half_not_finite(sv[i]);
+          if (bad && !zero) spoiled |= 1ull << key;
         }
-        if (bad && !zero) spoiled |= 1ull << key;  // the row is cleared before its products
+      }
+      if constexpr (T != kKvF16) {
+        const bool mine = past_half<T>(sv[i]);
+        past = past || mine;
+        zero = zero || mine;
       }
       put(rv[i], sv[i], zero, base + L::kV + key * L::kVRow, e);
     }
-    if (edge) {
+    if (T != kKvF16 && __ballot(past)) {  // hardly ever
+#pragma unroll
+      for (int i = 0; i < L::kUnits; ++i) {
+        const int u = i * kThreads + x, key = kSame ? i * kRowsOn + key0 : u / L::kUnit;
+        if (key < kStep && past_half<T>(sv[i]) && present >> key & 1) spoiled |= 1ull << key;
+      }
+    }
+    if (T != kKvF16 || edge) {
       if (__ballot(spoiled != 0)) {  // hardly ever
 #pragma unroll
         for (int s = 32; s > 0; s >>= 1)
           spoiled |= (unsigned long long)__shfl_xor((long long)spoiled, s, kWave);
       }
       if (lane == 0) spoiled_of[buf][wave] = spoiled;
+      if (T != kKvF16 && spoiled != 0) met = 1;
     }
   };
 
+  if constexpr (T != kKvF16) {
+    if (tid == 0) met = 0;
+    __syncthreads();
+  }
   int page = page_of(entry_of(step0)), next = entry_of(step0 + 1);
   if (step0 < step1) {
     load(step0, page);
@@ -303,10 +322,13 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     if (step + 1 < step1) load(step + 1, next_page);
     next = entry_of(step + 2);
 
-    // Keys with values that are not finite: their whole rows are cleared, once every
-    // thread's part is there, and reach the rows that see them at the end.
+    // Keys with values that are not finite, where rows see different keys: their whole
+    // rows are cleared, once every thread's part is there, and reach the rows that see
+    // them at the end.  Of a quantized key the records past 16 bits were not stored.
     unsigned long long spoiled = 0;
-    if (is_edge(pos, present)) {
+    uint32_t any = 0;
+    if constexpr (T != kKvF16) any = met;  // looked at after the products
+    if (T == kKvF16 && is_edge(pos, present)) {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) spoiled |= spoiled_of[buf][w];
       spoiled = (unsigned long long)(uint32_t)uniform((int)(spoiled >> 32)) << 32 | (uint32_t)uniform((int)spoiled);
@@ -436,6 +458,12 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         }
         asm volatile("" : "+v"(l));  // summed here: 32 weights more in registers would not fit
       }
+      if constexpr (T != kKvF16) {
+        if (uniform((int)any) != 0) {
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) spoiled |= spoiled_of[buf][w];
+        }
+      }
       while (spoiled) {
         const int key = __builtin_ctzll(spoiled);
         spoiled &= spoiled - 1;
@@ -454,12 +482,14 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         w = __shfl(w, 32 * (key / 4 & 1) + c, kWave);
         if (seen_bits(a, 1ull, pos + key, qpos)) {
 #pragma unroll
-          for (int v = 0; v < NB; ++v)
+          for (int v = 0; v < NB; ++v) {
+            if (T != kKvF16 && !past_half<T>(uniform((int)ld_u16(vr + v * KvRecord<T>::kBytes)))) continue;
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               o[v][e] += w * value_of<T>(vr, 32 * v + 8 * (e / 4) + 4 * h + e % 4);
               asm volatile("" ::: "memory");  // one value at a time: no registers for this path
             }
+          }
         }
       }
     }
