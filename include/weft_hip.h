@@ -405,8 +405,9 @@ int weft_ggml_kv_read(const weft_ggml_tensor *k_cache, const weft_ggml_tensor *v
  * rows of no sequence stay as they are.  D: 64, 96, 128, 192 or 256.
  * Queries, keys and values pass through 16-bit floats: past 65504 queries and
  * keys are infinite (quantized values stay as they are), below 6e-5 all are
- * rounded to multiples of 6e-8.  Sums, the softmax's maximum and sum, and
- * accumulators have 32 bits.
+ * rounded to multiples of 6e-8.  So do weights, of which those down to 2^-26 of
+ * a row's largest keep 11 bits and those below 2^-37 are lost.  Sums, the softmax's
+ * maximum and sum, and accumulators have 32 bits.
  * wdata: weft_ggml_attention_work_size bytes, 16-byte aligned (scratch; its
  * content need not be kept or cleared). */
 size_t weft_ggml_attention_work_size(const weft_ggml_tensor *q, const weft_ggml_tensor *k_cache,

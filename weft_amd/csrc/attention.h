@@ -195,12 +195,18 @@ __device__ __forceinline__ float quarters_sum(float x) {
   return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// A row's maximum moves only when a score is more than 2^kLag times its weight's
-// scale: weights up to 2^kLag keep their 11 bits in 16, and the sums are not
-// rescaled at nearly every step.
-constexpr float kLag = 8.f;
+// A row's weights are powers of two of its scores over a reference that lies kUp below
+// the largest score, so that the 16 bits they are rounded to reach far down: weights of
+// 2^-26 of the largest keep 11 bits, those below 2^-37 are lost.  (With the largest score
+// itself as the reference that was 2^-14 and 2^-25: beside a key that takes nearly all the
+// weight and has small values, outputs whose weights were e^-15 of it were 0.3 to 1.4 %
+// off.)  The reference moves when a score is kMost above it, 2^15 as a weight: three past
+// kUp, so that sums are not rescaled at nearly every step.  From 2^22 on, where kUp is no
+// longer exact beside a score, the reference is the score.
+constexpr float kUp = 12.f, kMost = 15.f;
+__device__ __forceinline__ float reference(float top) { return fabsf(top) < 0x1p22f ? top - kUp : top; }
 
-// exp2 of an argument <= kLag (results below 2^-126 are zero)
+// exp2 of an argument <= kMost (results below 2^-126 are zero)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Four code bytes as 16-bit integers, exactly: byte u as 0x6400 | u is 1024 + u.

@@ -17,7 +17,7 @@
 namespace weft {
 namespace {
 
-// The splits of a (token, head) row, each with its maximum, sum and weighted
+// The splits of a (token, head) row, each with its reference, sum and weighted
 // values: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i.
 constexpr int kJoinThreads = 256, kMaxSplits = 256;
 

@@ -30,7 +30,7 @@
 // too, and a record's step multiplies their 32-bit sum.  A query in 32 bits is
 // two 16-bit parts, two products.  V's values are rounded to 16 bits (code times
 // step); against them the weights are two parts as well, so that V's rounding is
-// all that the sum carries.  A 16-bit V is exact and takes rounded weights.  A V whose
+// all that the sum carries, down to weights of 2^-25 of a row's largest.  A 16-bit V is exact and takes rounded weights.  A V whose
 // values may be past 16 bits is added apart, in 32.
 // Maximum, sum and accumulators are in 32 bits.
 #include <algorithm>
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
   const int last_pos = (int)max(-1ll, t.pos0 + (t.row0 + t.rows - 1) / a.share);
 
   f32x4 o[2 * NB] = {};
-  float m = -INFINITY, l = 0.f;
+  float ref = -INFINITY, l = 0.f;
 
   uint8_t* const vrow = lds[wave];
   float* const ksteps = reinterpret_cast<float*>(lds[wave] + L::kSteps);
@@ -547,19 +547,19 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
     }
     float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     top = quarters_max(top);
-    if (__ballot(top > m + kLag)) {
-      const float now = fmaxf(m, top);
-      const float f = now == -INFINITY ? 1.f : exp2_fast(m - now);
-      m = now;
+    if (__ballot(top - ref > kMost)) {
+      const float now = fmaxf(ref, reference(top));
+      const float f = now == -INFINITY ? 1.f : exp2_fast(ref - now);
+      ref = now;
       l *= f;
 #pragma unroll
       for (int v = 0; v < 2 * NB; ++v) o[v] *= f;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
+    const float from = ref == -INFINITY ? 0.f : ref;
     f16x8 ph, pl;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float p = exp2_fast(x[e] - ref);
+      const float p = exp2_fast(x[e] - from);
       l += p;
       ph[e] = (_Float16)p;
       if constexpr (T != kKvF16) pl[e] = (_Float16)(p - (float)ph[e]);
@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kWaves* kWave, NB <= 4 ? 3 : 1) attend_few_ker
   float* mine = reinterpret_cast<float*>(lds[wave]) + col * L::kORow + last / 16 * 4;
 #pragma unroll
   for (int v = 0; v < 2 * NB; ++v) *reinterpret_cast<f32x4*>(mine + 16 * v) = o[v];
-  if (last < 16) ml[wave][col][0] = m, ml[wave][col][1] = sum;
+  if (last < 16) ml[wave][col][0] = ref, ml[wave][col][1] = sum;
   __syncthreads();
   const int row = threadIdx.x / 16;
   if (row >= t.rows) return;

@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
   }
 
   f32x16 o[NB] = {};
-  float m = -INFINITY, l = 0.f;
+  float ref = -INFINITY, l = 0.f;
   f32x16 minus = {};  // the reference, negative, in every place
 
   // The table's entry for a step's key `lane` (of 32: keys twice), looked up two steps
@@ -371,7 +371,8 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_s_setprio(0);
-      const float ref0 = m == -INFINITY ? 0.f : m;
+      const bool first = ref == -INFINITY;
+      const float ref0 = first ? 0.f : ref;
       if (!folded) {
 #pragma unroll
         for (int i = 0; i < kPart; ++i)
@@ -404,21 +405,24 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
         const u32x2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
         top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
       }
-      if (__ballot(top + ref0 > m + kLag)) {
-        const float now = fmaxf(m, top + ref0);
-        const float f = now == -INFINITY ? 1.f : exp2_fast(m - now);
-        m = now;
+      if (__ballot(top > (first ? -INFINITY : kMost))) {
+        // the scores are over the reference already; it moves by
+        float by = reference(top);
+        if (top == -INFINITY || (!first && by < 0.f)) by = 0.f;
+        const float now = ref0 + by;
+        if (fabsf(now) < 0x1p22f) by = now - ref0;  // as it is rounded
+        const float f = first ? 0.f : exp2_fast(-by);  // at first there are no sums
+        if (!first || top != -INFINITY) ref = now;
         l *= f;
 #pragma unroll
         for (int v = 0; v < NB; ++v) o[v] *= f;
-        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
         for (int i = 0; i < kPart; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[i][e] += ref0 - ref;
+          for (int e = 0; e < 16; ++e) s[i][e] -= by;
         if (folded) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) minus[e] = -ref;
+          for (int e = 0; e < 16; ++e) minus[e] = -now;
         }
       }
       f16x8 p[2 * kPart];
@@ -513,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, NB <= 4 ? 2 : 1) attend_many_kernel(
     for (int v = 0; v < NB; ++v)
 #pragma unroll
       for (int e = 0; e < 16; ++e) part[32 * v + 8 * (e / 4) + 4 * h + e % 4] = o[v][e];
-    if (h == 0) part[D] = m, part[D + 1] = l;
+    if (h == 0) part[D] = ref, part[D + 1] = l;
     return;
   }
   const float f = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing: zeros
