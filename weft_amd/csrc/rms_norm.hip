@@ -8,8 +8,10 @@
 // One workgroup a row, a lane owning groups of four consecutive values: a
 // Q8_0 / Q8_1 record is eight lanes, a Q8_K record one wave, and the values stay
 // in registers between the sum of squares and the records, so memory is read
-// and written once.  The square sum is held in 32 bits: per lane over at most
-// 64 values, then a tree over the lanes and waves.
+// and written once (rows past 16384 values: the sum, or the inputs, are read again).
+// The square sum is held in 32 bits: a lane sums its values, 16 at most in registers
+// and one in 1024 of a longer row, then trees over the lanes and waves; the terms
+// are not negative, so its error is at most 2^-24 for each of those additions.
 //
 // Bound by memory: 16384 rows of 8192 values with a residual and its sum, to Q8_K,
 // take 307 us (5.7 TB/s); 509 rows of 11008 to Q8_0 17.4 us (4.2 TB/s); a row of
