@@ -123,8 +123,9 @@ __device__ __forceinline__ int wave_max_count(int v) {  // of values >= 0
 // Where a tile of the call lies: tile number `tile` in the sequences' order, or
 // with `row` >= 0 the tile of that new token's row (token, head in its group).
 // Also the steps a split takes: the longest sequence's over the most splits, the
-// same for every tile, so that a batch of uneven sequences makes splits of even
-// work.  The whole wave calls it; 64 sequences are looked at at once, so a call's
+// same for every tile, so that shorter sequences make fewer splits of the same work.
+// (The most splits are the host's; a call with as many tiles as run at once has one, and
+// lasts as long as its longest sequence.)  The whole wave calls it; 64 sequences are looked at at once, so a call's
 // starts and lengths cost one trip to memory.  A start below one before it counts as
 // that one, so no row is in two sequences and a call has no more tiles than the host
 // planned for.

@@ -6,8 +6,9 @@
 // j > p - window or j < sinks.  A query that sees no key gets zeros.
 //
 // attention_few.hip has tiles of 16 query rows, attention_many.hip of 128; this
-// file checks calls, chooses tiles and splits, and joins the splits (2 to 4 us for a
-// token; 8 us for 512 tokens of 64 heads in two splits, 25 MB).
+// file checks calls, chooses tiles and splits, and joins the splits (a token's 32 splits
+// in 4.4 us, 96 in 7.5, 48 tokens' in 6.8; 8 us for 512 tokens of 64 heads in two
+// splits, 25 MB).
 #include <algorithm>
 #include <cmath>
 
@@ -168,7 +169,9 @@ Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
   const int64_t tokens = q->ne[2], share = q->ne[1] / w.heads, seqs = w.seqs.n_seqs;
   const int64_t rows = tokens * share;
   // 32 rows a sequence on average: below, a tile of 16 rows reads the cache at its
-  // full rate; above, 128 rows share a step's conversion
+  // full rate; above, 128 rows share a step's conversion (us in tiles of 16 and of 128,
+  // Q8_0, 32 heads over 8 of 128, 16 / 32 / 64 / 128 rows: one sequence of 8192 keys
+  // 21, 20, 30, 41 and 29, 29, 32, 41; 16 of up to 2048 31, 38, 50, 80 and 31, 32, 34, 44)
   p.many = rows > 32 * seqs;
   p.tile = p.many ? 128 : 16;
   p.step = p.many ? many_step(w.d) : 32;
@@ -176,7 +179,11 @@ Plan plan_of(const weft_ggml_tensor* q, const KvView& w) {
   p.least = 4;
   // as many workgroups as run at once, unless there are that many tiles: more of
   // them cost 10 % (131072 keys, Q8_0: 70 us at three a CU, 80 at six), as their
-  // first steps and joins add up
+  // first steps and joins add up.  us at 1, 2, 3 and 4 a CU: a token over 65536 keys
+  // Q8_0, heads of 64 37 29 29 29, of 128 49 41 41 44, of 256 81 88 102 103, F16 of 128
+  // 48 49 52 52; tokens of 32 sequences of up to 4096 keys, in that order, 56 43 39 37,
+  // 79 62 59 62, 132 144 153 156, 77 80 83 86; 300 tokens over 16384 keys, heads of 128
+  // 103 100 92 97, of 256 355 278 289 286
   const int64_t resident = w.d > 128 ? 1 : p.many || w.type == kKvF16 ? 2 : 3;
   const int64_t items = (int64_t)p.tiles * w.heads, want = resident * (int64_t)cu_count();
   const int64_t steps = ((int64_t)w.seqs.max_pages * w.seqs.page_size + p.step - 1) / p.step;

@@ -1,9 +1,9 @@
 // Attention of few query rows a kv head: decode steps and short chunks.
 //
 // Bound by reading the cache, 4-bit codes by converting them beside that: 48
-// sequences of up to 8192 Q8_0 tokens, 32 heads over 8 of 128 values, take 125 us
+// sequences of up to 8192 Q8_0 tokens, 32 heads over 8 of 128 values, take 126 us
 // (4.0 TB/s); one of 131072 Q4_0 tokens 52 us (2.9 TB/s, about 450 VALU
-// instructions a wave and step, 65 % of the busy cycles); 1023 Q8_0 tokens 11.8 us
+// instructions a wave and step, 65 % of the busy cycles); 1023 Q8_0 tokens 11.6 us
 // with the join, both launches and a dozen dependent trips to memory.
 //
 // Each of a workgroup's four waves takes every

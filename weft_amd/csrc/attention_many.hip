@@ -2,11 +2,11 @@
 //
 // Bound by the matrix pipe and the softmax beside it, which two waves a SIMD overlap
 // in part only: a prompt of 4096 16-bit tokens, 32 heads over 8 of 128 values, takes
-// 170 to 185 us (0.74 to 0.81 PFLOP/s; the matrix pipe is busy for 35 % of it, the
-// vector unit for 36 %, a quarter of a wave's time waits for records or the step's
+// 169 to 180 us (0.76 to 0.81 PFLOP/s; the matrix pipe is busy for 34 % of it, the
+// vector unit for 38 %, a quarter of a wave's time waits for records or the step's
 // barrier); 512 tokens of 64 heads of 64 in a window of 4096 behind 32768 Q8_0 keys
-// 71 to 79 us with the join (0.44 to 0.48 PFLOP/s); nine chunks of up to 640 tokens
-// over up to 3001 Q4_0 keys with no shared heads 111 to 114 us (0.37 PFLOP/s: the
+// 73 us with the join (0.47 PFLOP/s); nine chunks of up to 640 tokens
+// over up to 3001 Q4_0 keys with no shared heads 114 us (0.37 PFLOP/s: the
 // longest tile's 47 steps; each workgroup converts the records for its 128 rows only).
 //
 // A workgroup owns 128 rows,

@@ -10,7 +10,7 @@
 // Both directions are one pass bound by memory: a workgroup's threads take
 // consecutive groups of four (write) or eight (read) values, keys and values
 // in one launch.  Writing 5500 tokens of 8 heads of 128 F32 values as Q4_0 takes
-// 17 us (3.0 TB/s); reading 32 sequences of up to 16384 Q8_0 tokens into F16
+// 18 us (2.9 TB/s), as Q8_0 18 (3.1), as F16 13.5 (5.0); reading 32 sequences of up to 16384 Q8_0 tokens into F16
 // 545 us (5.3 TB/s, the zeros past their lengths with them); one token 3.3 us, and
 // 131 tokens back 4.7 us: launches and the dependent loads of a row's place.
 #include <limits.h>
@@ -188,8 +188,10 @@ __device__ __forceinline__ void values8(const Bytes16& b, int part, uint32_t ste
 // blockIdx.x: kReadTokens positions, blockIdx.y: sequence, blockIdx.z: keys or
 // values; zeros where the sequence has no value.  The positions' rows are looked
 // up once; then a thread has four groups of eight values in flight, and a wave
-// writes 1 KiB of F16 in one store, past the caches: 32 sequences of up to 16384
-// tokens take 545 us so and 584 through them, four of up to 8192 31 and 45.
+// writes 1 KiB of F16 in one store, past the caches (us past them and through them, 134
+// MB written: 29 and 29, 268 MB: 65 and 86, 2147 MB: 542 and 582; with a copy of it all
+// right after: 79 and 82, 178 and 177, 1239 and 1282; with a reduction instead: 112 and
+// 93, 225 and 234, 1582 and 1634: a reader of what the Infinity Cache would hold loses).
 typedef _Float16 half8 __attribute__((ext_vector_type(8), aligned(2)));
 typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
 constexpr int kReadTokens = 8;
