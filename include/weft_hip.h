@@ -381,8 +381,8 @@ typedef struct weft_ggml_kv_batch {
 } weft_ggml_kv_batch;
 
 /* Caches are (D, page size, kv heads, pages) of F16, Q8_0 or Q4_0, D a multiple
- * of 32, any page size, any 2-byte-aligned strides (heads and slots may be
- * swapped); keys and values have one type and shape.
+ * of 32, D x kv heads at most 2^30, any page size, any 2-byte-aligned strides
+ * (heads and slots may be swapped); keys and values have one type and shape.
  *
  * Quantizes rows k, v (D, kv heads, tokens; F32 or F16, any strides) into
  * their sequences' slots.  Tokens of no sequence, and absent positions, are

@@ -378,6 +378,7 @@ hipError_t kv_view(const weft_ggml_tensor* kc, const weft_ggml_tensor* vc, const
       return hipErrorInvalidValue;
   }
   if (kc->ne[0] == 0 || kc->ne[0] % 32 || kc->ne[1] == 0 || kc->ne[2] == 0) return hipErrorInvalidValue;
+  if (kc->ne[0] * kc->ne[2] > (int64_t)1 << 30) return hipErrorInvalidValue;  // a token's values are counted in 32 bits
   if (!int_table(b->pages) || !int_table(b->starts) || !int_table(b->lengths)) return hipErrorInvalidValue;
   const int64_t n = b->lengths.ne[0];
   if (n > INT32_MAX - 1 || b->lengths.ne[1] != 1 || b->starts.ne[0] != n + 1 || b->starts.ne[1] != 1 ||
