@@ -147,7 +147,7 @@ __device__ __forceinline__ bool locate(const AttendArgs& a, int tile, int token,
     int steps = 0;
     if (count > 0) steps = visible_range(a, (long long)length - count, (long long)length - 1).steps;
     longest = max(longest, wave_max_count(steps));
-    const int tiles = (count * a.share + a.tile - 1) / a.tile;
+    const int tiles = (int)(((unsigned)(count * a.share) + (unsigned)a.tile - 1) / (unsigned)a.tile);
     const int sum = wave_scan(tiles), all = __builtin_amdgcn_readlane(sum, kWave - 1);
     if (found < 0) {
       const unsigned long long hit = token < 0 ? __ballot(before + sum > tile)
