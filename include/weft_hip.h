@@ -300,7 +300,10 @@ enum {
   WEFT_GGML_TYPE_IQ2_XS = 17,
   WEFT_GGML_TYPE_I32 = 26,
   WEFT_GGML_TYPE_MXFP4 = 39,
-  WEFT_GGML_TYPE_NVFP4 = 40
+  WEFT_GGML_TYPE_NVFP4 = 40,
+  /* 8-bit floats (e4m3), whose scales are a tensor of their own; no GGML type, and outside
+   * GGML's range of ids */
+  WEFT_GGML_TYPE_F8_E4M3 = 4096
 };
 
 /* the fields of struct ggml_tensor (ggml/include/ggml.h:667-692) MUL_MAT reads */
@@ -417,6 +420,80 @@ int weft_ggml_attention(const weft_ggml_tensor *q, const weft_ggml_tensor *k_cac
                         const weft_ggml_tensor *v_cache, const weft_ggml_kv_batch *batch,
                         const weft_ggml_tensor *dst, float scale, int64_t window, int64_t sinks,
                         void *wdata, size_t wsize);
+
+/* ----------------------------------- 8-bit float products, and what is around them */
+/* No counterpart in the reference; as above, every call is stream-ordered, allocates
+ * nothing and returns 0 or the error it also records.
+ *
+ * F8_E4M3 codes are e4m3 numbers (largest 448, no infinity, NaN 0x7f) that a scale
+ * multiplies: value = code x scale, one F32 scale for each 128 values of a row (scales
+ * (ceil(K / 128), rows)) or for each block of 128 rows x 128 values (scales
+ * (ceil(K / 128), ceil(rows / 128))); blocks at the ends may be short.
+ *
+ * Quantizes x (K, rows; F32 or F16) into codes (F8_E4M3, the same shape) and scales (F32),
+ * whose shape says which of the two: with a = max(2^-100, the largest finite |x| of
+ * the block) in 32 bits, scale = a / 448, code = the e4m3 number nearest x (448 / a), ties to
+ * even; an x that is not finite becomes NaN.  Rows lie any whole elements apart, scales any
+ * whole floats. */
+int weft_ggml_quantize_f8(const weft_ggml_tensor *x, const weft_ggml_tensor *codes,
+                          const weft_ggml_tensor *scales);
+
+/* dst = w x: w (K, N; F8_E4M3) with w_scales (ceil(K / 128), ceil(N / 128); F32), x (K, M)
+ * as F32 or F16, quantized as above a row at a time (x_scales NULL), or as F8_E4M3 with
+ * x_scales (ceil(K / 128), M; F32); dst (N, M): F32 or F16.  K >= 1; rows lie any whole
+ * elements apart.  Products and sums have 32 bits; a block's sum is multiplied by the
+ * product of its two scales, which has to be finite in 32 bits and loses bits below 2^-126.
+ * NaN codes reach their row's outputs and no others.
+ * wdata: weft_ggml_mul_mat_f8_work_size bytes, 16-byte aligned (scratch; its content need
+ * not be kept or cleared); the size depends on the shapes and types only. */
+size_t weft_ggml_mul_mat_f8_work_size(const weft_ggml_tensor *w, const weft_ggml_tensor *x);
+int weft_ggml_mul_mat_f8(const weft_ggml_tensor *w, const weft_ggml_tensor *w_scales,
+                         const weft_ggml_tensor *x, const weft_ggml_tensor *x_scales,
+                         const weft_ggml_tensor *dst, void *wdata, size_t wsize);
+
+/* How heads are normed and turned. */
+typedef struct weft_ggml_head_rope {
+  int32_t normed;     /* 0: no norm (no weights then) */
+  int32_t n_rot;      /* values of a head that are turned, from its first; even, 0 for none */
+  int32_t neighbours; /* pairs are (2i, 2i + 1), else (i, i + n_rot / 2) */
+  float eps;
+  double base;        /* pair i turns base^(-2i / n_rot) a position, */
+  double scale;       /* times scale, over factors[i] */
+  double magnitude;   /* and turned values are multiplied by this */
+} weft_ggml_head_rope;
+
+/* Each head of q (D, heads, tokens) and k (D, kv heads, tokens; NULL for none), F32 or F16,
+ * normed over its D values (y = x / sqrt(mean(x^2) + eps) * weight) and its pairs (a, b)
+ * turned by the token's position p (positions, I32 (tokens)) to magnitude (a cos t - b sin t,
+ * a sin t + b cos t), t = p scale base^(-2i / n_rot) / factors[i], into q_dst and k_dst
+ * (same shapes, F32 or F16; a destination may be its source's own memory with its strides).
+ * q_weight, k_weight: F32 (D) or NULL (ones); factors: F32 (n_rot / 2) or NULL (ones);
+ * positions may be NULL if n_rot is 0.  D: at most 256; heads and tokens lie any whole
+ * elements apart.  Angles are reduced in 64 bits; sums have 32. */
+int weft_ggml_head_norm_rope(const weft_ggml_tensor *q, const weft_ggml_tensor *k,
+                             const weft_ggml_tensor *q_dst, const weft_ggml_tensor *k_dst,
+                             const weft_ggml_tensor *positions, const weft_ggml_head_rope *rope,
+                             const weft_ggml_tensor *q_weight, const weft_ggml_tensor *k_weight,
+                             const weft_ggml_tensor *factors);
+
+/* Of rows of logits (V, rows; F32 or F16), each times scale (> 0: one over a temperature):
+ * token_lp (n, rows; F32): the log probabilities of tokens (n, rows; I32); an id outside
+ * [0, V) leaves its output as it was;
+ * entropy (rows; F32), in nats;
+ * top_ids (I32), top_lp (F32; both (A, rows), A <= WEFT_GGML_MOST_ALTERNATIVES and <= V):
+ * the A largest logits' ids and log probabilities, largest first, of equal ones the lowest
+ * id.  Each may be NULL (tokens with token_lp, top_ids with top_lp).
+ * Logits of minus infinity have probability 0; a row of nothing else has log probabilities
+ * of minus infinity and entropy 0.  NaN or plus infinity makes its row's log
+ * probabilities and entropy NaN; NaN is no alternative (id -1 where no other is left).
+ * wdata: weft_ggml_log_probs_work_size(logits, A) bytes, 16-byte aligned (scratch); the size
+ * depends on the shapes only. */
+#define WEFT_GGML_MOST_ALTERNATIVES 64
+size_t weft_ggml_log_probs_work_size(const weft_ggml_tensor *logits, int64_t n_top);
+int weft_ggml_log_probs(const weft_ggml_tensor *logits, const weft_ggml_tensor *tokens,
+                        const weft_ggml_tensor *token_lp, const weft_ggml_tensor *entropy,
+                        const weft_ggml_tensor *top_ids, const weft_ggml_tensor *top_lp,
+                        float scale, void *wdata, size_t wsize);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,188 @@
+"""mul_mat_f8 against 64 bits (GPU).
+
+What 32 bits may do to an output, with A the sum of |x w| over its row: e4m3 products are
+exact; a block's 127 additions, cut or rounded, are off by 2^-23 A each at most; the
+product of the scales by 2^-24, and so is each of the additions of the blocks' sums, whatever
+their order.  16-bit outputs add 2^-11 of their size (2^-25 below 2^-14).  Rows that are
+quantized within the call are quantized by the same formula, bit for bit."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from tests._f8 import BLOCK, F8, F16, F32, VALUE, Rows, Scales, quantize, up, values
+from weft_amd import ggml as G
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(mass, want, k, t):
+    b = mass * (127 * 2.0 ** -23 + (2 + up(k)) * 2.0 ** -24) + 1e-37
+    return b + (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 if t == F16 else 0)
+
+
+class Case:
+    def __init__(self, hip, m, n, k, src=F32, dst=F32, seed=0, w_pad=0, x_pad=0, y_pad=0, w_offset=0, x_offset=0,
+                 y_offset=0, major=False, w=None, x=None):
+        self.hip, self.m, self.n, self.k, self.src, self.dst = hip, m, n, k, src, dst
+        rng = np.random.default_rng(seed + 31 * m + 7 * n + k)
+        if w is None:
+            w = (rng.standard_normal((n, k)) * 0.05 * np.exp(rng.standard_normal(n))[:, None]).astype(np.float32)
+        if x is None:
+            x = np.clip(rng.standard_normal((m, k)) * np.exp(rng.standard_normal(k)), -6e4, 6e4)
+        x = x.astype(np.float16 if src == F16 else np.float32)
+        self.w_codes, self.w_scales = quantize(w, BLOCK)
+        self.x_codes, self.x_scales = quantize(x.astype(np.float32), 1)
+        self.wd, self.wsd = Rows(hip, F8, self.w_codes, pad=w_pad, offset=w_offset), Scales(hip, self.w_scales, block_major=major, pad=2)
+        self.xd = Rows(hip, src, self.x_codes if src == F8 else x, pad=x_pad, offset=x_offset)
+        self.xsd = Scales(hip, self.x_scales, block_major=not major, pad=1) if src == F8 else None
+        self.yd = Rows(hip, dst, shape=(m, n), pad=y_pad, offset=y_offset)
+
+    def call(self):
+        hip = self.hip
+        size = G.mul_mat_f8_work_size(self.wd.tensor, self.xd.tensor)
+        self.work = hip.empty(size, fill=0x7f)
+        print(f"mul_mat_f8 m={self.m} n={self.n} k={self.k} src={self.src} dst={self.dst} work={size}", flush=True)
+        G.mul_mat_f8(self.wd.tensor, self.wsd.tensor, self.xd.tensor, self.xsd.tensor if self.xsd else None, self.yd.tensor,
+                     self.work.ptr, size)
+
+    def want(self):
+        w, x = values(self.w_codes, self.w_scales, BLOCK), values(self.x_codes, self.x_scales, 1)
+        return x @ w.T, np.abs(x) @ np.abs(w).T
+
+    def check(self):
+        self.call()
+        self.hip.torch.cuda.synchronize()
+        assert self.hip.last_error() == 0
+        got = self.yd.numpy().astype(np.float64)
+        want, mass = self.want()
+        nan = np.isnan(want)
+        assert np.array_equal(np.isnan(got), nan)
+        assert (np.abs(got - want)[~nan] <= bound(mass, want, self.k, self.dst)[~nan]).all()
+        return got
+
+
+TYPES = [(s, d) for s in (F32, F16, F8) for d in (F32, F16)]
+
+
+@pytest.mark.parametrize("src,dst", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 16, 128), (1, 17, 129), (2, 130, 48), (3, 33, 1000), (1, 300, 4096),
+                                   (7, 129, 513), (16, 64, 256), (17, 200, 640), (33, 257, 384), (40, 128, 2048),
+                                   (65, 131, 272), (130, 270, 400), (1, 5, 16400)])
+def test_sizes(hip, m, n, k, src, dst):
+    Case(hip, m, n, k, src, dst).check()
+
+
+@pytest.mark.parametrize("src,dst", TYPES)
+@pytest.mark.parametrize("m,n,k", [(256, 256, 512), (509, 515, 1111), (300, 1000, 1024), (1024, 384, 640), (129, 2049, 256),
+                                   (2000, 130, 144)])
+def test_many_tokens(hip, m, n, k, src, dst):
+    Case(hip, m, n, k, src, dst).check()
+
+
+@pytest.mark.parametrize("src", [F32, F16, F8])
+@pytest.mark.parametrize("m", [1, 5, 20, 70, 200, 600])
+def test_strides_and_alignment(hip, m, src):
+    e = {F32: 4, F16: 2, F8: 1}[src]
+    for kw in ({"w_pad": 16, "x_pad": 16, "y_pad": 4}, {"w_pad": 3, "x_pad": 5, "y_pad": 1, "major": True},
+               {"w_offset": 1, "x_offset": e, "y_offset": 4}, {"w_pad": 1, "w_offset": 7, "x_offset": 3 * e},
+               {"x_pad": 4, "x_offset": 16, "w_offset": 16}):
+        for dst, k in ((F32, 400), (F16, 401)):
+            Case(hip, m, 150, k, src, dst, **kw).check()
+
+
+@pytest.mark.parametrize("m", [1, 4, 37, 150, 700])
+def test_nan_and_infinity_stay_in_their_rows(hip, m):
+    """A NaN weight reaches its column of the result, a token's its row."""
+    rng = np.random.default_rng(m)
+    w, x = rng.standard_normal((270, 515)).astype(np.float32), rng.standard_normal((m, 515)).astype(np.float32)
+    w[3, 514], w[200, 0], x[m - 1, 130] = np.nan, np.inf, -np.inf
+    for src in (F32, F8):
+        got = Case(hip, m, 270, 515, src, w=w, x=x).check()
+        nan = np.isnan(got)
+        assert nan[:, [3, 200]].all() and nan[m - 1].all() and nan.sum() == 2 * m + 270 - 2
+
+
+@pytest.mark.parametrize("m", [1, 20, 300])
+def test_zeros_and_scales(hip, m):
+    """Blocks of zeros, scales of zero and large ones beside small ones."""
+    c = Case(hip, m, 140, 700, F8)
+    c.w_scales[0, 2] = 0
+    c.w_scales[1, 3] = 1e20
+    c.x_scales[0, 1] = 1e-20
+    c.x_codes[m - 1] = 0x80  # minus zero
+    c = Case2(hip, c)
+    c.check()
+
+
+def Case2(hip, c):
+    """The case again with its changed codes and scales on the device."""
+    c.wd, c.wsd = Rows(hip, F8, c.w_codes), Scales(hip, c.w_scales)
+    c.xd, c.xsd = Rows(hip, F8, c.x_codes), Scales(hip, c.x_scales)
+    return c
+
+
+@pytest.mark.parametrize("m", [1, 30, 300])
+def test_every_code(hip, m):
+    """Codes of every value against codes of every value, unit scales: sums of exact products."""
+    rng = np.random.default_rng(m)
+    c = Case(hip, m, 256, 256, F8)
+    finite = np.array([i for i in range(256) if np.isfinite(VALUE[i])], np.uint8)
+    c.w_codes = rng.permuted(np.resize(finite, (256, 256)), axis=1)
+    c.x_codes = rng.choice(finite, (m, 256))
+    c.w_scales[:], c.x_scales[:] = 1, 1
+    Case2(hip, c).check()
+    # one code a row: each product alone, in every place of a block
+    for k0 in range(0, 256, 37):
+        c.x_codes = np.zeros((m, 256), np.uint8)
+        c.x_codes[:, k0] = rng.choice(finite, m)
+        got = Case2(hip, c).check()
+        assert np.array_equal(got, np.float32(np.outer(VALUE[c.x_codes[:, k0]], VALUE[c.w_codes[:, k0]])))
+
+
+@pytest.mark.parametrize("m", [1, 8, 50, 400])
+def test_calls_agree_and_overlap(hip, m):
+    """The same call twice gives the same bits; calls on two streams, each with its own work buffer, do not meet."""
+    torch = hip.torch
+    cases = [Case(hip, m, 390, 1300, F32, seed=s) for s in (1, 2)]
+    first = [c.check() for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    try:
+        for _ in range(3):
+            for c, s in zip(cases, streams):
+                hip._lib.set_stream(s.cuda_stream)
+                c.call()
+    finally:
+        hip._lib.set_stream(torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    for c, f in zip(cases, first):
+        assert np.array_equal(c.yd.numpy().astype(np.float64), f)
+
+
+@pytest.mark.parametrize("m", [1, 24, 300])
+def test_a_graph_replayed_with_other_inputs(hip, m):
+    torch = hip.torch
+    c = Case(hip, m, 140, 500, F32)
+    c.check()
+    size = G.mul_mat_f8_work_size(c.wd.tensor, c.xd.tensor)
+    work = hip.empty(size, fill=0x7f)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=side):
+            hip._lib.set_stream(side.cuda_stream)
+            G.mul_mat_f8(c.wd.tensor, c.wsd.tensor, c.xd.tensor, None, c.yd.tensor, work.ptr, size)
+    finally:
+        hip._lib.set_stream(torch.cuda.current_stream().cuda_stream)
+    for seed in range(3):
+        x = np.random.default_rng(seed).standard_normal((m, 500)).astype(np.float32)
+        c.xd.dev.t[:x.nbytes].copy_(torch.from_numpy(x.view(np.uint8).reshape(-1)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = c.yd.numpy().copy()
+        c.x_codes, c.x_scales = quantize(x, 1)
+        want, mass = c.want()
+        assert (np.abs(got - want) <= bound(mass, want, 500, F32)).all()
+        c.call()
+        torch.cuda.synchronize()
+        assert np.array_equal(c.yd.numpy(), got)

@@ -117,7 +117,13 @@ def _bind_ggml(lib: ctypes.CDLL) -> None:
                             ("weft_ggml_kv_read", [vp, vp, vp, vp, vp], ctypes.c_int),
                             ("weft_ggml_attention_work_size", [vp, vp, vp, vp], sz),
                             ("weft_ggml_attention",
-                             [vp, vp, vp, vp, vp, ctypes.c_float, i64, i64, vp, sz], ctypes.c_int)):
+                             [vp, vp, vp, vp, vp, ctypes.c_float, i64, i64, vp, sz], ctypes.c_int),
+                            ("weft_ggml_quantize_f8", [vp, vp, vp], ctypes.c_int),
+                            ("weft_ggml_mul_mat_f8_work_size", [vp, vp], sz),
+                            ("weft_ggml_mul_mat_f8", [vp, vp, vp, vp, vp, vp, sz], ctypes.c_int),
+                            ("weft_ggml_head_norm_rope", [vp] * 9, ctypes.c_int),
+                            ("weft_ggml_log_probs_work_size", [vp, i64], sz),
+                            ("weft_ggml_log_probs", [vp, vp, vp, vp, vp, vp, ctypes.c_float, vp, sz], ctypes.c_int)):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, res
 

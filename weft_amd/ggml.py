@@ -1,6 +1,7 @@
 """GGML operator boundary of libweft_hip from Python: MUL_MAT / MUL_MAT_ID and,
-between them in a decoder layer, the residual norm, the paged key / value
-cache and the attention over it.
+between them in a decoder layer, the residual norm, the norm and rotation of
+heads, the paged key / value cache and the attention over it; the product of
+8-bit floats; log probabilities.
 
 ``Tensor`` is the part of ``struct ggml_tensor`` (ggml/include/ggml.h:667-692)
 that MUL_MAT reads: type id, ``ne``, byte strides ``nb`` and a device data
@@ -20,10 +21,11 @@ from . import _lib
 F32, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K, IQ2_XXS, I32, MXFP4, NVFP4 = 0, 2, 8, 12, 13, 14, 15, 16, 26, 39, 40
 Q4_1, Q8_1, IQ2_XS = 3, 9, 17
 F16 = 1  # activations and cache rows; no MUL_MAT type
+F8_E4M3 = 4096  # 8-bit floats with scales beside them: mul_mat_f8; no GGML type
 
 
 # bytes of the types that are no records and that MUL_MAT does not know
-_PLAIN = {I32: 4, F16: 2}
+_PLAIN = {I32: 4, F16: 2, F8_E4M3: 1}
 
 
 class Tensor(ctypes.Structure):
@@ -166,3 +168,72 @@ def attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, batch: KvBatch, dst: 
     _done(lib, lib.weft_ggml_attention(_ref(q), _ref(k_cache), _ref(v_cache), _ref(batch), _ref(dst), scale, window,
                                        sinks, wdata, wsize),
           "weft_ggml_attention")
+
+
+def quantize_f8(x: Tensor, codes: Tensor, scales: Tensor) -> None:
+    """Enqueue the quantization of rows x (K, rows; F32 or F16) to 8-bit floats:
+    ``scales`` of (ceil(K / 128), rows) is one for each 128 values of a row, of
+    (ceil(K / 128), ceil(rows / 128)) one for each block of 128 x 128 (weights)."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_quantize_f8(_ref(x), _ref(codes), _ref(scales)), "weft_ggml_quantize_f8")
+
+
+def mul_mat_f8_work_size(w: Tensor, x: Tensor) -> int:
+    return _lib.load().weft_ggml_mul_mat_f8_work_size(_ref(w), _ref(x))
+
+
+def mul_mat_f8(w: Tensor, w_scales: Tensor, x: Tensor, x_scales: Tensor | None, dst: Tensor, wdata: int = 0,
+               wsize: int = 0) -> None:
+    """Enqueue dst (N, M) = the product of weights w (K, N; 8-bit floats, scales by
+    blocks) with rows x (K, M): F32 or F16, quantized on the way, or 8-bit floats
+    with their x_scales."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_mul_mat_f8(_ref(w), _ref(w_scales), _ref(x), _ref(x_scales), _ref(dst), wdata, wsize),
+          "weft_ggml_mul_mat_f8")
+
+
+class HeadRope(ctypes.Structure):
+    """How heads are normed and turned (weft_ggml_head_rope); ``head_norm_rope`` sets
+    normed and eps."""
+    _fields_ = [("normed", ctypes.c_int32), ("n_rot", ctypes.c_int32), ("neighbours", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("base", ctypes.c_double), ("scale", ctypes.c_double),
+                ("magnitude", ctypes.c_double)]
+
+
+def head_rope(n_rot: int, neighbours: bool = False, base: float = 10000.0, scale: float = 1.0,
+              magnitude: float = 1.0) -> HeadRope:
+    """The rotation of a head's first n_rot values: pairs (i, i + n_rot / 2), or
+    neighbours (2i, 2i + 1), by position * scale * base^(-2i / n_rot)."""
+    return HeadRope(0, n_rot, neighbours, 0.0, base, scale, magnitude)
+
+
+def head_norm_rope(q: Tensor, k: Tensor | None, q_dst: Tensor, k_dst: Tensor | None, positions: Tensor | None,
+                   rope: HeadRope, eps: float | None = None, q_weight: Tensor | None = None,
+                   k_weight: Tensor | None = None, factors: Tensor | None = None) -> None:
+    """Enqueue the norm (unless eps is None) of every head of q and k (D, heads,
+    tokens) and its rotation by the tokens' positions (I32); a destination may be its
+    source.  factors (n_rot / 2) divide the pairs' frequencies."""
+    lib = _lib.load()
+    how = HeadRope(eps is not None, rope.n_rot, rope.neighbours, 0.0 if eps is None else eps, rope.base, rope.scale,
+                   rope.magnitude)
+    _done(lib, lib.weft_ggml_head_norm_rope(_ref(q), _ref(k), _ref(q_dst), _ref(k_dst), _ref(positions), _ref(how),
+                                            _ref(q_weight), _ref(k_weight), _ref(factors)),
+          "weft_ggml_head_norm_rope")
+
+
+MOST_ALTERNATIVES = 64
+
+
+def log_probs_work_size(logits: Tensor, n_top: int) -> int:
+    return _lib.load().weft_ggml_log_probs_work_size(_ref(logits), n_top)
+
+
+def log_probs(logits: Tensor, tokens: Tensor | None, token_lp: Tensor | None, entropy: Tensor | None,
+              top_ids: Tensor | None, top_lp: Tensor | None, scale: float = 1.0, wdata: int = 0, wsize: int = 0) -> None:
+    """Enqueue, for rows of logits (V, rows) times scale: the log probabilities of
+    tokens (n, rows), the rows' entropy and their largest logits' ids and log
+    probabilities (A, rows), largest first, of equal ones the lowest id."""
+    lib = _lib.load()
+    _done(lib, lib.weft_ggml_log_probs(_ref(logits), _ref(tokens), _ref(token_lp), _ref(entropy), _ref(top_ids),
+                                       _ref(top_lp), scale, wdata, wsize),
+          "weft_ggml_log_probs")
