@@ -112,5 +112,7 @@ struct F8Product {
 
 // The product for any sizes, strides and alignment: tiles of 16 weights, K split over the waves.
 void f8_few(const F8Product& p);
+// Tiles of many tokens through LDS.
+void f8_many(const F8Product& p);
 
 }  // namespace weft

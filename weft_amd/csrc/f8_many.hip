@@ -1,0 +1,375 @@
+// The product of 8-bit floats for many tokens: tiles of TN weights x TM tokens, K a block of
+// 128 values at a time.
+//
+// A step's rows (128 bytes each) and scales come to LDS by direct 16-byte loads some steps
+// ahead; a row's eight chunks of 16 bytes lie at places XORed with the row, so that the
+// rows of an operand read meet in different banks.  Waves own 32 x 32 parts of the tile:
+// a block's sums start at zero on the matrix pipe, then go to the part's sums times the two
+// scales, one multiply-add a value (a lane has one token, so one factor).
+//
+// kExact: operands are widened to 16-bit floats on their way from LDS, and products and sums
+// have 32 bits, at the rate of 16-bit products.  Else v_mfma_f32_32x32x64_f8f6f4 takes the codes as they
+// are, at twice the rate; measured on the device, it adds each eight products of a lane
+// after cutting them below 2^-13 of the largest one's power of two, and the rest in 32
+// bits.  Sums that end in a 16-bit output, whose own step is 2^-11, are taken so; 32-bit
+// outputs are exact.
+#include <algorithm>
+
+#include "f8.h"
+#include "runtime.h"
+
+namespace weft {
+
+__device__ uint4 g_f8_zeros;  // the chunks past a row's end
+
+namespace {
+
+typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+struct __attribute__((packed, aligned(1))) Bytes16 {
+  uint32_t w[4];
+};
+
+// 16 (4) bytes per lane from global straight into LDS: lane l writes [lds + 16 l, +16)
+// ([lds + 4 l, +4)).  The kernel waits itself; nothing else in it uses M0.
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(lds), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma16(const uint8_t* at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(at)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const float* at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(lds), "v"(at)
+               : "memory", "m0");
+}
+// The wave's own loads but the last N have arrived and its LDS reads are done; then all waves'.
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+__device__ __forceinline__ half8 halves(int lo, int hi) {
+  const half2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
+  const half2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
+  const half2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
+  const half2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
+  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
+struct Shape {
+  static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
+  static constexpr int RN = TN / WN / 32, RM = TM / WM / 32;  // 32 x 32 parts of a wave
+  static constexpr int kData = (TN + TM) * kF8Block;
+  static constexpr int kSlot = kData + (TM + kWave) * 4;  // and the tokens' scales, the weights'
+  static constexpr int kLds = STAGES * kSlot;
+  static constexpr int kLoadsN = TN / 8 / kWaves, kLoadsM = TM / 8 / kWaves, kLoads = kLoadsN + kLoadsM + 1;
+  static_assert(TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0 && TM / kWave + 1 <= kWaves, "whole loads");
+  static_assert(kDirect || STAGES == 2, "loads through registers fill the other slot");
+};
+
+// Tile t of tiles_m x tiles_n.  Workgroup b runs on XCD b % 8, so consecutive tiles are given
+// to one XCD; they are bands of eight token tiles, one weight tile after the other, so that
+// an XCD's 32 workgroups read 8 + 4 tiles through its L2.
+__device__ __forceinline__ void place(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int tiles = tiles_m * tiles_n, each = tiles / 8, rest = tiles % 8, x = b % 8;
+  int t = x * each + min(x, rest) + b / 8;
+  const int band = t / (8 * tiles_n);
+  t -= band * 8 * tiles_n;
+  const int wide = min(8, tiles_m - 8 * band);
+  tn = t / wide;
+  tm = 8 * band + t - tn * wide;
+}
+
+template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
+__global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int tiles_m, int tiles_n) {
+  using S = Shape<TN, TM, WN, WM, STAGES, kExact, kDirect>;
+  constexpr int RN = S::RN, RM = S::RM, LN = S::kLoadsN, LM = S::kLoadsM;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  int tm, tn;
+  place((int)blockIdx.x, tiles_m, tiles_n, tm, tn);
+  const int n0 = tn * TN, m0 = tm * TM;
+  const int blocks = (p.k + kF8Block - 1) / kF8Block;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)lds;
+
+  // ---- loads: unit i of a wave is rows 8 (i waves + wave) .. + 7 of the weights (tokens)
+  const int row8 = lane >> 3, chunk = (lane & 7) ^ row8;
+  const uint8_t* w_base = p.w.codes + n0 * p.w.row;
+  const uint8_t* x_base = p.x.codes + m0 * p.x.row;
+  // rows past the ends are read as the last one and not stored
+  auto w_row = [&](int i) { return min(n0 + 8 * (i * S::kWaves + wave) + row8, p.n - 1) - n0; };
+  auto x_row = [&](int i) { return min(m0 + 8 * (i * S::kWaves + wave) + row8, p.m - 1) - m0; };
+  uint32_t w_off[LN], x_off[LM];
+  if constexpr (kDirect) {
+#pragma unroll
+    for (int i = 0; i < LN; ++i) w_off[i] = (uint32_t)w_row(i) * (uint32_t)p.w.row + 16 * chunk;
+#pragma unroll
+    for (int i = 0; i < LM; ++i) x_off[i] = (uint32_t)x_row(i) * (uint32_t)p.x.row + 16 * chunk;
+  }
+  // waves below TM / 64 load tokens' scales, the others the weights' (the same ones)
+  const bool of_tokens = wave < TM / kWave;
+  const int w_blocks = (p.n + kF8Block - 1) / kF8Block;
+  const float* s_at = of_tokens ? p.x.scales + min(m0 + kWave * wave + lane, p.m - 1) * p.x.s_row
+                                : p.w.scales + min(n0 / kF8Block + lane, w_blocks - 1) * p.w.s_row;
+  const long long s_step = of_tokens ? p.x.s_block : p.w.s_block;
+  const uint32_t s_lds = S::kData + (of_tokens ? wave * kWave * 4 : TM * 4);
+
+  auto issue = [&](int b, int slot) {
+    const uint32_t to = lds0 + slot * S::kSlot;
+    const uint8_t* w = w_base + (long long)b * kF8Block;
+    const uint8_t* x = x_base + (long long)b * kF8Block;
+    if ((b + 1) * kF8Block <= p.k) {
+#pragma unroll
+      for (int i = 0; i < LN; ++i) dma16(w, w_off[i], to + (i * S::kWaves + wave) * 1024);
+#pragma unroll
+      for (int i = 0; i < LM; ++i) dma16(x, x_off[i], to + TN * kF8Block + (i * S::kWaves + wave) * 1024);
+    } else {  // chunks past k are zeros
+      const bool in = b * kF8Block + 16 * chunk < p.k;
+      const uint8_t* zeros = reinterpret_cast<const uint8_t*>(&g_f8_zeros);
+#pragma unroll
+      for (int i = 0; i < LN; ++i) dma16(in ? w + w_off[i] : zeros, to + (i * S::kWaves + wave) * 1024);
+#pragma unroll
+      for (int i = 0; i < LM; ++i) dma16(in ? x + x_off[i] : zeros, to + TN * kF8Block + (i * S::kWaves + wave) * 1024);
+    }
+    dma4(s_at + b * s_step, to + s_lds);
+  };
+
+  // ---- the same through registers, for rows of any alignment
+  uint4 held[kDirect ? 1 : LN + LM];
+  float held_scale = 0.f;
+  auto fetch1 = [&](const uint8_t* row, int b) {
+    const int left = p.k - b * kF8Block - 16 * chunk;
+    uint4 v = {0, 0, 0, 0};
+    const uint8_t* q = row + (long long)b * kF8Block + 16 * chunk;
+    if (left >= 16) {
+      const Bytes16 r = *reinterpret_cast<const Bytes16*>(q);
+      v = {r.w[0], r.w[1], r.w[2], r.w[3]};
+    } else if (left > 0) {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e < left) w[e / 4] |= (uint32_t)q[e] << (8 * (e & 3));
+      v = {w[0], w[1], w[2], w[3]};
+    }
+    return v;
+  };
+  auto fetch = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < LN; ++i) held[i] = fetch1(w_base + w_row(i) * p.w.row, b);
+#pragma unroll
+    for (int i = 0; i < LM; ++i) held[LN + i] = fetch1(x_base + x_row(i) * p.x.row, b);
+    held_scale = s_at[b * s_step];
+  };
+  auto put = [&](int slot) {
+    uint8_t* to = lds + slot * S::kSlot;
+#pragma unroll
+    for (int i = 0; i < LN; ++i) *reinterpret_cast<uint4*>(to + (i * S::kWaves + wave) * 1024 + 16 * lane) = held[i];
+#pragma unroll
+    for (int i = 0; i < LM; ++i)
+      *reinterpret_cast<uint4*>(to + TN * kF8Block + (i * S::kWaves + wave) * 1024 + 16 * lane) = held[LN + i];
+    *reinterpret_cast<float*>(to + s_lds + 4 * lane) = held_scale;
+  };
+
+  // ---- the wave's parts of the tile
+  const int r = lane & 31, h = lane >> 5;
+  const int wn = wave % WN, wm = wave / WN;
+  v16f acc[RN][RM] = {};
+  const v16f zero = {};
+  int place16[4];  // where a lane's chunks of a row lie: 16 bytes each of K 64 (c / 2) + 32 h + 16 (c & 1)
+#pragma unroll
+  for (int c = 0; c < 4; ++c) place16[c] = ((4 * (c >> 1) + 2 * h + (c & 1)) ^ (r & 7)) * 16;
+  auto operand = [&](const uint8_t* rows, int half) {
+    const int4 a = *reinterpret_cast<const int4*>(rows + place16[2 * half]);
+    const int4 b = *reinterpret_cast<const int4*>(rows + place16[2 * half + 1]);
+    return v8i{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  };
+  auto compute = [&](int slot) {
+    const uint8_t* w = lds + slot * S::kSlot + (wn * (TN / WN) + r) * kF8Block;
+    const uint8_t* x = lds + slot * S::kSlot + TN * kF8Block + (wm * (TM / WM) + r) * kF8Block;
+    const float* scales = reinterpret_cast<const float*>(lds + slot * S::kSlot + S::kData);
+    const float sw = scales[TM + wn * (TN / WN) / kF8Block];
+    float s[RM];
+#pragma unroll
+    for (int j = 0; j < RM; ++j) s[j] = sw * scales[wm * (TM / WM) + 32 * j + r];
+    if constexpr (kExact) {
+      half8 xh[RM][8];
+#pragma unroll
+      for (int j = 0; j < RM; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const v8i v = operand(x + 32 * j * kF8Block, half);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) xh[j][4 * half + q] = halves(v[2 * q], v[2 * q + 1]);
+        }
+#pragma unroll
+      for (int i = 0; i < RN; ++i) {
+        half8 wh[8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const v8i v = operand(w + 32 * i * kF8Block, half);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) wh[4 * half + q] = halves(v[2 * q], v[2 * q + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < RM; ++j) {
+          v16f c = zero;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(wh[q], xh[j][q], c, 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[e], s[j], acc[i][j][e]);
+        }
+      }
+    } else {
+      v8i xv[RM][2];
+#pragma unroll
+      for (int j = 0; j < RM; ++j)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) xv[j][half] = operand(x + 32 * j * kF8Block, half);
+#pragma unroll
+      for (int i = 0; i < RN; ++i) {
+        v8i wv[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) wv[half] = operand(w + 32 * i * kF8Block, half);
+#pragma unroll
+        for (int j = 0; j < RM; ++j) {
+          v16f c = zero;
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            // scales of 2^0 for every 32 values
+            c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[half], xv[j][half], c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[e], s[j], acc[i][j][e]);
+        }
+      }
+    }
+  };
+
+  if constexpr (kDirect) {
+#pragma unroll
+    for (int b = 0; b < STAGES - 1; ++b)
+      if (b < blocks) issue(b, b);
+    int slot = 0;
+    for (int b = 0; b < blocks; ++b) {
+      // step b has arrived when only the steps after it are on their way
+      if (b + STAGES - 1 <= blocks)
+        arrive<(STAGES - 2) * S::kLoads>();
+      else
+        arrive<0>();
+      // the slot of step b - 1, which every wave has left
+      if (b + STAGES - 1 < blocks) issue(b + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+      compute(slot);
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+  } else {
+    fetch(0);
+    put(0);
+    for (int b = 0; b < blocks; ++b) {
+      __syncthreads();
+      if (b + 1 < blocks) fetch(b + 1);
+      compute(b & 1);
+      if (b + 1 < blocks) put((b + 1) & 1);  // the slot of step b - 1, which every wave has left
+    }
+  }
+
+  // ---- a lane has weights 8 g + 4 h .. + 3 (g < 4) of token r of each part
+#pragma unroll
+  for (int j = 0; j < RM; ++j) {
+    const int m = m0 + wm * (TM / WM) + 32 * j + r;
+    if (m >= p.m) continue;
+    uint8_t* y = p.y + m * p.y_row;
+#pragma unroll
+    for (int i = 0; i < RN; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int n = n0 + wn * (TN / WN) + 32 * i + 8 * g + 4 * h;
+        const v16f& a = acc[i][j];
+        if (p.half_out) {
+          _Float16* q = reinterpret_cast<_Float16*>(y) + n;
+          const half4 v = {(_Float16)a[4 * g], (_Float16)a[4 * g + 1], (_Float16)a[4 * g + 2], (_Float16)a[4 * g + 3]};
+          if (n + 3 < p.n && (reinterpret_cast<uintptr_t>(q) & 7u) == 0) {
+            *reinterpret_cast<half4*>(q) = v;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < p.n) q[e] = v[e];
+          }
+        } else {
+          float* q = reinterpret_cast<float*>(y) + n;
+          if (n + 3 < p.n && (reinterpret_cast<uintptr_t>(q) & 15u) == 0) {
+            *reinterpret_cast<v4f*>(q) = v4f{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n + e < p.n) q[e] = a[4 * g + e];
+          }
+        }
+      }
+  }
+}
+
+template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
+void launch(const F8Product& p, const char* name) {
+  using S = Shape<TN, TM, WN, WM, STAGES, kExact, kDirect>;
+  const int tiles_m = (p.m + TM - 1) / TM, tiles_n = (p.n + TN - 1) / TN;
+  f8_many_kernel<TN, TM, WN, WM, STAGES, kExact, kDirect>
+      <<<dim3((unsigned)(tiles_m * tiles_n)), S::kThreads, S::kLds, current_stream()>>>(p, tiles_m, tiles_n);
+  check_launch(name);
+}
+
+}  // namespace
+
+void f8_many(const F8Product& all) {
+  const bool exact = !all.half_out;
+  // direct loads take rows in aligned chunks of 16 and 32-bit offsets in a tile
+  const bool direct = all.k % 16 == 0 && all.w.row % 16 == 0 && all.x.row % 16 == 0 && aligned(all.w.codes, 16) &&
+                      aligned(all.x.codes, 16) && all.w.row < (1 << 24) && all.x.row < (1 << 24);
+  // a launch has fewer than 2^31 threads
+  constexpr int kMost = 1 << 16;
+  for (int64_t m = 0; m < all.m; m += kMost)
+    for (int64_t n = 0; n < all.n; n += kMost) {
+      F8Product p = all;
+      p.m = (int)std::min<int64_t>(all.m - m, kMost);
+      p.n = (int)std::min<int64_t>(all.n - n, kMost);
+      p.x.codes += m * p.x.row;
+      p.x.scales += m * p.x.s_row;
+      p.w.codes += n * p.w.row;
+      p.w.scales += n / kF8Block * p.w.s_row;
+      p.y += m * p.y_row + n * (p.half_out ? 2 : 4);
+      const int64_t big = (int64_t)((p.m + 255) / 256) * ((p.n + 255) / 256);
+      const int64_t mid = (int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128);
+      if (!direct) {
+        if (exact)
+          launch<128, 128, 2, 2, 2, true, false>(p, "f8_many_kernel");
+        else
+          launch<128, 128, 2, 2, 2, false, false>(p, "f8_many_kernel");
+      } else if (exact) {
+        if (mid >= cu_count())
+          launch<128, 128, 2, 2, 2, true, true>(p, "f8_many_kernel");
+        else
+          launch<128, 64, 4, 1, 4, true, true>(p, "f8_many_kernel");
+      } else if (big >= cu_count()) {
+        launch<256, 256, 2, 4, 2, false, true>(p, "f8_many_kernel");
+      } else if (mid >= cu_count()) {
+        launch<128, 128, 2, 2, 4, false, true>(p, "f8_many_kernel");
+      } else {
+        launch<128, 64, 4, 1, 4, false, true>(p, "f8_many_kernel");
+      }
+    }
+}
+
+}  // namespace weft

@@ -95,7 +95,10 @@ hipError_t mul_mat_f8(const weft_ggml_tensor* w, const weft_ggml_tensor* w_scale
                      plan.pitch, (int)plan.pitch, scales, 1, m, m, (int)k);
     p.x = {codes, scales, plan.pitch, 1, m};
   }
-  f8_few(p);
+  if (m <= 64)
+    f8_few(p);
+  else
+    f8_many(p);
   return pending_error();
 }
 
