@@ -113,6 +113,9 @@ struct F8Product {
 // The product for any sizes, strides and alignment: tiles of 16 weights, K split over the waves.
 void f8_few(const F8Product& p);
 // Tiles of many tokens through LDS.
-void f8_many(const F8Product& p);
+size_t f8_many_work(int64_t m, int64_t n, int64_t k);  // bytes, of shapes alone
+void f8_many(const F8Product& p, float* work);
+// Up to so many tokens the first is taken.
+constexpr int64_t kF8Few = 64;
 
 }  // namespace weft

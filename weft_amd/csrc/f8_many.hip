@@ -95,8 +95,19 @@ __device__ __forceinline__ void place(int b, int tiles_m, int tiles_n, int& tm, 
   tm = 8 * band + t - tn * wide;
 }
 
+// Two waves a SIMD, so that all registers are plain ones: sums in the matrix pipe's own are
+// copied out one by one (two instructions a value).
+// K in `n` ranges of `each` blocks, whose sums go to [range][token][weight, pitch floats a token];
+// n == 1: straight to the output.
+struct Parts {
+  float* sums;
+  long long range;  // floats between ranges
+  int n, each, pitch;
+};
+
 template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
-__global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_many_kernel(F8Product p, Parts parts, int tiles_m,
+                                                                 int tiles_n) {
   using S = Shape<TN, TM, WN, WM, STAGES, kExact, kDirect>;
   constexpr int RN = S::RN, RM = S::RM, LN = S::kLoadsN, LM = S::kLoadsM;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -104,11 +115,12 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
   int tm, tn;
   place((int)blockIdx.x, tiles_m, tiles_n, tm, tn);
   const int n0 = tn * TN, m0 = tm * TM;
-  const int blocks = (p.k + kF8Block - 1) / kF8Block;
+  const int first = (int)blockIdx.y * parts.each;
+  const int blocks = min((p.k + kF8Block - 1) / kF8Block - first, parts.each);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_ptr)lds;
 
   // ---- loads: unit i of a wave is rows 8 (i waves + wave) .. + 7 of the weights (tokens)
-  const int row8 = lane >> 3, chunk = (lane & 7) ^ row8;
+  const int row8 = lane >> 3, chunk = (lane & 7) ^ (4 * (wave & 1) + (row8 >> 1));
   const uint8_t* w_base = p.w.codes + n0 * p.w.row;
   const uint8_t* x_base = p.x.codes + m0 * p.x.row;
   // rows past the ends are read as the last one and not stored
@@ -129,7 +141,8 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
   const long long s_step = of_tokens ? p.x.s_block : p.w.s_block;
   const uint32_t s_lds = S::kData + (of_tokens ? wave * kWave * 4 : TM * 4);
 
-  auto issue = [&](int b, int slot) {
+  auto issue = [&](int step, int slot) {
+    const int b = first + step;
     const uint32_t to = lds0 + slot * S::kSlot;
     const uint8_t* w = w_base + (long long)b * kF8Block;
     const uint8_t* x = x_base + (long long)b * kF8Block;
@@ -168,7 +181,8 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
     }
     return v;
   };
-  auto fetch = [&](int b) {
+  auto fetch = [&](int step) {
+    const int b = first + step;
 #pragma unroll
     for (int i = 0; i < LN; ++i) held[i] = fetch1(w_base + w_row(i) * p.w.row, b);
 #pragma unroll
@@ -192,7 +206,7 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
   const v16f zero = {};
   int place16[4];  // where a lane's chunks of a row lie: 16 bytes each of K 64 (c / 2) + 32 h + 16 (c & 1)
 #pragma unroll
-  for (int c = 0; c < 4; ++c) place16[c] = ((4 * (c >> 1) + 2 * h + (c & 1)) ^ (r & 7)) * 16;
+  for (int c = 0; c < 4; ++c) place16[c] = ((4 * (c >> 1) + 2 * h + (c & 1)) ^ (r >> 1 & 7)) * 16;
   auto operand = [&](const uint8_t* rows, int half) {
     const int4 a = *reinterpret_cast<const int4*>(rows + place16[2 * half]);
     const int4 b = *reinterpret_cast<const int4*>(rows + place16[2 * half + 1]);
@@ -202,11 +216,14 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
     const uint8_t* w = lds + slot * S::kSlot + (wn * (TN / WN) + r) * kF8Block;
     const uint8_t* x = lds + slot * S::kSlot + TN * kF8Block + (wm * (TM / WM) + r) * kF8Block;
     const float* scales = reinterpret_cast<const float*>(lds + slot * S::kSlot + S::kData);
-    const float sw = scales[TM + wn * (TN / WN) / kF8Block];
     float s[RM];
+    auto factors = [&] {
+      const float sw = scales[TM + wn * (TN / WN) / kF8Block];
 #pragma unroll
-    for (int j = 0; j < RM; ++j) s[j] = sw * scales[wm * (TM / WM) + 32 * j + r];
+      for (int j = 0; j < RM; ++j) s[j] = sw * scales[wm * (TM / WM) + 32 * j + r];
+    };
     if constexpr (kExact) {
+      factors();
       half8 xh[RM][8];
 #pragma unroll
       for (int j = 0; j < RM; ++j)
@@ -235,26 +252,55 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
         }
       }
     } else {
-      v8i xv[RM][2];
+      constexpr int kW = RN * RM > 4 ? 1 : 2;  // weights of the next part on their way, where registers hold them
+      v8i xv[RM][2], wv[kW][2];
 #pragma unroll
-      for (int j = 0; j < RM; ++j)
+      for (int half = 0; half < 2; ++half) {
+        wv[0][half] = operand(w, half);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) xv[j][half] = operand(x + 32 * j * kF8Block, half);
+        for (int j = 0; j < RM; ++j) xv[j][half] = operand(x + 32 * j * kF8Block, half);
+      }
+      float sw = scales[TM + wn * (TN / WN) / kF8Block];
 #pragma unroll
-      for (int i = 0; i < RN; ++i) {
-        v8i wv[2];
+      for (int j = 0; j < RM; ++j) s[j] = scales[wm * (TM / WM) + 32 * j + r];
+      __builtin_amdgcn_sched_barrier(0);
+      // a part's sums are added while the matrix pipe works on the next part
+      v16f c[2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) wv[half] = operand(w + 32 * i * kF8Block, half);
+      for (int q = 0; q <= RN * RM; ++q) {
+        if (q < RN * RM) {
+          const int i = q / RM, j = q % RM;
+          if (kW == 2 && j == 0 && i + 1 < RN) {
 #pragma unroll
-        for (int j = 0; j < RM; ++j) {
-          v16f c = zero;
+            for (int half = 0; half < 2; ++half) wv[(i + 1) % kW][half] = operand(w + 32 * (i + 1) * kF8Block, half);
+          }
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
+          for (int half = 0; half < 2; ++half) {
             // scales of 2^0 for every 32 values
-            c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[half], xv[j][half], c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+            c[q & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i % kW][half], xv[j][half], half ? c[q & 1] : zero, 0, 0,
+                                                                       0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+            if (q == 1 && half == 0) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[e], s[j], acc[i][j][e]);
+              for (int j = 0; j < RM; ++j) s[j] *= sw;
+            }
+            if (q > 0) {
+              const int i = (q - 1) / RM, j = (q - 1) % RM;
+#pragma unroll
+              for (int e = 8 * half; e < 8 * half + 8; ++e) acc[i][j][e] = fmaf(c[(q - 1) & 1][e], s[j], acc[i][j][e]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
         }
+        if (q == RN * RM) {
+          const int i = (q - 1) / RM, j = (q - 1) % RM;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[(q - 1) & 1][e], s[j], acc[i][j][e]);
+        }
+        if (kW == 1 && q < RN * RM && q % RM == RM - 1 && q / RM + 1 < RN) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) wv[0][half] = operand(w + 32 * (q / RM + 1) * kF8Block, half);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
@@ -292,13 +338,16 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
     const int m = m0 + wm * (TM / WM) + 32 * j + r;
     if (m >= p.m) continue;
     uint8_t* y = p.y + m * p.y_row;
+    float* sums = parts.sums + blockIdx.y * parts.range + (long long)m * parts.pitch;
 #pragma unroll
     for (int i = 0; i < RN; ++i)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int n = n0 + wn * (TN / WN) + 32 * i + 8 * g + 4 * h;
         const v16f& a = acc[i][j];
-        if (p.half_out) {
+        if (parts.n > 1) {
+          if (n < parts.pitch) *reinterpret_cast<v4f*>(sums + n) = v4f{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
+        } else if (p.half_out) {
           _Float16* q = reinterpret_cast<_Float16*>(y) + n;
           const half4 v = {(_Float16)a[4 * g], (_Float16)a[4 * g + 1], (_Float16)a[4 * g + 2], (_Float16)a[4 * g + 3]};
           if (n + 3 < p.n && (reinterpret_cast<uintptr_t>(q) & 7u) == 0) {
@@ -322,22 +371,106 @@ __global__ void __launch_bounds__(64 * WN * WM) f8_many_kernel(F8Product p, int 
   }
 }
 
+// The ranges' sums added in their order, four weights a thread.
+__global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, Parts parts) {
+  const int quads = parts.pitch / 4;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  const long long m = i / quads;
+  const int n = 4 * (int)(i - m * quads);
+  if (m >= p.m) return;
+  const float* at = parts.sums + m * parts.pitch + n;
+  v4f v = *reinterpret_cast<const v4f*>(at);
+  for (int s = 1; s < parts.n; ++s) v += *reinterpret_cast<const v4f*>(at + s * parts.range);
+  uint8_t* y = p.y + m * p.y_row;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= p.n) break;
+    if (p.half_out)
+      reinterpret_cast<_Float16*>(y)[n + e] = (_Float16)v[e];
+    else
+      reinterpret_cast<float*>(y)[n + e] = v[e];
+  }
+}
+
 template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
-void launch(const F8Product& p, const char* name) {
+void launch(const F8Product& p, const Parts& parts) {
   using S = Shape<TN, TM, WN, WM, STAGES, kExact, kDirect>;
   const int tiles_m = (p.m + TM - 1) / TM, tiles_n = (p.n + TN - 1) / TN;
   f8_many_kernel<TN, TM, WN, WM, STAGES, kExact, kDirect>
-      <<<dim3((unsigned)(tiles_m * tiles_n)), S::kThreads, S::kLds, current_stream()>>>(p, tiles_m, tiles_n);
-  check_launch(name);
+      <<<dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts.n), S::kThreads, S::kLds, current_stream()>>>(p, parts, tiles_m,
+                                                                                                       tiles_n);
+  check_launch("f8_many_kernel");
+}
+
+int pitch_of(int64_t n) { return (int)((n + 3) / 4 * 4); }
+
+// What a call takes: 256 x 256 tiles (16-bit outputs) when they fill the card, else tiles of
+// 128 weights x 64 or 128 tokens, two workgroups of them a CU, and ranges of K.
+struct Plan {
+  int tokens;  // of a tile: 256, 128 or 64
+  Parts parts;
+};
+
+// A step of a workgroup alone on its CU, and of one of several, in us (measured: 512 x 4096 x 4096,
+// one 64-token tile a CU 0.5; 1024 x 4096 x 4096, two 0.4 each, 128-token tiles 0.8 and 0.72;
+// twice that with operands widened); 3 us to begin; ranges are written and read
+// again at about 5.5 TB/s and joined by a launch of their own.  So 509 x 4101 x 11008 takes
+// three ranges of 128-token tiles (46.8 us; one range 76, 64-token tiles 59), 512 x 4096 x 4096
+// one of 64 (21.6; two of them 23.8, four of 128 26.0).
+Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
+  constexpr int kCus = 256;
+  const int64_t blocks = f8_blocks(k);
+  Plan best{};
+  best.tokens = 128;
+  best.parts.n = 1;
+  best.parts.each = (int)blocks;
+  if (!exact && ((m + 255) / 256) * ((n + 255) / 256) >= 200) {
+    best.tokens = 256;
+    return best;
+  }
+  double least = 0;
+  for (const int tokens : {64, 128}) {
+    const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + 127) / 128);
+    const double alone = (tokens == 64 ? 0.5 : 0.8) * (exact ? 2 : 1), shared = (tokens == 64 ? 0.4 : 0.72) * (exact ? 2 : 1);
+    for (int64_t want = 1; want <= 16 && (want == 1 || (tiles * want <= 2 * kCus && blocks >= 4 * want)); ++want) {
+      const int64_t each = (blocks + want - 1) / want, parts = (blocks + each - 1) / each;
+      const int64_t load = (tiles * parts + kCus - 1) / kCus;
+      double us = 3 + (double)each * (load == 1 ? alone : shared * (double)load);
+      if (parts > 1) us += 3 + (double)parts * (double)m * (double)n * 4 * 2 / 5.5e6;
+      if (least > 0 && us >= least) continue;
+      least = us;
+      best.tokens = tokens;
+      best.parts.n = (int)parts;
+      best.parts.each = (int)each;
+    }
+  }
+  if (best.parts.n > 1) {
+    best.parts.pitch = pitch_of(n);
+    best.parts.range = (long long)m * best.parts.pitch;
+  }
+  return best;
 }
 
 }  // namespace
 
-void f8_many(const F8Product& all) {
+size_t f8_many_work(int64_t m, int64_t n, int64_t k) {
+  // for either output type
+  size_t most = 0;
+  for (const bool exact : {false, true}) {
+    const Plan plan = plan_of(m, n, k, exact);
+    if (plan.parts.n > 1) most = std::max(most, (size_t)plan.parts.n * (size_t)plan.parts.range * sizeof(float));
+  }
+  return most;
+}
+
+void f8_many(const F8Product& all, float* work) {
   const bool exact = !all.half_out;
   // direct loads take rows in aligned chunks of 16 and 32-bit offsets in a tile
   const bool direct = all.k % 16 == 0 && all.w.row % 16 == 0 && all.x.row % 16 == 0 && aligned(all.w.codes, 16) &&
                       aligned(all.x.codes, 16) && all.w.row < (1 << 24) && all.x.row < (1 << 24);
+  Plan plan = plan_of(all.m, all.n, all.k, exact);
+  plan.parts.sums = work;
+  const Parts& parts = plan.parts;
   // a launch has fewer than 2^31 threads
   constexpr int kMost = 1 << 16;
   for (int64_t m = 0; m < all.m; m += kMost)
@@ -350,26 +483,29 @@ void f8_many(const F8Product& all) {
       p.w.codes += n * p.w.row;
       p.w.scales += n / kF8Block * p.w.s_row;
       p.y += m * p.y_row + n * (p.half_out ? 2 : 4);
-      const int64_t big = (int64_t)((p.m + 255) / 256) * ((p.n + 255) / 256);
-      const int64_t mid = (int64_t)((p.m + 127) / 128) * ((p.n + 127) / 128);
       if (!direct) {
         if (exact)
-          launch<128, 128, 2, 2, 2, true, false>(p, "f8_many_kernel");
+          launch<128, 128, 2, 2, 2, true, false>(p, parts);
         else
-          launch<128, 128, 2, 2, 2, false, false>(p, "f8_many_kernel");
+          launch<128, 128, 2, 2, 2, false, false>(p, parts);
       } else if (exact) {
-        if (mid >= cu_count())
-          launch<128, 128, 2, 2, 2, true, true>(p, "f8_many_kernel");
+        if (plan.tokens == 64)
+          launch<128, 64, 4, 1, 3, true, true>(p, parts);
         else
-          launch<128, 64, 4, 1, 4, true, true>(p, "f8_many_kernel");
-      } else if (big >= cu_count()) {
-        launch<256, 256, 2, 4, 2, false, true>(p, "f8_many_kernel");
-      } else if (mid >= cu_count()) {
-        launch<128, 128, 2, 2, 4, false, true>(p, "f8_many_kernel");
+          launch<128, 128, 2, 2, 2, true, true>(p, parts);
+      } else if (plan.tokens == 256) {
+        launch<256, 256, 2, 4, 2, false, true>(p, parts);
+      } else if (plan.tokens == 64) {
+        launch<128, 64, 4, 1, 3, false, true>(p, parts);
       } else {
-        launch<128, 64, 4, 1, 4, false, true>(p, "f8_many_kernel");
+        launch<128, 128, 2, 2, 2, false, true>(p, parts);
       }
     }
+  if (parts.n > 1) {
+    const int64_t threads = (int64_t)all.m * (parts.pitch / 4);
+    f8_join_kernel<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, current_stream()>>>(all, parts);
+    check_launch("f8_join_kernel");
+  }
 }
 
 }  // namespace weft

@@ -12,11 +12,12 @@ hipError_t fail(hipError_t e) {
   return e;
 }
 
-// An activation that arrives as plain rows is quantized into the work buffer: codes of whole
-// blocks (zeros past k), then scales, block-major.
+// The work buffer.  An activation that arrives as plain rows is quantized into it: codes of
+// whole blocks (zeros past k), then scales, block-major; then come the sums of K's ranges.
 struct Plan {
   int64_t pitch = 0;  // bytes of a row of codes; 0: the activation arrives quantized
   size_t scales = 0;  // where the scales begin
+  size_t sums = 0;    // where the sums do, 16-byte aligned
   size_t size = 0;
 };
 
@@ -28,6 +29,11 @@ bool plan_of(const weft_ggml_tensor* w, const weft_ggml_tensor* x, Plan* out) {
     p.pitch = f8_blocks(k) * kF8Block;
     p.scales = (size_t)m * (size_t)p.pitch;
     p.size = p.scales + (size_t)m * (size_t)f8_blocks(k) * sizeof(float);
+  }
+  if (m > kF8Few && n > 0) {
+    p.sums = (p.size + 15) / 16 * 16;
+    const size_t bytes = f8_many_work(m, n, k);
+    if (bytes > 0) p.size = p.sums + bytes;
   }
   if (m == 0 || n == 0) p.size = 0;
   *out = p;
@@ -95,10 +101,10 @@ hipError_t mul_mat_f8(const weft_ggml_tensor* w, const weft_ggml_tensor* w_scale
                      plan.pitch, (int)plan.pitch, scales, 1, m, m, (int)k);
     p.x = {codes, scales, plan.pitch, 1, m};
   }
-  if (m <= 64)
+  if (m <= kF8Few)
     f8_few(p);
   else
-    f8_many(p);
+    f8_many(p, reinterpret_cast<float*>(static_cast<uint8_t*>(wdata) + plan.sums));
   return pending_error();
 }
 
