@@ -110,12 +110,13 @@ struct F8Product {
   bool half_out;
 };
 
-// The product for any sizes, strides and alignment: tiles of 16 weights, K split over the waves.
-void f8_few(const F8Product& p);
-// Tiles of many tokens through LDS.
-size_t f8_many_work(int64_t m, int64_t n, int64_t k);  // bytes, of shapes alone
+// Up to 16 tokens: a tile of 16 weights a workgroup, K split over its waves.  plain: rows to be
+// quantized on the way (p.x is not read), where f8_few_quantizes.
+constexpr int64_t kF8Few = 16;
+bool f8_few_quantizes(int64_t m, int64_t k);
+void f8_few(const F8Product& p, const uint8_t* plain = nullptr, bool plain_half = false, long long plain_row = 0);
+// More: tiles of 32 to 256 tokens through LDS; work: f8_many_work bytes, of the shapes alone.
+size_t f8_many_work(int64_t m, int64_t n, int64_t k);
 void f8_many(const F8Product& p, float* work);
-// Up to so many tokens the first is taken.
-constexpr int64_t kF8Few = 64;
 
 }  // namespace weft

@@ -1,16 +1,23 @@
-// The product of 8-bit floats for few tokens (and for any sizes, strides and alignment):
+// The product of 8-bit floats for up to 16 tokens, for any strides and alignment:
 //   y[t][n] = sum over blocks b of  sx[t][b] sw[n / 128][b]  sum over k in b of x[t][k] w[n][k]
 //
 // e4m3 numbers are 16-bit floats, so a block's 128 values are four
 // v_mfma_f32_16x16x32_f16 of a tile of 16 weights (rows of the result) and 16 tokens
 // (columns), whose products are exact and whose sums have 32 bits.  The block's sums are
 // added to the tile's times the two scales, one multiply-add a value: a lane has one token,
-// so one scale.
+// so one factor.
 //
-// Lane l of a tile holds K values 32 (l / 16) .. + 31 of row l % 16, for weights and tokens
-// alike; which of them an instruction takes does not matter as both have the same.
+// Lane l of a tile holds two chunks of 16 of row l % 16's values, for weights and tokens alike;
+// which of them an instruction takes does not matter as both have the same.
 // The blocks of a row are dealt to the workgroup's waves in turn (its 16 rows are then read
 // as whole contiguous pieces) and their sums meet in LDS in the order of the waves.
+//
+// Bound by the reading of the weights and by latency: a launch, the tokens' codes (quantized
+// by each workgroup while its first weights are on their way: a launch of its own for 4096
+// values costs 3 us more), then a trip to memory for each of a wave's blocks.  One token and
+// 4096 x 4096 weights take 6.8 us (2.5 TB/s), 11008 x 4096 12.4 (3.6 TB/s), 4096 x 11008 11.3 (4.0).
+// Tried: two blocks a wave on their way at once (7.1, 13.8, 12.5), the next block's loads before a
+// block's products (6.9, 15.5, 11.2), 32 weights a wave (6.8, 14.5 and 11.3).
 #include <algorithm>
 
 #include "f8.h"
@@ -28,29 +35,32 @@ struct __attribute__((packed, aligned(1))) Bytes16 {
   int w[4];
 };
 
-// 32 codes of a row from p on, of which `left` are in the row; zeros behind.  kWide: rows in
-// aligned groups of 16, so that a group is wholly in the row or behind it.
+// A lane's 32 codes of a block of 128: chunks g and g + 4 of 16, so that a load's four lanes of
+// a row read 64 contiguous bytes.  p: the block's first code, left: codes of the row from there;
+// zeros behind it.  kWide: rows in aligned groups of 16, so that a chunk is wholly in the row or
+// behind it.
 template <bool kWide>
-__device__ __forceinline__ v8i load32(const uint8_t* p, int left) {
+__device__ __forceinline__ v8i load32(const uint8_t* p, int g, int left) {
   v8i v = {0, 0, 0, 0, 0, 0, 0, 0};
-  if constexpr (kWide) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (left > 16 * h) {
-        const int4 q = *reinterpret_cast<const int4*>(p + 16 * h);
-        v[4 * h] = q.x, v[4 * h + 1] = q.y, v[4 * h + 2] = q.z, v[4 * h + 3] = q.w;
+  for (int h = 0; h < 2; ++h) {
+    const int at = 64 * h + 16 * g;
+    if (kWide || left >= at + 16) {
+      if (left <= at) continue;
+      Bytes16 q;
+      if constexpr (kWide) {
+        const int4 w = *reinterpret_cast<const int4*>(p + at);
+        q = {{w.x, w.y, w.z, w.w}};
+      } else {
+        q = *reinterpret_cast<const Bytes16*>(p + at);
       }
-  } else if (left >= 32) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const Bytes16 q = *reinterpret_cast<const Bytes16*>(p + 16 * h);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[4 * h + e] = q.w[e];
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (e < left) v[e / 4] |= (int)((uint32_t)p[e] << (8 * (e & 3)));
+      for (int e = 0; e < 16; ++e)
+        if (at + e < left) v[4 * h + e / 4] |= (int)((uint32_t)p[at + e] << (8 * (e & 3)));
+    }
   }
   return v;
 }
@@ -64,72 +74,82 @@ __device__ __forceinline__ half8 halves(int lo, int hi) {
   return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-__device__ __forceinline__ v4f product16(v8i a, v8i b) {
-  v4f c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 8; i += 2)
-    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(a[i], a[i + 1]), halves(b[i], b[i + 1]), c, 0, 0, 0);
-  return c;
-}
+// Plain rows of tokens, for a workgroup that quantizes them itself.
+struct PlainRows {
+  const uint8_t* x;
+  long long row;  // bytes
+};
+enum Source { kCodes = 0, kF32 = 1, kF16 = 2 };
+constexpr int kFusedValues = 16384;  // of all tokens, at most
 
-template <int MT, bool kWide>
-__global__ void __launch_bounds__(1024) f8_few_kernel(F8Product p) {
-  extern __shared__ float sums[];  // [wave][token][16 weights]
+// From plain rows each workgroup quantizes all tokens into LDS, its first weights on their way
+// meanwhile.
+template <bool kWide, int kSource>
+__global__ void __launch_bounds__(1024) f8_few_kernel(F8Product p, PlainRows plain) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, waves = blockDim.x / kWave;
   const int r = lane & 15, g = lane >> 4;
-  const int n0 = (int)blockIdx.x * 16, m0 = (int)blockIdx.y * 16 * MT;
+  const int n0 = (int)blockIdx.x * 16;
   const int blocks = (p.k + kF8Block - 1) / kF8Block;
+  float* sums = lds;  // [wave][token][16 weights]
+  uint8_t* codes = reinterpret_cast<uint8_t*>(lds + waves * 256);
+  const int pitch = blocks * kF8Block + 16;  // rows of tokens meet in different banks
+  float* scales = reinterpret_cast<float*>(codes + p.m * pitch);
+
   // rows past the ends are read as the last one and not stored
-  const uint8_t* w = p.w.codes + min(n0 + r, p.n - 1) * p.w.row + 32 * g;
+  const int token = min(r, p.m - 1);
+  const uint8_t* w = p.w.codes + min(n0 + r, p.n - 1) * p.w.row;
   const float* sw = p.w.scales + (n0 / kF8Block) * p.w.s_row;
-  const uint8_t* x[MT];
-  const float* sx[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int token = min(m0 + 16 * t + r, p.m - 1);
-    x[t] = p.x.codes + token * p.x.row + 32 * g;
-    sx[t] = p.x.scales + token * p.x.s_row;
+  const uint8_t* x = kSource ? codes + token * pitch : p.x.codes + token * p.x.row;
+  const float* sx = kSource ? scales + token * blocks : p.x.scales + token * p.x.s_row;
+  const long long sx_block = kSource ? 1 : p.x.s_block;
+
+  v8i wv;
+  float swv;
+  auto load_weights = [&](int b) {
+    if (b >= blocks) return;
+    wv = load32<kWide>(w + (long long)b * kF8Block, g, p.k - b * kF8Block);
+    swv = sw[b * p.w.s_block];
+  };
+  load_weights(wave);
+
+  if constexpr (kSource != kCodes) {
+    const int part = threadIdx.x & 15;
+    for (int i = threadIdx.x / 16; i < p.m * blocks; i += blockDim.x / 16) {
+      const int t = i / blocks, b = i - t * blocks;
+      float v[8];
+      f8_load8<kSource == kF16>(plain.x + t * plain.row, b * kF8Block + 8 * part, p.k, v);
+      float scale;
+      const uint2 c = f8_quantize_16lanes(v, scale);
+      *reinterpret_cast<uint2*>(codes + t * pitch + b * kF8Block + 8 * part) = c;
+      if (part == 0) scales[i] = scale;
+    }
+    __syncthreads();
   }
-  v4f acc[MT] = {};
-  constexpr int U = 2;
-  for (int b0 = wave; b0 < blocks; b0 += U * waves) {
-    v8i wv[U], xv[U][MT];
-    float swv[U], sxv[U][MT];
+
+  v4f acc = {0.f, 0.f, 0.f, 0.f};
+  for (int b = wave; b < blocks; b += waves) {
+    if (b != wave) load_weights(b);
+    // codes quantized here are whole blocks
+    const v8i xv =
+        load32<kWide || kSource != kCodes>(x + (long long)b * kF8Block, g, kSource ? kF8Block : p.k - b * kF8Block);
+    const float s = swv * sx[b * sx_block];
+    v4f c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int b = b0 + u * waves;
-      if (b >= blocks) break;
-      const int left = p.k - b * kF8Block - 32 * g;
-      wv[u] = load32<kWide>(w + (long long)b * kF8Block, left);
-      swv[u] = sw[b * p.w.s_block];
+    for (int i = 0; i < 8; i += 2)
+      c = __builtin_amdgcn_mfma_f32_16x16x32_f16(halves(wv[i], wv[i + 1]), halves(xv[i], xv[i + 1]), c, 0, 0, 0);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        xv[u][t] = load32<kWide>(x[t] + (long long)b * kF8Block, left);
-        sxv[u][t] = sx[t][b * p.x.s_block];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (b0 + u * waves >= blocks) break;
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const v4f c = product16(wv[u], xv[u][t]);
-        const float s = swv[u] * sxv[u][t];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(c[i], s, acc[t][i]);
-      }
-    }
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf(c[e], s, acc[e]);
   }
   // lane l has weights 4 (l / 16) .. + 3 of token l % 16
-#pragma unroll
-  for (int t = 0; t < MT; ++t) *reinterpret_cast<v4f*>(sums + ((wave * MT + t) * 16 + r) * 16 + 4 * g) = acc[t];
+  *reinterpret_cast<v4f*>(sums + (wave * 16 + r) * 16 + 4 * g) = acc;
   __syncthreads();
-  for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
+  for (int i = threadIdx.x; i < 256; i += blockDim.x) {
     float v = 0.f;
-    for (int s = 0; s < waves; ++s) v += sums[s * MT * 256 + i];
-    const int token = m0 + i / 16, n = n0 + (i & 15);
-    if (token >= p.m || n >= p.n) continue;
-    uint8_t* at = p.y + token * p.y_row;
+    for (int s = 0; s < waves; ++s) v += sums[s * 256 + i];
+    const int t = i / 16, n = n0 + i % 16;
+    if (t >= p.m || n >= p.n) continue;
+    uint8_t* at = p.y + t * p.y_row;
     if (p.half_out)
       reinterpret_cast<_Float16*>(at)[n] = (_Float16)v;
     else
@@ -137,43 +157,45 @@ __global__ void __launch_bounds__(1024) f8_few_kernel(F8Product p) {
   }
 }
 
-template <int MT>
-void launch(const F8Product& p, bool wide, dim3 grid, int waves) {
-  const size_t lds = (size_t)waves * MT * 256 * sizeof(float);
+template <int kSource>
+void launch(const F8Product& p, const PlainRows& plain, bool wide) {
+  const int blocks = (int)f8_blocks(p.k), tiles = (p.n + 15) / 16;
+  // 16 waves up to two workgroups a CU, 8 past that (us, 16 and 8: 4096 x 11008 11.3 and 12.4,
+  // 1000 x 16384 11.5 and 13.2; 11008 x 4096 14.5 and 12.4)
+  int waves = tiles <= 512 ? 16 : 8;
+  while (waves > 1 && waves / 2 >= blocks) waves /= 2;
+  size_t lds = (size_t)waves * 256 * sizeof(float);
+  if (kSource) lds += (size_t)p.m * ((size_t)blocks * kF8Block + 16 + blocks * sizeof(float));
   if (wide)
-    f8_few_kernel<MT, true><<<grid, waves * kWave, lds, current_stream()>>>(p);
+    f8_few_kernel<true, kSource><<<dim3((unsigned)tiles), waves * kWave, lds, current_stream()>>>(p, plain);
   else
-    f8_few_kernel<MT, false><<<grid, waves * kWave, lds, current_stream()>>>(p);
+    f8_few_kernel<false, kSource><<<dim3((unsigned)tiles), waves * kWave, lds, current_stream()>>>(p, plain);
   check_launch("f8_few_kernel");
 }
 
 }  // namespace
 
-void f8_few(const F8Product& all) {
-  const int blocks = (int)f8_blocks(all.k);
-  int waves = 1;
-  while (waves < 8 && waves < blocks) waves *= 2;
-  const bool wide = all.k % 16 == 0 && all.w.row % 16 == 0 && all.x.row % 16 == 0 && aligned(all.w.codes, 16) &&
-                    aligned(all.x.codes, 16);
-  // a launch has fewer than 2^32 threads, and 65535 groups in y
-  constexpr int kMostN = 1 << 20, kMostM = 1 << 15;
-  for (int64_t m = 0; m < all.m; m += kMostM)
-    for (int64_t n = 0; n < all.n; n += kMostN) {
-      F8Product p = all;
-      p.m = (int)std::min<int64_t>(all.m - m, kMostM);
-      p.n = (int)std::min<int64_t>(all.n - n, kMostN);
-      p.x.codes += m * p.x.row;
-      p.x.scales += m * p.x.s_row;
-      p.w.codes += n * p.w.row;
-      p.w.scales += n / kF8Block * p.w.s_row;
-      p.y += m * p.y_row + n * (p.half_out ? 2 : 4);
-      const int tiles = (p.m + 15) / 16;
-      const unsigned gx = (unsigned)((p.n + 15) / 16);
-      if (tiles == 1)
-        launch<1>(p, wide, dim3(gx, 1), waves);
-      else
-        launch<2>(p, wide, dim3(gx, (unsigned)((tiles + 1) / 2)), waves);
-    }
+bool f8_few_quantizes(int64_t m, int64_t k) { return m <= kF8Few && m * f8_blocks(k) * kF8Block <= kFusedValues; }
+
+void f8_few(const F8Product& all, const uint8_t* plain, bool plain_half, long long plain_row) {
+  const bool wide_w = all.k % 16 == 0 && all.w.row % 16 == 0 && aligned(all.w.codes, 16);
+  const bool wide = wide_w && (plain != nullptr || (all.x.row % 16 == 0 && aligned(all.x.codes, 16)));
+  // a launch has fewer than 2^32 threads
+  constexpr int kMostN = 1 << 24;
+  for (int64_t n = 0; n < all.n; n += kMostN) {
+    F8Product p = all;
+    p.n = (int)std::min<int64_t>(all.n - n, kMostN);
+    p.w.codes += n * p.w.row;
+    p.w.scales += n / kF8Block * p.w.s_row;
+    p.y += n * (p.half_out ? 2 : 4);
+    const PlainRows rows{plain, plain_row};
+    if (plain == nullptr)
+      launch<kCodes>(p, rows, wide);
+    else if (plain_half)
+      launch<kF16>(p, rows, wide);
+    else
+      launch<kF32>(p, rows, wide);
+  }
 }
 
 }  // namespace weft

@@ -75,10 +75,11 @@ struct Shape {
   static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
   static constexpr int RN = TN / WN / 32, RM = TM / WM / 32;  // 32 x 32 parts of a wave
   static constexpr int kData = (TN + TM) * kF8Block;
-  static constexpr int kSlot = kData + (TM + kWave) * 4;  // and the tokens' scales, the weights'
+  static constexpr int kTokenWaves = (TM + kWave - 1) / kWave;  // which load the tokens' scales
+  static constexpr int kSlot = kData + (kTokenWaves + 1) * kWave * 4;  // and the tokens' scales, the weights'
   static constexpr int kLds = STAGES * kSlot;
   static constexpr int kLoadsN = TN / 8 / kWaves, kLoadsM = TM / 8 / kWaves, kLoads = kLoadsN + kLoadsM + 1;
-  static_assert(TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0 && TM / kWave + 1 <= kWaves, "whole loads");
+  static_assert(TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0 && kTokenWaves + 1 <= kWaves, "whole loads");
   static_assert(kDirect || STAGES == 2, "loads through registers fill the other slot");
 };
 
@@ -133,13 +134,13 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
 #pragma unroll
     for (int i = 0; i < LM; ++i) x_off[i] = (uint32_t)x_row(i) * (uint32_t)p.x.row + 16 * chunk;
   }
-  // waves below TM / 64 load tokens' scales, the others the weights' (the same ones)
-  const bool of_tokens = wave < TM / kWave;
+  // the first waves load tokens' scales, the others the weights' (the same ones)
+  const bool of_tokens = wave < S::kTokenWaves;
   const int w_blocks = (p.n + kF8Block - 1) / kF8Block;
   const float* s_at = of_tokens ? p.x.scales + min(m0 + kWave * wave + lane, p.m - 1) * p.x.s_row
                                 : p.w.scales + min(n0 / kF8Block + lane, w_blocks - 1) * p.w.s_row;
   const long long s_step = of_tokens ? p.x.s_block : p.w.s_block;
-  const uint32_t s_lds = S::kData + (of_tokens ? wave * kWave * 4 : TM * 4);
+  const uint32_t s_lds = S::kData + (of_tokens ? wave : S::kTokenWaves) * kWave * 4;
 
   auto issue = [&](int step, int slot) {
     const int b = first + step;
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
     const float* scales = reinterpret_cast<const float*>(lds + slot * S::kSlot + S::kData);
     float s[RM];
     auto factors = [&] {
-      const float sw = scales[TM + wn * (TN / WN) / kF8Block];
+      const float sw = scales[S::kTokenWaves * kWave + wn * (TN / WN) / kF8Block];
 #pragma unroll
       for (int j = 0; j < RM; ++j) s[j] = sw * scales[wm * (TM / WM) + 32 * j + r];
     };
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
 #pragma unroll
         for (int j = 0; j < RM; ++j) xv[j][half] = operand(x + 32 * j * kF8Block, half);
       }
-      float sw = scales[TM + wn * (TN / WN) / kF8Block];
+      float sw = scales[S::kTokenWaves * kWave + wn * (TN / WN) / kF8Block];
 #pragma unroll
       for (int j = 0; j < RM; ++j) s[j] = scales[wm * (TM / WM) + 32 * j + r];
       __builtin_amdgcn_sched_barrier(0);
@@ -279,7 +280,7 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
             // scales of 2^0 for every 32 values
             c[q & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i % kW][half], xv[j][half], half ? c[q & 1] : zero, 0, 0,
                                                                        0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-            if (q == 1 && half == 0) {
+            if (q == 0 && half == 1) {
 #pragma unroll
               for (int j = 0; j < RM; ++j) s[j] *= sw;
             }
@@ -407,12 +408,13 @@ int pitch_of(int64_t n) { return (int)((n + 3) / 4 * 4); }
 // What a call takes: 256 x 256 tiles (16-bit outputs) when they fill the card, else tiles of
 // 128 weights x 64 or 128 tokens, two workgroups of them a CU, and ranges of K.
 struct Plan {
-  int tokens;  // of a tile: 256, 128 or 64
+  int tokens;  // of a tile: 256, 128, 64 or 32
   Parts parts;
 };
 
 // A step of a workgroup alone on its CU, and of one of several, in us (measured: 512 x 4096 x 4096,
-// one 64-token tile a CU 0.5; 1024 x 4096 x 4096, two 0.4 each, 128-token tiles 0.8 and 0.72;
+// one 64-token tile a CU 0.5; 1024 x 4096 x 4096, two 0.4 each, 128-token tiles 0.8 and 0.72, 32-token ones
+// 0.4 and 0.3;
 // twice that with operands widened); 3 us to begin; ranges are written and read
 // again at about 5.5 TB/s and joined by a launch of their own.  So 509 x 4101 x 11008 takes
 // three ranges of 128-token tiles (46.8 us; one range 76, 64-token tiles 59), 512 x 4096 x 4096
@@ -429,9 +431,10 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
     return best;
   }
   double least = 0;
-  for (const int tokens : {64, 128}) {
+  for (const int tokens : {32, 64, 128}) {
     const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + 127) / 128);
-    const double alone = (tokens == 64 ? 0.5 : 0.8) * (exact ? 2 : 1), shared = (tokens == 64 ? 0.4 : 0.72) * (exact ? 2 : 1);
+    const double alone = (tokens == 32 ? 0.4 : tokens == 64 ? 0.5 : 0.8) * (exact ? 2 : 1);
+    const double shared = (tokens == 32 ? 0.3 : tokens == 64 ? 0.4 : 0.72) * (exact ? 2 : 1);
     for (int64_t want = 1; want <= 16 && (want == 1 || (tiles * want <= 2 * kCus && blocks >= 4 * want)); ++want) {
       const int64_t each = (blocks + want - 1) / want, parts = (blocks + each - 1) / each;
       const int64_t load = (tiles * parts + kCus - 1) / kCus;
@@ -489,12 +492,16 @@ void f8_many(const F8Product& all, float* work) {
         else
           launch<128, 128, 2, 2, 2, false, false>(p, parts);
       } else if (exact) {
-        if (plan.tokens == 64)
+        if (plan.tokens == 32)
+          launch<128, 32, 4, 1, 3, true, true>(p, parts);
+        else if (plan.tokens == 64)
           launch<128, 64, 4, 1, 3, true, true>(p, parts);
         else
           launch<128, 128, 2, 2, 2, true, true>(p, parts);
       } else if (plan.tokens == 256) {
         launch<256, 256, 2, 4, 2, false, true>(p, parts);
+      } else if (plan.tokens == 32) {
+        launch<128, 32, 4, 1, 3, false, true>(p, parts);
       } else if (plan.tokens == 64) {
         launch<128, 64, 4, 1, 3, false, true>(p, parts);
       } else {

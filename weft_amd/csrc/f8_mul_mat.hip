@@ -15,7 +15,7 @@ hipError_t fail(hipError_t e) {
 // The work buffer.  An activation that arrives as plain rows is quantized into it: codes of
 // whole blocks (zeros past k), then scales, block-major; then come the sums of K's ranges.
 struct Plan {
-  int64_t pitch = 0;  // bytes of a row of codes; 0: the activation arrives quantized
+  int64_t pitch = 0;  // bytes of a row of codes; 0: the activation arrives quantized, or the product's kernel does it
   size_t scales = 0;  // where the scales begin
   size_t sums = 0;    // where the sums do, 16-byte aligned
   size_t size = 0;
@@ -25,7 +25,7 @@ bool plan_of(const weft_ggml_tensor* w, const weft_ggml_tensor* x, Plan* out) {
   const int64_t k = w->ne[0], n = w->ne[1], m = x->ne[1];
   if (k < 1 || n < 0 || m < 0 || k > INT32_MAX / 2 || n > INT32_MAX || m > INT32_MAX || x->ne[0] != k) return false;
   Plan p;
-  if (x->type != WEFT_GGML_TYPE_F8_E4M3) {
+  if (x->type != WEFT_GGML_TYPE_F8_E4M3 && !f8_few_quantizes(m, k)) {
     p.pitch = f8_blocks(k) * kF8Block;
     p.scales = (size_t)m * (size_t)p.pitch;
     p.size = p.scales + (size_t)m * (size_t)f8_blocks(k) * sizeof(float);
@@ -94,6 +94,9 @@ hipError_t mul_mat_f8(const weft_ggml_tensor* w, const weft_ggml_tensor* w_scale
   p.half_out = dst->type == WEFT_GGML_TYPE_F16;
   if (quantized) {
     p.x = rows_of(x, x_scales);
+  } else if (plan.pitch == 0) {
+    f8_few(p, static_cast<const uint8_t*>(x->data), x->type == WEFT_GGML_TYPE_F16, (long long)x->nb[1]);
+    return pending_error();
   } else {
     uint8_t* codes = static_cast<uint8_t*>(wdata);
     float* scales = reinterpret_cast<float*>(codes + plan.scales);
