@@ -451,30 +451,28 @@ int weft_ggml_mul_mat_f8(const weft_ggml_tensor *w, const weft_ggml_tensor *w_sc
                          const weft_ggml_tensor *x, const weft_ggml_tensor *x_scales,
                          const weft_ggml_tensor *dst, void *wdata, size_t wsize);
 
-/* How heads are normed and turned. */
+/* How heads are turned. */
 typedef struct weft_ggml_head_rope {
-  int32_t normed;     /* 0: no norm (no weights then) */
   int32_t n_rot;      /* values of a head that are turned, from its first; even, 0 for none */
   int32_t neighbours; /* pairs are (2i, 2i + 1), else (i, i + n_rot / 2) */
-  float eps;
   double base;        /* pair i turns base^(-2i / n_rot) a position, */
   double scale;       /* times scale, over factors[i] */
   double magnitude;   /* and turned values are multiplied by this */
 } weft_ggml_head_rope;
 
 /* Each head of q (D, heads, tokens) and k (D, kv heads, tokens; NULL for none), F32 or F16,
- * normed over its D values (y = x / sqrt(mean(x^2) + eps) * weight) and its pairs (a, b)
+ * normed over its D values if `normed` (y = x / sqrt(mean(x^2) + eps) * weight) and its pairs (a, b)
  * turned by the token's position p (positions, I32 (tokens)) to magnitude (a cos t - b sin t,
  * a sin t + b cos t), t = p scale base^(-2i / n_rot) / factors[i], into q_dst and k_dst
  * (same shapes, F32 or F16; a destination may be its source's own memory with its strides).
- * q_weight, k_weight: F32 (D) or NULL (ones); factors: F32 (n_rot / 2) or NULL (ones);
+ * q_weight, k_weight: F32 (D) or NULL (ones; NULL without the norm); factors: F32 (n_rot / 2) or NULL (ones);
  * positions may be NULL if n_rot is 0.  D: at most 256; heads and tokens lie any whole
  * elements apart.  Angles are reduced in 64 bits; sums have 32. */
 int weft_ggml_head_norm_rope(const weft_ggml_tensor *q, const weft_ggml_tensor *k,
                              const weft_ggml_tensor *q_dst, const weft_ggml_tensor *k_dst,
                              const weft_ggml_tensor *positions, const weft_ggml_head_rope *rope,
-                             const weft_ggml_tensor *q_weight, const weft_ggml_tensor *k_weight,
-                             const weft_ggml_tensor *factors);
+                             int32_t normed, float eps, const weft_ggml_tensor *q_weight,
+                             const weft_ggml_tensor *k_weight, const weft_ggml_tensor *factors);
 
 /* Of rows of logits (V, rows; F32 or F16), each times scale (> 0: one over a temperature):
  * token_lp (n, rows; F32): the log probabilities of tokens (n, rows; I32); an id outside

@@ -121,7 +121,7 @@ def _bind_ggml(lib: ctypes.CDLL) -> None:
                             ("weft_ggml_quantize_f8", [vp, vp, vp], ctypes.c_int),
                             ("weft_ggml_mul_mat_f8_work_size", [vp, vp], sz),
                             ("weft_ggml_mul_mat_f8", [vp, vp, vp, vp, vp, vp, sz], ctypes.c_int),
-                            ("weft_ggml_head_norm_rope", [vp] * 9, ctypes.c_int),
+                            ("weft_ggml_head_norm_rope", [vp] * 6 + [i32, ctypes.c_float] + [vp] * 3, ctypes.c_int),
                             ("weft_ggml_log_probs_work_size", [vp, i64], sz),
                             ("weft_ggml_log_probs", [vp, vp, vp, vp, vp, vp, ctypes.c_float, vp, sz], ctypes.c_int)):
         fn = getattr(lib, name)

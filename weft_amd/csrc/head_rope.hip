@@ -250,7 +250,7 @@ bool vector_of(const weft_ggml_tensor* t, int64_t n) {
 
 hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, const weft_ggml_tensor* q_dst,
                           const weft_ggml_tensor* k_dst, const weft_ggml_tensor* positions, const weft_ggml_head_rope* r,
-                          const weft_ggml_tensor* q_weight, const weft_ggml_tensor* k_weight,
+                          bool normed, float eps, const weft_ggml_tensor* q_weight, const weft_ggml_tensor* k_weight,
                           const weft_ggml_tensor* factors) {
   if (q == nullptr || q_dst == nullptr || r == nullptr || (k == nullptr) != (k_dst == nullptr))
     return fail(hipErrorInvalidValue);
@@ -264,7 +264,7 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
   if (d < 1 || tokens < 0 || tokens > INT32_MAX) return fail(hipErrorInvalidValue);
   if (d > kMostHead) return fail(hipErrorNotSupported);
   if (r->n_rot < 0 || r->n_rot > d || r->n_rot % 2) return fail(hipErrorInvalidValue);
-  if (r->normed ? !(r->eps >= 0.f) : (q_weight != nullptr || k_weight != nullptr)) return fail(hipErrorInvalidValue);
+  if (normed ? !(eps >= 0.f) : (q_weight != nullptr || k_weight != nullptr)) return fail(hipErrorInvalidValue);
   if (r->n_rot > 0 && (!(r->base > 0) || !std::isfinite(r->base) || !std::isfinite(r->scale) || !std::isfinite(r->magnitude)))
     return fail(hipErrorInvalidValue);
   const size_t in = q->type == WEFT_GGML_TYPE_F32 ? 4 : 2, out = q_dst->type == WEFT_GGML_TYPE_F32 ? 4 : 2;
@@ -296,9 +296,9 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
   a.d = (int)d;
   a.n_rot = r->n_rot;
   a.tokens = tokens;
-  a.normed = r->normed != 0;
+  a.normed = normed;
   a.neighbours = r->neighbours != 0;
-  a.eps = r->eps;
+  a.eps = eps;
   if (r->n_rot > 0) {
     a.positions = static_cast<const int32_t*>(positions->data);
     a.factors = factors != nullptr ? static_cast<const float*>(factors->data) : nullptr;
@@ -331,7 +331,7 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
 extern "C" int weft_ggml_head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k,
                                         const weft_ggml_tensor* q_dst, const weft_ggml_tensor* k_dst,
                                         const weft_ggml_tensor* positions, const weft_ggml_head_rope* rope,
-                                        const weft_ggml_tensor* q_weight, const weft_ggml_tensor* k_weight,
-                                        const weft_ggml_tensor* factors) {
-  return (int)weft::head_norm_rope(q, k, q_dst, k_dst, positions, rope, q_weight, k_weight, factors);
+                                        int32_t normed, float eps, const weft_ggml_tensor* q_weight,
+                                        const weft_ggml_tensor* k_weight, const weft_ggml_tensor* factors) {
+  return (int)weft::head_norm_rope(q, k, q_dst, k_dst, positions, rope, normed != 0, eps, q_weight, k_weight, factors);
 }

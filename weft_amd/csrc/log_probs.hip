@@ -10,11 +10,14 @@
 //
 // The largest logits: each wave keeps the 64 best of its values sorted, one a lane, as
 // 64-bit keys of the value and the inverted index, so that of equal values the first wins.
-// In its first chunk the n-th largest of the lanes' own maxima bounds the n-th largest value
-// from below (n lanes have a value that large); later chunks are compared with the list's
-// n-th.  What passes goes to LDS and is sorted into the list 64 at a time.
+// Only few values are looked at: in the first chunk, with w waves and n asked for, each wave takes the
+// p-th largest of its lanes' maxima (p = ceil(n / w)) and all the ceil(n / p)-th largest of
+// those, which n values at least reach; later ones have to beat the list's n-th.  What
+// passes goes to LDS and from there into the wave's list by rank: a key's place is the number of larger
+// ones.  The waves' lists, and in the join those of the ranges, meet by rank too.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "runtime.h"
 #include "weft_common.h"
@@ -25,7 +28,7 @@ namespace {
 
 constexpr int kMost = WEFT_GGML_MOST_ALTERNATIVES;  // one a lane
 constexpr int kHold = 32;                           // values a lane holds of a chunk
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kMostThreads = 1024;  // of the join, and of a range at most
 static_assert(kMost == kWave, "a list is one key a lane");
 
 typedef unsigned long long Key;
@@ -79,61 +82,98 @@ __device__ __forceinline__ Key key_of(float x, int i) { return (Key)ordered(x) <
 __device__ __forceinline__ float value_of(Key k) { return from_ordered((uint32_t)(k >> 32)); }
 __device__ __forceinline__ int index_of(Key k) { return (int)~(uint32_t)k; }
 
-// one step of a bitonic network: the larger of lanes l and l ^ o to the lower lane if `down`
-__device__ __forceinline__ Key exchange(Key k, int o, bool down, int lane) {
-  const Key other = __shfl_xor(k, o, kWave);
-  const bool larger = ((lane & o) == 0) == down;
-  return (k > other) == larger ? k : other;
-}
-// 64 keys, the largest in lane 0
-__device__ __forceinline__ Key sort64(Key k, int lane) {
-#pragma unroll
-  for (int n = 2; n <= kWave; n <<= 1)
-#pragma unroll
-    for (int o = n / 2; o > 0; o >>= 1) k = exchange(k, o, (lane & n) == 0, lane);
-  return k;
-}
-// the 64 largest of two sorted lists, sorted
-__device__ __forceinline__ Key merge64(Key a, Key b, int lane) {
-  const Key r = __shfl(b, kWave - 1 - lane, kWave);
-  Key k = a > r ? a : r;
-#pragma unroll
-  for (int o = kWave / 2; o > 0; o >>= 1) k = exchange(k, o, true, lane);
-  return k;
+__device__ __forceinline__ Key lane_key(Key k, int lane) {
+  return (Key)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
 }
 
-struct __attribute__((packed, aligned(4))) Floats4 {
-  float f[4];
-};
-struct __attribute__((packed, aligned(2))) Halves8 {
-  _Float16 h[8];
-};
-// values i .. of a row, minus infinity past its end
-template <bool kHalf, int N>
-__device__ __forceinline__ void load(const uint8_t* row, long long i, int v, float* x) {
-  if (i + N <= v) {
-    if constexpr (kHalf) {
-      const Halves8 q = *reinterpret_cast<const Halves8*>(row + 2 * i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = (float)q.h[e];
-    } else {
-      const Floats4 q = *reinterpret_cast<const Floats4*>(row + 4 * i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = q.f[e];
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      if (i + e >= v)
-        x[e] = -INFINITY;
-      else if constexpr (kHalf)
-        x[e] = (float)reinterpret_cast<const _Float16*>(row)[i + e];
-      else
-        x[e] = reinterpret_cast<const float*>(row)[i + e];
-    }
+// The 64 largest keys of what a wave has seen (0: none), sorted, one a lane, and keys on their
+// way there: `pending`, in LDS.
+struct Best {
+  Key* pending;
+  int n_pending;
+  Key list;
+  bool sorted;  // keys have gone into the list
+  __device__ __forceinline__ explicit Best(Key* at) : pending(at), n_pending(0), list(0), sorted(false) {}
+
+  // the lanes' keys that are `in`, behind those on their way
+  __device__ __forceinline__ void add(bool in, Key k, int lane) {
+    const unsigned long long who = __ballot(in);
+    if (in) pending[n_pending + __popcll(who & ((1ull << lane) - 1))] = k;
+    n_pending += __popcll(who);
   }
+  // the last n (at most 64) keys on their way into the list
+  __device__ __forceinline__ void take(int n, int lane) {
+    n_pending -= n;
+    Key* p = pending + n_pending;
+    __builtin_amdgcn_wave_barrier();  // the wave's own writes
+    const Key mine = lane < n ? p[lane] : 0;
+    __builtin_amdgcn_wave_barrier();
+    int down = lane, rank = 0;  // where this lane's list entry, and its new key, go
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const Key k = lane_key(mine, j);
+      const unsigned long long above = __ballot(list > k);
+      down += k > list ? 1 : 0;
+      rank += k > mine ? 1 : 0;
+      if (lane == j) rank += __popcll(above);
+    }
+    // 64 entries and n keys have places 0 to 63 + n
+    if (down < kWave) p[down] = list;
+    if (lane < n && rank < kWave) p[rank] = mine;
+    __builtin_amdgcn_wave_barrier();
+    list = p[lane];
+    __builtin_amdgcn_wave_barrier();
+    sorted = true;
+  }
+  // a key a lane, in any order, among them the `top` largest
+  __device__ __forceinline__ Key rest(int lane, int top) {
+    if (sorted && n_pending > 0) take(n_pending, lane);
+    if (sorted) return lane < top ? list : 0;
+    __builtin_amdgcn_wave_barrier();
+    return lane < n_pending ? pending[lane] : 0;
+  }
+};
+
+// What a wave leaves for the others, beside its list.
+struct Left {
+  Stats st;
+  float bound;  // of the first chunk
+  int count;    // of keys
+  int unused[3];
+};
+static_assert(sizeof(Left) == 32, "keys behind it are aligned");
+
+// The keys of a workgroup (one a lane at most, 0: none) go to `all` (64 a wave), one after the other, and a
+// thread gets one of them back with its place among them: the first waves, so that most rank none.
+// n: how many there are; no thread past it has a place.
+struct Placed {
+  Key k;
+  int place, n;
+};
+__device__ __forceinline__ Placed place_of(Key* all, Left* left, Key k, int lane, int wave, int waves) {
+  const bool in = k != 0;
+  const unsigned long long who = __ballot(in);
+  if (lane == 0) left[wave].count = __popcll(who);
+  __syncthreads();
+  int at = __popcll(who & ((1ull << lane) - 1)), n = 0;
+  for (int w = 0; w < waves; ++w) {
+    at += w < wave ? left[w].count : 0;
+    n += left[w].count;
+  }
+  if (in) all[at] = k;
+  __syncthreads();
+  const int tid = wave * kWave + lane;
+  Placed p = {0, 0, n};
+  if (tid >= n) return p;
+  p.k = all[tid];
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) p.place += all[i] > p.k ? 1 : 0;
+  return p;
 }
 
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
 template <bool kHalf>
 __device__ __forceinline__ float logit(const uint8_t* row, int i) {
   if constexpr (kHalf)
@@ -142,24 +182,46 @@ __device__ __forceinline__ float logit(const uint8_t* row, int i) {
     return reinterpret_cast<const float*>(row)[i];
 }
 
-// A row's answers, by one wave with the row's sums and list.
+// Values i .. of a row, 16-byte aligned there; a wave's lanes lie one after the other from `first` on
+// (its lane 0's i).  Minus infinity before the row's begin (i modulo 2^32) and past its end.  The branches
+// are the wave's and nothing is converted here, so that its loads do not wait for each other (each
+// waited for the one before: 1024 rows of 131072 with 20 alternatives 127 us, now 104).
 template <bool kHalf>
-__device__ __forceinline__ void answer(const LogProbsArgs& a, long long row, const Stats& st, Key list, int lane) {
-  const uint8_t* x = a.x + row * a.x_row;
-  const bool none = st.s == 0.f;  // every logit is minus infinity
-  const float log_s = logf(st.s);
-  for (int i = lane; i < a.given; i += kWave) {
-    const int id = a.tokens[row * a.tokens_row + i];
-    if ((uint32_t)id >= (uint32_t)a.v) continue;
-    a.token_lp[row * a.token_lp_row + i] = none ? -INFINITY : (logit<kHalf>(x, id) - st.m) * a.scale - log_s;
+using Loaded = std::conditional_t<kHalf, half8, float4v>;
+template <bool kHalf>
+__device__ __forceinline__ Loaded<kHalf> load(const uint8_t* row, uint32_t i, uint32_t first, uint32_t v) {
+  using T = std::conditional_t<kHalf, _Float16, float>;
+  constexpr int N = 16 / sizeof(T);
+  const T* p = reinterpret_cast<const T*>(row);
+  Loaded<kHalf> x;
+  if (first < v && v - first >= N * kWave) {
+    x = *reinterpret_cast<const Loaded<kHalf>*>(p + i);
+  } else if (first < v || (int32_t)first < 0) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool in = i + e < v;
+      const T q = p[in ? i + e : 0];
+      x[e] = in ? q : (T)-INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = (T)-INFINITY;
   }
-  if (a.entropy != nullptr && lane == 0) a.entropy[row * a.entropy_row] = none ? 0.f : log_s - st.t / st.s;
-  if (lane < a.top) {
-    // a key of zero: fewer numbers than alternatives
-    a.top_ids[row * a.top_ids_row + lane] = list ? index_of(list) : -1;
-    a.top_lp[row * a.top_lp_row + lane] =
-        list ? (none ? -INFINITY : (value_of(list) - st.m) * a.scale - log_s) : st.s + NAN;
-  }
+  return x;
+}
+
+struct Row {
+  Stats st;
+  float log_s;
+  bool none;  // every logit is minus infinity
+};
+__device__ __forceinline__ Row row_of(const Stats& st) { return {st, logf(st.s), st.s == 0.f}; }
+
+// and an alternative at its place; a key of zero: fewer numbers than alternatives
+__device__ __forceinline__ void answer_top(const LogProbsArgs& a, long long row, const Row& r, Key k, int place) {
+  a.top_ids[row * a.top_ids_row + place] = k ? index_of(k) : -1;
+  a.top_lp[row * a.top_lp_row + place] =
+      k ? (r.none ? -INFINITY : (value_of(k) - r.st.m) * a.scale - r.log_s) : r.st.s + NAN;
 }
 
 __device__ __forceinline__ Stats* work_stats(const LogProbsArgs& a, long long row) {
@@ -169,150 +231,215 @@ __device__ __forceinline__ Key* work_keys(const LogProbsArgs& a, long long row) 
   return reinterpret_cast<Key*>(a.work + row * a.splits * (16 + 8ll * a.top));
 }
 
-// The candidates of a wave: those of one group of loads, and fewer than 64 before them.
-template <int N>
-constexpr int pending_keys() {
-  return kWave * (N + 1);
+// The keys on their way of a wave: those of four values a lane, fewer than 64 before them,
+// and room for the list's 64 beside the last 64.
+constexpr int kGroup = 4, kPending = kWave * (kGroup + 2);
+
+// The largest number, in steps of 16 bits of the ordered value, that `n` lanes' values reach.
+__device__ __forceinline__ float reached_by(float x, int n) {
+  const uint32_t o = ordered(x);
+  uint32_t bound = 0;
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+    if (__popcll(__ballot(o >= (bound | bit))) >= n) bound |= bit;
+  return bound > ordered(-INFINITY) ? from_ordered(bound) : -INFINITY;
+}
+
+// The given token of this thread (the first of them: others are read at the end), on its way before
+// the rest, and its logit, asked for when the rest is on its way.
+template <bool kHalf>
+struct Given {
+  int id;
+  float x;
+  __device__ __forceinline__ Given(const LogProbsArgs& a, long long row, bool wanted) : id(-1), x(0.f) {
+    if (wanted && (int)threadIdx.x < a.given) id = a.tokens[row * a.tokens_row + threadIdx.x];
+  }
+  __device__ __forceinline__ void fetch(const LogProbsArgs& a, long long row) {
+    if ((uint32_t)id < (uint32_t)a.v) x = logit<kHalf>(a.x + row * a.x_row, id);
+  }
+};
+
+// A row's answers, by the threads of a workgroup
+template <bool kHalf>
+__device__ __forceinline__ void answer(const LogProbsArgs& a, long long row, const Row& r, const Given<kHalf>& first) {
+  for (int i = threadIdx.x; i < a.given; i += blockDim.x) {
+    Given<kHalf> g = first;
+    if (i != (int)threadIdx.x) {
+      g.id = a.tokens[row * a.tokens_row + i];
+      g.fetch(a, row);
+    }
+    if ((uint32_t)g.id >= (uint32_t)a.v) continue;
+    a.token_lp[row * a.token_lp_row + i] = r.none ? -INFINITY : (g.x - r.st.m) * a.scale - r.log_s;
+  }
+  if (a.entropy != nullptr && threadIdx.x == 0) a.entropy[row * a.entropy_row] = r.none ? 0.f : r.log_s - r.st.t / r.st.s;
 }
 
 template <bool kHalf, bool kTop>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(LogProbsArgs a) {
+__global__ void __launch_bounds__(kMostThreads) log_probs_kernel(LogProbsArgs a) {
   constexpr int N = kHalf ? 8 : 4;  // values a load
-  constexpr int kPending = pending_keys<N>();
-  __shared__ Key pending[kTop ? kThreads / kWave : 1][kTop ? kPending : 1];
-  __shared__ Stats stats[kThreads / kWave];
-  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, threads = blockDim.x;
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave, threads = blockDim.x, waves = threads / kWave;
+  Left* left = reinterpret_cast<Left*>(lds);
+  Key* all = reinterpret_cast<Key*>(left + waves);
+  Key* pending = all + waves * kWave;  // kPending a wave
   const long long row = a.row0 + (long long)(blockIdx.x / (unsigned)a.splits);
   const int split = (int)(blockIdx.x % (unsigned)a.splits);
   const uint8_t* x_row = a.x + row * a.x_row;
-  const int c1 = min(a.chunks, (split + 1) * a.chunks_each);
+  const int c0 = split * a.chunks_each, c1 = min(a.chunks, c0 + a.chunks_each);
+  // loads are 16-byte aligned: the first begins before a row that is not
+  const int before = (int)(reinterpret_cast<uintptr_t>(x_row) & 15) / (kHalf ? 2 : 4);
+  Given<kHalf> given(a, row, a.splits == 1);
+  const float log2_scale = a.scale * 1.44269504088896341f;
 
   Stats st = {-3.402823466e38f, 0.f, 0.f};
-  Key list = 0;
-  int n_pending = 0;
+  Best best(pending + wave * kPending);
   float limit = -INFINITY;  // what a candidate has at least
-  auto take = [&](int n) {  // n pending keys into the list
-    __builtin_amdgcn_wave_barrier();  // the wave's own writes
-    const Key k = lane < n ? pending[wave][n_pending - n + lane] : 0;
-    __builtin_amdgcn_wave_barrier();
-    n_pending -= n;
-    list = merge64(list, sort64(k, lane), lane);
-    const Key last = __shfl(list, a.top - 1, kWave);
-    if (last) {
-      // indexes that follow are larger: an equal value does not enter
-      limit = fmaxf(limit, nextafterf(value_of(last), INFINITY));
-      if (value_of(last) == INFINITY) limit = NAN;
-    }
+  auto raise = [&] {
+    const Key last = lane_key(best.list, a.top - 1);
+    // indexes that follow are larger: an equal value does not enter, and nothing beside infinities
+    if (last) limit = value_of(last) == INFINITY ? NAN : fmaxf(limit, nextafterf(value_of(last), INFINITY));
   };
 
-  for (int c = split * a.chunks_each; c < c1; ++c) {
-    const long long at = (long long)c * threads * kHold + (long long)N * tid;
+  for (int c = c0; c < c1; ++c) {
+    const uint32_t first = __builtin_amdgcn_readfirstlane((uint32_t)c * threads * kHold + N * kWave * wave - before);
+    const uint32_t at = first + N * lane;
+    Loaded<kHalf> q[kHold / N];
+#pragma unroll
+    for (int j = 0; j < kHold / N; ++j)
+      q[j] = load<kHalf>(x_row, at + (uint32_t)(j * N * threads), first + (uint32_t)(j * N * threads), (uint32_t)a.v);
+    if (c == c0) given.fetch(a, row);
     float x[kHold];
 #pragma unroll
-    for (int j = 0; j < kHold / N; ++j) load<kHalf, N>(x_row, at + (long long)j * N * threads, a.v, x + j * N);
-    float mine = -INFINITY;
+    for (int i = 0; i < kHold; ++i) x[i] = (float)q[i / N][i % N];
+    float most = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kHold; ++i) mine = fmaxf(mine, x[i]);
-    const float m = fmaxf(st.m, wave_max(mine));
+    for (int i = 0; i < kHold; ++i) most = fmaxf(most, x[i]);
+    if (kTop && c == c0) {
+      const int p = (a.top + waves - 1) / waves;
+      const float bound = reached_by(most, p);
+      if (lane == 0) left[wave].bound = bound;
+    }
+    const float m = fmaxf(st.m, wave_max(most));
     const float d0 = fmaxf((st.m - m) * a.scale, -1e4f), e0 = exp_of(d0);
     st = {m, st.s * e0, (st.t + d0 * st.s) * e0};
+    float t = 0.f;  // sum of e^d d / scale
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
-      const float d = (x[i] - m) * a.scale, e = exp_of(d);
+      const float d = x[i] - m, e = __builtin_amdgcn_exp2f(d * log2_scale);
       st.s += e;
-      st.t = fmaf(e, fmaxf(d, -1e4f), st.t);  // minus infinity counts nothing; NaN stays in e
+      t = fmaf(e, fmaxf(d, -3.402823466e38f), t);  // minus infinity counts nothing; NaN stays in e
     }
+    st.t = fmaf(t, a.scale, st.t);
     if constexpr (kTop) {
-      if (c == split * a.chunks_each) {
-        const uint32_t o = ordered(mine);
-        uint32_t bound = 0;
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
-          const int n = __popcll(__ballot(o >= (bound | bit)));
-          if (n >= a.top) bound |= bit;
-          if (n == a.top) break;
-        }
-        limit = from_ordered(max(bound, ordered(-INFINITY)));
+      if (c == c0) {
+        __syncthreads();  // all waves have a first chunk
+        const int p = (a.top + waves - 1) / waves;
+        limit = reached_by(lane < waves ? left[lane].bound : -INFINITY, (a.top + p - 1) / p);
       }
+      bool taken = false;
 #pragma unroll
-      for (int j = 0; j < kHold / N; ++j) {
-        const long long i0 = at + (long long)j * N * threads;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const bool in = x[j * N + e] >= limit && i0 + e < a.v;
-          const unsigned long long who = __ballot(in);
-          if (who == 0) continue;
-          if (in) pending[wave][n_pending + __popcll(who & ((1ull << lane) - 1))] = key_of(x[j * N + e], (int)(i0 + e));
-          n_pending += __popcll(who);
+      for (int j = 0; j < kHold / kGroup; ++j) {
+        // indexes grow from load to load, not within one
+        if (taken && j % (N / kGroup) == 0) {
+          raise();
+          taken = false;
         }
-        while (n_pending >= kWave) take(kWave);
+        // value e of the group is e + kGroup (j % (N / kGroup)) of load j / (N / kGroup)
+        const uint32_t i0 = at + (uint32_t)(j / (N / kGroup) * N * threads + kGroup * (j % (N / kGroup)));
+        const float* g = x + j * kGroup;
+        if (__ballot(fmaxf(fmaxf(g[0], g[1]), fmaxf(g[2], g[3])) >= limit) == 0) continue;
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) best.add(g[e] >= limit && i0 + e < (uint32_t)a.v, key_of(g[e], (int)(i0 + e)), lane);
+        const bool full = best.n_pending >= kWave;
+        while (best.n_pending >= kWave) best.take(kWave, lane);
+        taken |= full;
       }
+      if (taken) raise();
     }
   }
-  if constexpr (kTop)
-    if (n_pending > 0) take(n_pending);
+  const Key mine = kTop ? best.rest(lane, a.top) : 0;
 
   st.s = wave_sum_f(st.s);
   st.t = wave_sum_f(st.t);
-  if (lane == 0) stats[wave] = st;
-  if constexpr (kTop) pending[wave][lane] = list;
-  __syncthreads();
-  if (wave > 0) return;
-  for (int w = 1; w < threads / kWave; ++w) {
-    st = join(st, stats[w], a.scale);
-    if constexpr (kTop) list = merge64(list, pending[w][lane], lane);
-  }
+  if (lane == 0) left[wave].st = st;
+  Placed key = {0, 0, 0};
+  if constexpr (kTop)
+    key = place_of(all, left, mine, lane, wave, waves);
+  else
+    __syncthreads();
+  st = left[0].st;
+  for (int w = 1; w < waves; ++w) st = join(st, left[w].st, a.scale);
+  // places past the numbers have none
+  const int place = !kTop ? a.top : tid < key.n ? key.place : tid;
   if (a.splits == 1) {
-    answer<kHalf>(a, row, st, list, lane);
+    const Row r = row_of(st);
+    answer<kHalf>(a, row, r, given);
+    if (place < a.top) answer_top(a, row, r, key.k, place);
     return;
   }
-  if (lane == 0) work_stats(a, row - a.row0)[split] = st;
-  if (lane < a.top) work_keys(a, row - a.row0)[(long long)split * a.top + lane] = list;
+  if (tid == 0) work_stats(a, row - a.row0)[split] = st;
+  if (place < a.top) work_keys(a, row - a.row0)[(long long)split * a.top + place] = key.k;
 }
 
+// The ranges' sums and lists, a list a lane for the bound: p-th entries as above.
 template <bool kHalf>
 __global__ void __launch_bounds__(kThreads) log_probs_join_kernel(LogProbsArgs a) {
-  __shared__ Key lists[kThreads / kWave][kWave];
-  __shared__ Stats stats[kThreads / kWave];
+  constexpr int kWaves = kThreads / kWave;
+  __shared__ Key pending[kWaves][kPending];
+  __shared__ Key all[kThreads];
+  __shared__ Left left[kWaves];
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const long long row = blockIdx.x;
   const Stats* parts = work_stats(a, row);
   const Key* keys = work_keys(a, row);
+  Given<kHalf> given(a, a.row0 + row, true);
   Stats st = {-3.402823466e38f, 0.f, 0.f};
-  for (int s = threadIdx.x; s < a.splits; s += kThreads) st = join(st, parts[s], a.scale);
-  st = join_wave(st, a.scale);
-  Key list = 0;
-  if (a.top > 0)
-    for (int s = wave; s < a.splits; s += kThreads / kWave)
-      list = merge64(list, lane < a.top ? keys[(long long)s * a.top + lane] : 0, lane);
-  if (lane == 0) stats[wave] = st;
-  lists[wave][lane] = list;
-  __syncthreads();
-  if (wave > 0) return;
-  for (int w = 1; w < kThreads / kWave; ++w) {
-    st = join(st, stats[w], a.scale);
-    if (a.top > 0) list = merge64(list, lists[w][lane], lane);
+  if (lane < a.splits) st = parts[lane];
+  Best best(pending[wave]);
+  if (a.top == 0) {
+    given.fetch(a, a.row0 + row);
+  } else {
+    const int p = (a.top + a.splits - 1) / a.splits;
+    const Key entry = lane < a.splits ? keys[(long long)lane * a.top + p - 1] : 0;
+    given.fetch(a, a.row0 + row);
+    const float limit = reached_by(entry ? value_of(entry) : -INFINITY, (a.top + p - 1) / p);
+    const int n = a.splits * a.top;
+    for (int i = wave * kWave; i < n; i += kThreads) {
+      const Key k = i + lane < n ? keys[i + lane] : 0;
+      if (best.n_pending >= kWave) best.take(kWave, lane);
+      best.add(k != 0 && value_of(k) >= limit, k, lane);
+    }
+    // at most 64 are left
+    if (best.n_pending > kWave) best.take(kWave, lane);
   }
-  answer<kHalf>(a, a.row0 + row, st, list, lane);
+  st = join_wave(st, a.scale);
+  const Row r = row_of(st);
+  answer<kHalf>(a, a.row0 + row, r, given);
+  if (a.top == 0) return;
+  const Placed key = place_of(all, left, best.rest(lane, a.top), lane, wave, kWaves);
+  const int place = (int)threadIdx.x < key.n ? key.place : (int)threadIdx.x;
+  if (place < a.top) answer_top(a, a.row0 + row, r, key.k, place);
 }
 
-// How a call is cut: workgroups of one wave for short rows; ranges until there are 1024
-// workgroups, 256 ranges a row at most.
+// How a call is cut (us): workgroups of one wave for short rows, of 16 for few rows that fit one chunk
+// (256 rows of 32000: 13.2, in ranges of four waves 15.8), else of four in ranges until there are 1024
+// of them (48 rows of 131072: 17.0, of 16 waves 18.0; one row 12.8 and 15.1); 64 ranges a row at
+// most, a list a lane of the join.  Of the shape alone, as the work buffer's size is.
 struct Plan {
-  int threads, chunks, chunks_each, splits;
+  int threads, splits;
   size_t row_bytes;  // of the work buffer
   int64_t rows;      // a launch
 };
+int64_t chunks_of(int64_t v, int threads) { return (v + (int64_t)threads * kHold - 1) / (threads * kHold); }
 Plan plan_of(int64_t v, int64_t rows, int64_t top) {
   Plan p{};
-  p.threads = v <= kWave * kHold ? kWave : kThreads;
-  const int64_t chunk = (int64_t)p.threads * kHold;
-  p.chunks = (int)((v + chunk - 1) / chunk);
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(rows, 1), p.chunks, 256}));
-  p.chunks_each = (int)((p.chunks + want - 1) / want);
-  p.splits = (p.chunks + p.chunks_each - 1) / p.chunks_each;
+  p.threads = v <= kWave * kHold ? kWave : v <= kMostThreads * kHold && v > kThreads * kHold && rows <= 512 ? kMostThreads : kThreads;
+  const int64_t chunks = chunks_of(v, p.threads);
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(rows, 1), chunks, kWave}));
+  const int64_t each = (chunks + want - 1) / want;
+  p.splits = (int)((chunks + each - 1) / each);
   p.row_bytes = p.splits > 1 ? (size_t)p.splits * (16 + 8 * (size_t)top) : 0;
   // a launch has fewer than 2^32 threads
-  p.rows = std::max<int64_t>(1, ((int64_t)1 << 31) / kThreads / p.splits);
+  p.rows = std::max<int64_t>(1, ((int64_t)1 << 31) / kMostThreads / p.splits);
   return p;
 }
 
@@ -373,8 +500,10 @@ hipError_t log_probs(const weft_ggml_tensor* x, const weft_ggml_tensor* tokens, 
   a.given = (int)given;
   a.top = (int)top;
   a.splits = p.splits;
-  a.chunks = p.chunks;
-  a.chunks_each = p.chunks_each;
+  // rows that are not 16-byte aligned begin up to seven values later
+  const bool even = aligned(x->data, 16) && (rows == 1 || x->nb[1] % 16 == 0);
+  a.chunks = (int)chunks_of(even ? v : v + 16 / (int64_t)x->nb[0] - 1, p.threads);
+  a.chunks_each = (a.chunks + p.splits - 1) / p.splits;
   const hipStream_t st = current_stream();
   const bool half = x->type == WEFT_GGML_TYPE_F16;
   for (int64_t r = 0; r < rows; r += p.rows) {
@@ -382,14 +511,16 @@ hipError_t log_probs(const weft_ggml_tensor* x, const weft_ggml_tensor* tokens, 
     a.row0 = r;
     a.work = static_cast<uint8_t*>(wdata) + (p.row_bytes > 0 ? p.row_bytes * (size_t)r : 0);
     const dim3 grid(n * (unsigned)p.splits);
+    const size_t waves = (size_t)(p.threads / kWave);
+    const size_t lds = waves * (sizeof(Left) + (top > 0 ? (kWave + kPending) * sizeof(Key) : 0));
     if (half && top > 0)
-      log_probs_kernel<true, true><<<grid, p.threads, 0, st>>>(a);
+      log_probs_kernel<true, true><<<grid, p.threads, lds, st>>>(a);
     else if (half)
-      log_probs_kernel<true, false><<<grid, p.threads, 0, st>>>(a);
+      log_probs_kernel<true, false><<<grid, p.threads, lds, st>>>(a);
     else if (top > 0)
-      log_probs_kernel<false, true><<<grid, p.threads, 0, st>>>(a);
+      log_probs_kernel<false, true><<<grid, p.threads, lds, st>>>(a);
     else
-      log_probs_kernel<false, false><<<grid, p.threads, 0, st>>>(a);
+      log_probs_kernel<false, false><<<grid, p.threads, lds, st>>>(a);
     check_launch("log_probs_kernel");
     if (p.splits == 1) continue;
     if (half)

@@ -193,18 +193,16 @@ def mul_mat_f8(w: Tensor, w_scales: Tensor, x: Tensor, x_scales: Tensor | None, 
 
 
 class HeadRope(ctypes.Structure):
-    """How heads are normed and turned (weft_ggml_head_rope); ``head_norm_rope`` sets
-    normed and eps."""
-    _fields_ = [("normed", ctypes.c_int32), ("n_rot", ctypes.c_int32), ("neighbours", ctypes.c_int32),
-                ("eps", ctypes.c_float), ("base", ctypes.c_double), ("scale", ctypes.c_double),
-                ("magnitude", ctypes.c_double)]
+    """How heads are turned (weft_ggml_head_rope)."""
+    _fields_ = [("n_rot", ctypes.c_int32), ("neighbours", ctypes.c_int32), ("base", ctypes.c_double),
+                ("scale", ctypes.c_double), ("magnitude", ctypes.c_double)]
 
 
 def head_rope(n_rot: int, neighbours: bool = False, base: float = 10000.0, scale: float = 1.0,
               magnitude: float = 1.0) -> HeadRope:
     """The rotation of a head's first n_rot values: pairs (i, i + n_rot / 2), or
     neighbours (2i, 2i + 1), by position * scale * base^(-2i / n_rot)."""
-    return HeadRope(0, n_rot, neighbours, 0.0, base, scale, magnitude)
+    return HeadRope(n_rot, neighbours, base, scale, magnitude)
 
 
 def head_norm_rope(q: Tensor, k: Tensor | None, q_dst: Tensor, k_dst: Tensor | None, positions: Tensor | None,
@@ -214,10 +212,8 @@ def head_norm_rope(q: Tensor, k: Tensor | None, q_dst: Tensor, k_dst: Tensor | N
     tokens) and its rotation by the tokens' positions (I32); a destination may be its
     source.  factors (n_rot / 2) divide the pairs' frequencies."""
     lib = _lib.load()
-    how = HeadRope(eps is not None, rope.n_rot, rope.neighbours, 0.0 if eps is None else eps, rope.base, rope.scale,
-                   rope.magnitude)
-    _done(lib, lib.weft_ggml_head_norm_rope(_ref(q), _ref(k), _ref(q_dst), _ref(k_dst), _ref(positions), _ref(how),
-                                            _ref(q_weight), _ref(k_weight), _ref(factors)),
+    _done(lib, lib.weft_ggml_head_norm_rope(_ref(q), _ref(k), _ref(q_dst), _ref(k_dst), _ref(positions), _ref(rope),
+                                            eps is not None, eps or 0.0, _ref(q_weight), _ref(k_weight), _ref(factors)),
           "weft_ggml_head_norm_rope")
 
 
