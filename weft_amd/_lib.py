@@ -41,6 +41,8 @@ def _share_torch_hip_runtime() -> None:
 
 def load() -> ctypes.CDLL:
     global _lib, _artifact
+    if _lib is not None:  # set last, when everything is bound
+        return _lib
     with _lock:
         if _lib is None:
             _share_torch_hip_runtime()
@@ -103,7 +105,11 @@ def load() -> ctypes.CDLL:
 
 def _bind_ggml(lib: ctypes.CDLL) -> None:
     """Types of the GGML operator boundary (weft_ggml_*)."""
+    from . import ggml
+
     i32, i64, sz, vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p
+    # descriptors are passed as they are: a byref for each argument costs a call 2 us more
+    t = ctypes.POINTER(ggml.Tensor)
     for name, args, res in (("weft_ggml_type_size", [i32], sz), ("weft_ggml_blck_size", [i32], i64),
                             ("weft_ggml_row_size", [i32, i64], sz),
                             ("weft_ggml_vec_dot_type", [i32], i32),
@@ -118,12 +124,13 @@ def _bind_ggml(lib: ctypes.CDLL) -> None:
                             ("weft_ggml_attention_work_size", [vp, vp, vp, vp], sz),
                             ("weft_ggml_attention",
                              [vp, vp, vp, vp, vp, ctypes.c_float, i64, i64, vp, sz], ctypes.c_int),
-                            ("weft_ggml_quantize_f8", [vp, vp, vp], ctypes.c_int),
-                            ("weft_ggml_mul_mat_f8_work_size", [vp, vp], sz),
-                            ("weft_ggml_mul_mat_f8", [vp, vp, vp, vp, vp, vp, sz], ctypes.c_int),
-                            ("weft_ggml_head_norm_rope", [vp] * 6 + [i32, ctypes.c_float] + [vp] * 3, ctypes.c_int),
-                            ("weft_ggml_log_probs_work_size", [vp, i64], sz),
-                            ("weft_ggml_log_probs", [vp, vp, vp, vp, vp, vp, ctypes.c_float, vp, sz], ctypes.c_int)):
+                            ("weft_ggml_quantize_f8", [t, t, t], ctypes.c_int),
+                            ("weft_ggml_mul_mat_f8_work_size", [t, t], sz),
+                            ("weft_ggml_mul_mat_f8", [t, t, t, t, t, vp, sz], ctypes.c_int),
+                            ("weft_ggml_head_norm_rope",
+                             [t] * 5 + [ctypes.POINTER(ggml.HeadRope), i32, ctypes.c_float] + [t] * 3, ctypes.c_int),
+                            ("weft_ggml_log_probs_work_size", [t, i64], sz),
+                            ("weft_ggml_log_probs", [t] * 6 + [ctypes.c_float, vp, sz], ctypes.c_int)):
         fn = getattr(lib, name)
         fn.argtypes, fn.restype = args, res
 

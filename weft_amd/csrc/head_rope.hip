@@ -8,9 +8,9 @@
 // A head is 8 to 64 lanes of eight values: four pairs, or eight values past the rotated ones.
 // A lane has both values of its pairs, so the rotation moves nothing between lanes.  The
 // angles depend on the token and the lane alone: a wave computes its own once for the
-// heads of a token it walks.  They are computed in 64 bits as turns, t / 2 pi, of which the
-// whole part is dropped before the sine and cosine are taken in 32: at position 10^6 a
-// turn in 32 bits would be off by 0.06.
+// heads of a token it walks, from the pairs' frequencies, computed once a workgroup.  They
+// are kept in 64 bits as turns, t / 2 pi, of which the whole part is dropped before the sine
+// and cosine are taken in 32: at position 10^6 a turn in 32 bits would be off by 0.06.
 #include <algorithm>
 #include <cmath>
 
@@ -41,7 +41,7 @@ struct RopeArgs {
   const float* factors;
   double turn;      // s / (2 pi)
   double log_step;  // -2 log2(base) / n
-  float magnitude, eps;
+  float magnitude, eps, per_value;  // per_value: 1 / d
   int d, n_rot, pair_units, units;  // units of eight values: pairs first, then the rest
   int parts;                        // waves a token
   long long tokens;
@@ -97,16 +97,38 @@ __device__ __forceinline__ void store4(uint8_t* row, int at, int n, const float*
   }
 }
 
+// the sum over aligned groups of G lanes, in each of them
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+  v += dppf<kDppXor1>(v);
+  v += dppf<kDppXor2>(v);
+  v += dppf<kDppHalfMirror>(v);
+  if constexpr (G > 8) v += dppf<kDppMirror>(v);
+  if constexpr (G > 16) v += __shfl_xor(v, 16, kWave);
+  if constexpr (G > 32) v += __shfl_xor(v, 32, kWave);
+  return v;
+}
+// 1 / sqrt(v) within two units of its last place; the instruction takes normal numbers, which v is
+// unless eps is next to nothing
+__device__ __forceinline__ float inverse_root(float v, float eps) {
+  return eps >= 1e-30f ? __builtin_amdgcn_rsqf(v) : 1.f / sqrtf(v);
+}
+
 // G lanes a head
 template <int G, bool kHalfIn, bool kHalfOut>
 __global__ void __launch_bounds__(kThreads) head_norm_rope_kernel(RopeArgs a, long long first) {
   const int lane = threadIdx.x & (kWave - 1);
-  const long long wave = first + (long long)blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave;
+  const long long wave =
+      first + (long long)blockIdx.x * (kThreads / kWave) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const long long token = wave / a.parts;
-  if (token >= a.tokens) return;
   const int unit = lane & (G - 1);
+  // turns a position, of every pair: once a workgroup
+  __shared__ double speed[kMostHead / 2];
+  for (int i = threadIdx.x; i < a.n_rot / 2; i += kThreads) {
+    const double v = a.turn * exp2(a.log_step * (double)i);
+    speed[i] = a.factors != nullptr ? v / (double)a.factors[i] : v;
+  }
   constexpr int kAtOnce = kWave / G;
-  const int heads = a.q.n + a.k.n;
 
   // where this lane's two groups of four lie in a head, and how many of each are there
   int at0, at1, n0, n1;
@@ -129,20 +151,24 @@ __global__ void __launch_bounds__(kThreads) head_norm_rope_kernel(RopeArgs a, lo
     n0 = n1 = min(4, a.n_rot / 2 - at0);
   }
 
-  int pass = (int)(wave - token * a.parts);
-  int h = pass * kAtOnce + lane / G;
+  // passes of kAtOnce heads: those of the queries, then those of the keys
+  const int q_passes = (a.q.n + kAtOnce - 1) / kAtOnce, passes = q_passes + (a.k.n + kAtOnce - 1) / kAtOnce;
+  const int sub = lane / G;
   float x[8];
-  auto load = [&](int head) {
-    if (head >= heads) return;
-    const bool is_k = head >= a.q.n;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  auto load = [&](int pass) {
+    if (pass >= passes || token >= a.tokens) return;
+    const bool is_k = pass >= q_passes;  // the wave's
     const Heads& s = is_k ? a.k : a.q;
-    const uint8_t* row = s.x + token * s.x_token + (is_k ? head - a.q.n : head) * s.x_head;
+    const int head = (is_k ? pass - q_passes : pass) * kAtOnce;
+    if (head + sub >= s.n) return;
+    const uint8_t* row = s.x + token * s.x_token + head * s.x_head + sub * s.x_head;
     load4<kHalfIn>(row, at0, n0, x);
     load4<kHalfIn>(row, at1, n1, x + 4);
   };
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  load(h);
+  int pass = (int)(wave - token * a.parts);
+  load(pass);
 
   float wq[8], wk[8];
 #pragma unroll
@@ -156,37 +182,41 @@ __global__ void __launch_bounds__(kThreads) head_norm_rope_kernel(RopeArgs a, lo
     load4<false>(reinterpret_cast<const uint8_t*>(a.k.weight), at1, n1, wk + 4);
   }
 
+  __syncthreads();
+  if (token >= a.tokens) return;
   float c[4], s[4];
   if (turned) {
-    const double p = (double)a.positions[token] * a.turn;
+    const double p = (double)a.positions[token];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int i = min(4 * unit + e, a.n_rot / 2 - 1);
-      double t = p * exp2(a.log_step * (double)i);
-      if (a.factors != nullptr) t /= (double)a.factors[i];
+      double t = p * speed[min(4 * unit + e, a.n_rot / 2 - 1)];
       t -= rint(t);
-      const float f = 2.f * (float)t;  // half turns, -1 to 1
-      c[e] = cospif(f) * a.magnitude;
-      s[e] = sinpif(f) * a.magnitude;
+      sincospif(2.f * (float)t, &s[e], &c[e]);  // half turns, -1 to 1
+      c[e] *= a.magnitude;
+      s[e] *= a.magnitude;
     }
   }
 
-  while ((h & ~(kAtOnce - 1)) < heads) {  // the same for the whole wave
-    float y[8];
+  for (; pass < passes; pass += a.parts) {
+    const bool is_k = pass >= q_passes;
+    const Heads& o = is_k ? a.k : a.q;
+    const int head = (is_k ? pass - q_passes : pass) * kAtOnce;
+    if (is_k) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) wq[e] = wk[e];
+    }
     float f = 1.f;
     if (a.normed) {
       float q = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) q = fmaf(x[e], x[e], q);
-      q = group_sum<G>(q);
-      f = 1.f / sqrtf(q / (float)a.d + a.eps);
+      q = lanes_sum<G>(q);
+      f = inverse_root(q * a.per_value + a.eps, a.eps);
     }
-    const bool is_k = h >= a.q.n;
+    float y[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = x[e] * f * (is_k ? wk[e] : wq[e]);
-    const int now = h;
-    h += a.parts * kAtOnce;
-    load(h);
+    for (int e = 0; e < 8; ++e) y[e] = x[e] * f * wq[e];
+    load(pass + a.parts);
     if (turned) {
       if (a.neighbours) {
 #pragma unroll
@@ -204,9 +234,8 @@ __global__ void __launch_bounds__(kThreads) head_norm_rope_kernel(RopeArgs a, lo
         }
       }
     }
-    if (now < heads) {
-      const Heads& o = is_k ? a.k : a.q;
-      uint8_t* row = o.y + token * o.y_token + (is_k ? now - a.q.n : now) * o.y_head;
+    if (head + sub < o.n) {
+      uint8_t* row = o.y + token * o.y_token + head * o.y_head + sub * o.y_head;
       store4<kHalfOut>(row, at0, n0, y);
       store4<kHalfOut>(row, at1, n1, y + 4);
     }
@@ -299,6 +328,7 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
   a.normed = normed;
   a.neighbours = r->neighbours != 0;
   a.eps = eps;
+  a.per_value = 1.f / (float)d;
   if (r->n_rot > 0) {
     a.positions = static_cast<const int32_t*>(positions->data);
     a.factors = factors != nullptr ? static_cast<const float*>(factors->data) : nullptr;
@@ -312,7 +342,8 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
   while (g < a.units) g *= 2;
   // a token's heads go to as many waves as there are passes over them, until a launch has
   // 4096 waves
-  const int passes = (a.q.n + a.k.n + kWave / g - 1) / (kWave / g);
+  const int at_once = kWave / g;
+  const int passes = (a.q.n + at_once - 1) / at_once + (a.k.n + at_once - 1) / at_once;
   a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(passes, 4096 / tokens));
   if (in == 2 && out == 2)
     launch_io<true, true>(a, g);

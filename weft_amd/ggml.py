@@ -175,11 +175,11 @@ def quantize_f8(x: Tensor, codes: Tensor, scales: Tensor) -> None:
     ``scales`` of (ceil(K / 128), rows) is one for each 128 values of a row, of
     (ceil(K / 128), ceil(rows / 128)) one for each block of 128 x 128 (weights)."""
     lib = _lib.load()
-    _done(lib, lib.weft_ggml_quantize_f8(_ref(x), _ref(codes), _ref(scales)), "weft_ggml_quantize_f8")
+    _done(lib, lib.weft_ggml_quantize_f8(x, codes, scales), "weft_ggml_quantize_f8")
 
 
 def mul_mat_f8_work_size(w: Tensor, x: Tensor) -> int:
-    return _lib.load().weft_ggml_mul_mat_f8_work_size(_ref(w), _ref(x))
+    return _lib.load().weft_ggml_mul_mat_f8_work_size(w, x)
 
 
 def mul_mat_f8(w: Tensor, w_scales: Tensor, x: Tensor, x_scales: Tensor | None, dst: Tensor, wdata: int = 0,
@@ -188,7 +188,7 @@ def mul_mat_f8(w: Tensor, w_scales: Tensor, x: Tensor, x_scales: Tensor | None, 
     blocks) with rows x (K, M): F32 or F16, quantized on the way, or 8-bit floats
     with their x_scales."""
     lib = _lib.load()
-    _done(lib, lib.weft_ggml_mul_mat_f8(_ref(w), _ref(w_scales), _ref(x), _ref(x_scales), _ref(dst), wdata, wsize),
+    _done(lib, lib.weft_ggml_mul_mat_f8(w, w_scales, x, x_scales, dst, wdata, wsize),
           "weft_ggml_mul_mat_f8")
 
 
@@ -212,8 +212,8 @@ def head_norm_rope(q: Tensor, k: Tensor | None, q_dst: Tensor, k_dst: Tensor | N
     tokens) and its rotation by the tokens' positions (I32); a destination may be its
     source.  factors (n_rot / 2) divide the pairs' frequencies."""
     lib = _lib.load()
-    _done(lib, lib.weft_ggml_head_norm_rope(_ref(q), _ref(k), _ref(q_dst), _ref(k_dst), _ref(positions), _ref(rope),
-                                            eps is not None, eps or 0.0, _ref(q_weight), _ref(k_weight), _ref(factors)),
+    _done(lib, lib.weft_ggml_head_norm_rope(q, k, q_dst, k_dst, positions, rope, eps is not None, eps or 0.0, q_weight,
+                                            k_weight, factors),
           "weft_ggml_head_norm_rope")
 
 
@@ -221,7 +221,7 @@ MOST_ALTERNATIVES = 64
 
 
 def log_probs_work_size(logits: Tensor, n_top: int) -> int:
-    return _lib.load().weft_ggml_log_probs_work_size(_ref(logits), n_top)
+    return _lib.load().weft_ggml_log_probs_work_size(logits, n_top)
 
 
 def log_probs(logits: Tensor, tokens: Tensor | None, token_lp: Tensor | None, entropy: Tensor | None,
@@ -230,6 +230,5 @@ def log_probs(logits: Tensor, tokens: Tensor | None, token_lp: Tensor | None, en
     tokens (n, rows), the rows' entropy and their largest logits' ids and log
     probabilities (A, rows), largest first, of equal ones the lowest id."""
     lib = _lib.load()
-    _done(lib, lib.weft_ggml_log_probs(_ref(logits), _ref(tokens), _ref(token_lp), _ref(entropy), _ref(top_ids),
-                                       _ref(top_lp), scale, wdata, wsize),
+    _done(lib, lib.weft_ggml_log_probs(logits, tokens, token_lp, entropy, top_ids, top_lp, scale, wdata, wsize),
           "weft_ggml_log_probs")
