@@ -118,5 +118,7 @@ void f8_few(const F8Product& p, const uint8_t* plain = nullptr, bool plain_half 
 // More: tiles of 32 to 256 tokens through LDS; work: f8_many_work bytes, of the shapes alone.
 size_t f8_many_work(int64_t m, int64_t n, int64_t k);
 void f8_many(const F8Product& p, float* work);
+// Its tiles of 256 x 256, for 16-bit outputs and rows in aligned chunks of 16.
+void f8_large(const F8Product& p);
 
 }  // namespace weft

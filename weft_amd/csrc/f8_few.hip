@@ -20,20 +20,11 @@
 // block's products (6.9, 15.5, 11.2), 32 weights a wave (6.8, 14.5 and 11.3).
 #include <algorithm>
 
-#include "f8.h"
+#include "f8_tile.h"
 #include "runtime.h"
 
 namespace weft {
 namespace {
-
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-
-struct __attribute__((packed, aligned(1))) Bytes16 {
-  int w[4];
-};
 
 // A lane's 32 codes of a block of 128: chunks g and g + 4 of 16, so that a load's four lanes of
 // a row read 64 contiguous bytes.  p: the block's first code, left: codes of the row from there;
@@ -50,12 +41,12 @@ __device__ __forceinline__ v8i load32(const uint8_t* p, int g, int left) {
       Bytes16 q;
       if constexpr (kWide) {
         const int4 w = *reinterpret_cast<const int4*>(p + at);
-        q = {{w.x, w.y, w.z, w.w}};
+        q = {{(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w}};
       } else {
         q = *reinterpret_cast<const Bytes16*>(p + at);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * h + e] = q.w[e];
+      for (int e = 0; e < 4; ++e) v[4 * h + e] = (int)q.w[e];
     } else {
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -63,15 +54,6 @@ __device__ __forceinline__ v8i load32(const uint8_t* p, int g, int left) {
     }
   }
   return v;
-}
-
-// the e4m3 numbers of eight codes
-__device__ __forceinline__ half8 halves(int lo, int hi) {
-  const half2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
-  const half2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
-  const half2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
-  const half2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
-  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // Plain rows of tokens, for a workgroup that quantizes them itself.

@@ -14,8 +14,9 @@
 // bits.  Sums that end in a 16-bit output, whose own step is 2^-11, are taken so; 32-bit
 // outputs are exact.
 #include <algorithm>
+#include <type_traits>
 
-#include "f8.h"
+#include "f8_tile.h"
 #include "runtime.h"
 
 namespace weft {
@@ -24,54 +25,9 @@ __device__ uint4 g_f8_zeros;  // the chunks past a row's end
 
 namespace {
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v4f __attribute__((ext_vector_type(4)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-typedef _Float16 half2 __attribute__((ext_vector_type(2)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
-struct __attribute__((packed, aligned(1))) Bytes16 {
-  uint32_t w[4];
-};
-
-// 16 (4) bytes per lane from global straight into LDS: lane l writes [lds + 16 l, +16)
-// ([lds + 4 l, +4)).  The kernel waits itself; nothing else in it uses M0.
-__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(lds), "v"(off), "s"(base)
-               : "memory", "m0");
-}
-__device__ __forceinline__ void dma16(const uint8_t* at, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(lds), "v"(at)
-               : "memory", "m0");
-}
-__device__ __forceinline__ void dma4(const float* at, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-               :
-               : "s"(lds), "v"(at)
-               : "memory", "m0");
-}
-// The wave's own loads but the last N have arrived and its LDS reads are done; then all waves'.
-template <int N>
-__device__ __forceinline__ void arrive() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
-}
-
-__device__ __forceinline__ half8 halves(int lo, int hi) {
-  const half2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false);
-  const half2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true);
-  const half2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false);
-  const half2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true);
-  return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
-
 template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
 struct Shape {
+  static constexpr int kTn = TN, kTm = TM, kWn = WN, kWm = WM;
   static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
   static constexpr int RN = TN / WN / 32, RM = TM / WM / 32;  // 32 x 32 parts of a wave
   static constexpr int kData = (TN + TM) * kF8Block;
@@ -83,28 +39,20 @@ struct Shape {
   static_assert(kDirect || STAGES == 2, "loads through registers fill the other slot");
 };
 
-// Tile t of tiles_m x tiles_n.  Workgroup b runs on XCD b % 8, so consecutive tiles are given
-// to one XCD; they are bands of eight token tiles, one weight tile after the other, so that
-// an XCD's 32 workgroups read 8 + 4 tiles through its L2.
-__device__ __forceinline__ void place(int b, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int tiles = tiles_m * tiles_n, each = tiles / 8, rest = tiles % 8, x = b % 8;
-  int t = x * each + min(x, rest) + b / 8;
-  const int band = t / (8 * tiles_n);
-  t -= band * 8 * tiles_n;
-  const int wide = min(8, tiles_m - 8 * band);
-  tn = t / wide;
-  tm = 8 * band + t - tn * wide;
-}
-
 // Two waves a SIMD, so that all registers are plain ones: sums in the matrix pipe's own are
 // copied out one by one (two instructions a value).
-// K in `n` ranges of `each` blocks, whose sums go to [range][token][weight, pitch floats a token];
-// n == 1: straight to the output.
+// K in `n` ranges of `each` blocks, whose sums go to the work buffer as the lanes have them, a
+// tile after the other; n == 1: straight to the output.
 struct Parts {
   float* sums;
-  long long range;  // floats between ranges
-  int n, each, pitch;
+  long long range;  // floats between ranges: whole tiles
+  int n, each;
 };
+// of a lane's first four values of a part, in groups of four
+template <class S>
+__device__ __forceinline__ long long sum_place(int tile, int wave, int part, int lane) {
+  return (((long long)tile * S::kWaves + wave) * (S::RN * S::RM) + part) * 4 * kWave + lane;
+}
 
 template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
 __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_many_kernel(F8Product p, Parts parts, int tiles_m,
@@ -334,63 +282,52 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
   }
 
   // ---- a lane has weights 8 g + 4 h .. + 3 (g < 4) of token r of each part
-#pragma unroll
-  for (int j = 0; j < RM; ++j) {
-    const int m = m0 + wm * (TM / WM) + 32 * j + r;
-    if (m >= p.m) continue;
-    uint8_t* y = p.y + m * p.y_row;
-    float* sums = parts.sums + blockIdx.y * parts.range + (long long)m * parts.pitch;
+  if (parts.n > 1) {
+    v4f* to = reinterpret_cast<v4f*>(parts.sums + blockIdx.y * parts.range) + sum_place<S>(tm * tiles_n + tn, wave, 0, lane);
 #pragma unroll
     for (int i = 0; i < RN; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int n = n0 + wn * (TN / WN) + 32 * i + 8 * g + 4 * h;
-        const v16f& a = acc[i][j];
-        if (parts.n > 1) {
-          if (n < parts.pitch) *reinterpret_cast<v4f*>(sums + n) = v4f{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-        } else if (p.half_out) {
-          _Float16* q = reinterpret_cast<_Float16*>(y) + n;
-          const half4 v = {(_Float16)a[4 * g], (_Float16)a[4 * g + 1], (_Float16)a[4 * g + 2], (_Float16)a[4 * g + 3]};
-          if (n + 3 < p.n && (reinterpret_cast<uintptr_t>(q) & 7u) == 0) {
-            *reinterpret_cast<half4*>(q) = v;
-          } else {
+      for (int j = 0; j < RM; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < p.n) q[e] = v[e];
-          }
-        } else {
-          float* q = reinterpret_cast<float*>(y) + n;
-          if (n + 3 < p.n && (reinterpret_cast<uintptr_t>(q) & 15u) == 0) {
-            *reinterpret_cast<v4f*>(q) = v4f{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n + e < p.n) q[e] = a[4 * g + e];
-          }
+        for (int g = 0; g < 4; ++g) {
+          const v16f& a = acc[i][j];
+          to[((i * RM + j) * 4 + g) * kWave] = v4f{a[4 * g], a[4 * g + 1], a[4 * g + 2], a[4 * g + 3]};
         }
-      }
+    return;
   }
+  __syncthreads();  // every wave has left its operands
+  auto output = [&](auto out) {
+    using Out = decltype(out);
+    static_assert(TM * kTileRow<TN, Out> <= S::kLds, "the tile fits");
+#pragma unroll
+    for (int j = 0; j < RM; ++j)
+#pragma unroll
+      for (int i = 0; i < RN; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          tile_put<TN, Out>(lds, wm * (TM / WM) + 32 * j + r, wn * (TN / WN) + 32 * i + 8 * g + 4 * h, acc[i][j][4 * g],
+                            acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+    __syncthreads();
+    tile_store<TN, TM, S::kThreads, Out>(lds, p, n0, m0);
+  };
+  output(std::conditional_t<kExact, float, _Float16>{});
 }
 
 // The ranges' sums added in their order, four weights a thread.
-__global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, Parts parts) {
-  const int quads = parts.pitch / 4;
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  const long long m = i / quads;
-  const int n = 4 * (int)(i - m * quads);
-  if (m >= p.m) return;
-  const float* at = parts.sums + m * parts.pitch + n;
-  v4f v = *reinterpret_cast<const v4f*>(at);
-  for (int s = 1; s < parts.n; ++s) v += *reinterpret_cast<const v4f*>(at + s * parts.range);
-  uint8_t* y = p.y + m * p.y_row;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    if (n + e >= p.n) break;
-    if (p.half_out)
-      reinterpret_cast<_Float16*>(y)[n + e] = (_Float16)v[e];
-    else
-      reinterpret_cast<float*>(y)[n + e] = v[e];
-  }
+template <class S>
+__global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, Parts parts, int tiles_n, long long threads) {
+  constexpr int kParts = S::RN * S::RM;
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (t >= threads) return;
+  const v4f* at = reinterpret_cast<const v4f*>(parts.sums) + t;
+  v4f v = at[0];
+#pragma unroll 4
+  for (int s = 1; s < parts.n; ++s) v += at[s * (parts.range / 4)];
+  const int lane = threadIdx.x & (kWave - 1), i = (int)(t / kWave);
+  const int g = i % 4, part = i / 4 % kParts, wave = i / 4 / kParts % S::kWaves, tile = i / 4 / kParts / S::kWaves;
+  const int m = tile / tiles_n * S::kTm + wave / S::kWn * (S::kTm / S::kWm) + 32 * (part % S::RM) + (lane & 31);
+  const int n = tile % tiles_n * S::kTn + wave % S::kWn * (S::kTn / S::kWn) + 32 * (part / S::RM) + 8 * g + 4 * (lane >> 5);
+  if (m < p.m) store_weights(p.y + m * p.y_row, n, p.n, p.half_out, v);
 }
 
 template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
@@ -401,9 +338,12 @@ void launch(const F8Product& p, const Parts& parts) {
       <<<dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts.n), S::kThreads, S::kLds, current_stream()>>>(p, parts, tiles_m,
                                                                                                        tiles_n);
   check_launch("f8_many_kernel");
+  if (parts.n > 1) {
+    const long long threads = (long long)tiles_m * tiles_n * S::kThreads * S::RN * S::RM * 4;
+    f8_join_kernel<S><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, current_stream()>>>(p, parts, tiles_n, threads);
+    check_launch("f8_join_kernel");
+  }
 }
-
-int pitch_of(int64_t n) { return (int)((n + 3) / 4 * 4); }
 
 // What a call takes: 256 x 256 tiles (16-bit outputs) when they fill the card, else tiles of
 // 128 weights x 64 or 128 tokens, two workgroups of them a CU, and ranges of K.
@@ -426,7 +366,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
   best.tokens = 128;
   best.parts.n = 1;
   best.parts.each = (int)blocks;
-  if (!exact && ((m + 255) / 256) * ((n + 255) / 256) >= 200) {
+  if (!exact && k % kF8Block == 0 && ((m + 255) / 256) * ((n + 255) / 256) >= 200) {
     best.tokens = 256;
     return best;
   }
@@ -447,10 +387,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
       best.parts.each = (int)each;
     }
   }
-  if (best.parts.n > 1) {
-    best.parts.pitch = pitch_of(n);
-    best.parts.range = (long long)m * best.parts.pitch;
-  }
+  best.parts.range = (m + best.tokens - 1) / best.tokens * best.tokens * ((n + 127) / 128 * 128);
   return best;
 }
 
@@ -486,33 +423,22 @@ void f8_many(const F8Product& all, float* work) {
       p.w.codes += n * p.w.row;
       p.w.scales += n / kF8Block * p.w.s_row;
       p.y += m * p.y_row + n * (p.half_out ? 2 : 4);
-      if (!direct) {
-        if (exact)
-          launch<128, 128, 2, 2, 2, true, false>(p, parts);
-        else
-          launch<128, 128, 2, 2, 2, false, false>(p, parts);
-      } else if (exact) {
+      const auto run = [&](auto exactly) {
+        constexpr bool kExact = decltype(exactly)::value;
         if (plan.tokens == 32)
-          launch<128, 32, 4, 1, 3, true, true>(p, parts);
+          direct ? launch<128, 32, 4, 1, 3, kExact, true>(p, parts) : launch<128, 32, 4, 1, 2, kExact, false>(p, parts);
         else if (plan.tokens == 64)
-          launch<128, 64, 4, 1, 3, true, true>(p, parts);
+          direct ? launch<128, 64, 4, 1, 3, kExact, true>(p, parts) : launch<128, 64, 4, 1, 2, kExact, false>(p, parts);
         else
-          launch<128, 128, 2, 2, 2, true, true>(p, parts);
-      } else if (plan.tokens == 256) {
-        launch<256, 256, 2, 4, 2, false, true>(p, parts);
-      } else if (plan.tokens == 32) {
-        launch<128, 32, 4, 1, 3, false, true>(p, parts);
-      } else if (plan.tokens == 64) {
-        launch<128, 64, 4, 1, 3, false, true>(p, parts);
-      } else {
-        launch<128, 128, 2, 2, 2, false, true>(p, parts);
-      }
+          direct ? launch<128, 128, 2, 2, 2, kExact, true>(p, parts) : launch<128, 128, 2, 2, 2, kExact, false>(p, parts);
+      };
+      if (plan.tokens == 256 && direct)
+        f8_large(p);
+      else if (exact)
+        run(std::true_type{});
+      else
+        run(std::false_type{});
     }
-  if (parts.n > 1) {
-    const int64_t threads = (int64_t)all.m * (parts.pitch / 4);
-    f8_join_kernel<<<dim3((unsigned)((threads + 255) / 256)), 256, 0, current_stream()>>>(all, parts);
-    check_launch("f8_join_kernel");
-  }
 }
 
 }  // namespace weft

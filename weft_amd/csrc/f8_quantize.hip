@@ -66,14 +66,21 @@ __global__ void __launch_bounds__(kThreads) f8_quantize_blocks_kernel(QuantizeAr
   const int i = block * kF8Block + 8 * part;
   float x[8][8];
   float m = 0.f;
+  // a whole block's loads have no branches of lanes between them, so they do not wait for each other
+  if ((band + 1) * kF8Block <= rows && (block + 1) * kF8Block <= a.k) {
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const long long row = band * kF8Block + 16 * p + sub;
-    if (row < rows) {
-      f8_load8<kHalf>(a.x + row * a.x_row, i, a.k, x[p]);
-    } else {
+    for (int p = 0; p < 8; ++p)
+      f8_load8<kHalf>(a.x + (band * kF8Block + 16 * p + sub) * a.x_row, i, i + 8, x[p]);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[p][e] = 0.f;
+    for (int p = 0; p < 8; ++p) {
+      const long long row = band * kF8Block + 16 * p + sub;
+      if (row < rows) {
+        f8_load8<kHalf>(a.x + row * a.x_row, i, a.k, x[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[p][e] = 0.f;
+      }
     }
   }
 #pragma unroll
