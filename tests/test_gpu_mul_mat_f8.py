@@ -104,6 +104,26 @@ def test_large_tiles(hip, m, n, k, src, dst):
     Case(hip, m, n, k, src, dst).check()
 
 
+@pytest.mark.parametrize("m,n,src,kw", [(4000, 4090, F8, {}), (3841, 4096, F32, {"y_pad": 3, "w_pad": 16}),
+                                        (4096, 3841, F16, {"y_offset": 2, "x_pad": 8})])
+def test_tiles_of_256(hip, m, n, src, kw):
+    """Calls that fill the card with the largest tiles, their edges and outputs of every alignment."""
+    hip._lib.launch_log()
+    Case(hip, m, n, 1024, src, F16, **kw).check()
+    assert "f8_large_kernel" in hip._lib.launch_log()
+
+
+@pytest.mark.parametrize("m,n,k,src,dst,kernels", [
+    (1, 4096, 4096, F32, F32, ["f8_few_kernel"]), (16, 300, 1024, F16, F16, ["f8_few_kernel"]),
+    (16, 300, 1152, F16, F16, ["f8_quantize_rows_kernel", "f8_few_kernel"]), (9, 64, 4096, F8, F32, ["f8_few_kernel"]),
+    (24, 2000, 4096, F32, F32, ["f8_quantize_rows_kernel", "f8_many_kernel", "f8_join_kernel"]),
+    (600, 9000, 512, F8, F16, ["f8_many_kernel"])])
+def test_what_is_launched(hip, m, n, k, src, dst, kernels):
+    hip._lib.launch_log()
+    Case(hip, m, n, k, src, dst).check()
+    assert hip._lib.launch_log() == kernels
+
+
 @pytest.mark.parametrize("src", [F32, F16, F8])
 @pytest.mark.parametrize("m", [1, 5, 20, 70, 200, 600])
 def test_strides_and_alignment(hip, m, src):

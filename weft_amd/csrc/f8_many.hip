@@ -345,49 +345,48 @@ void launch(const F8Product& p, const Parts& parts) {
   }
 }
 
-// What a call takes: 256 x 256 tiles (16-bit outputs) when they fill the card, else tiles of
-// 128 weights x 64 or 128 tokens, two workgroups of them a CU, and ranges of K.
+// What a call takes: tiles of 128 weights x 32, 64 or 128 tokens, two workgroups of them a CU, with
+// K in ranges, or of 256 x 256 (16-bit outputs, whole blocks), by the least of these times.
 struct Plan {
   int tokens;  // of a tile: 256, 128, 64 or 32
   Parts parts;
 };
 
-// A step of a workgroup alone on its CU, and of one of several, in us (measured: 512 x 4096 x 4096,
-// one 64-token tile a CU 0.5; 1024 x 4096 x 4096, two 0.4 each, 128-token tiles 0.8 and 0.72, 32-token ones
-// 0.4 and 0.3;
-// twice that with operands widened); 3 us to begin; ranges are written and read
-// again at about 5.5 TB/s and joined by a launch of their own.  So 509 x 4101 x 11008 takes
-// three ranges of 128-token tiles (46.8 us; one range 76, 64-token tiles 59), 512 x 4096 x 4096
-// one of 64 (21.6; two of them 23.8, four of 128 26.0).
+// us, measured.  A step (a block of K) of a workgroup alone on its CU, and of each of several:
+// 128 tokens 0.8 and 0.72, 64 tokens 0.5 and 0.4, 32 tokens 0.4 and 0.3, twice that with operands
+// widened; of 256 x 256 1.85, and 7 for its output; 3 us to begin; ranges are written and read
+// again at about 5.5 TB/s and joined by a launch of their own (3 us).  So 509 x 4101 x 11008 takes three
+// ranges of 128-token tiles (48 us; two 53, one 76, 64-token tiles 59), 512 x 4096 x 4096 one of 64
+// (21; two 24, four of 128 26), 1024 x 4096 x 4096 the same (29; of 128 33 to 35), 24 x 11008 x 4096 five of
+// 32 (14.5; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160).
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
   constexpr int kCus = 256;
   const int64_t blocks = f8_blocks(k);
   Plan best{};
-  best.tokens = 128;
-  best.parts.n = 1;
-  best.parts.each = (int)blocks;
-  if (!exact && k % kF8Block == 0 && ((m + 255) / 256) * ((n + 255) / 256) >= 200) {
-    best.tokens = 256;
-    return best;
-  }
   double least = 0;
-  for (const int tokens : {32, 64, 128}) {
-    const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + 127) / 128);
+  for (const int tokens : {32, 64, 128, 256}) {
+    if (tokens == 256 && (exact || k % kF8Block != 0)) continue;
+    const int64_t rows = tokens == 256 ? 256 : 128;
+    const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + rows - 1) / rows);
     const double alone = (tokens == 32 ? 0.4 : tokens == 64 ? 0.5 : 0.8) * (exact ? 2 : 1);
     const double shared = (tokens == 32 ? 0.3 : tokens == 64 ? 0.4 : 0.72) * (exact ? 2 : 1);
-    for (int64_t want = 1; want <= 16 && (want == 1 || (tiles * want <= 2 * kCus && blocks >= 4 * want)); ++want) {
+    for (int64_t want = 1; want <= 16 && (want == 1 || (tokens < 256 && tiles * want <= 2 * kCus && blocks >= 4 * want)); ++want) {
       const int64_t each = (blocks + want - 1) / want, parts = (blocks + each - 1) / each;
       const int64_t load = (tiles * parts + kCus - 1) / kCus;
-      double us = 3 + (double)each * (load == 1 ? alone : shared * (double)load);
+      double us = 3;
+      if (tokens == 256)
+        us += (double)load * (1.85 * (double)each + 7);
+      else
+        us += (double)each * (load == 1 ? alone : shared * (double)load);
       if (parts > 1) us += 3 + (double)parts * (double)m * (double)n * 4 * 2 / 5.5e6;
       if (least > 0 && us >= least) continue;
       least = us;
       best.tokens = tokens;
       best.parts.n = (int)parts;
       best.parts.each = (int)each;
+      best.parts.range = tiles * tokens * rows;
     }
   }
-  best.parts.range = (m + best.tokens - 1) / best.tokens * best.tokens * ((n + 127) / 128 * 128);
   return best;
 }
 
