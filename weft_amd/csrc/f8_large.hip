@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kWaves * kWave, 2) f8_large_kernel(F8Product p
         const int q = RM * phase + j, last = (q + RN * RM - 1) % (RN * RM);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          // scales of 2^0 for every 32 values
+          // (the form without scales)
           c[q & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[phase & 1][half], xv[j][half], half ? c[q & 1] : zero, 0, 0, 0,
                                                                      0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);

@@ -225,9 +225,9 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
           }
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            // scales of 2^0 for every 32 values
+            // (the form without scales)
             c[q & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i % kW][half], xv[j][half], half ? c[q & 1] : zero, 0, 0,
-                                                                       0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                                                                       0, 0, 0, 0);
             if (q == 0 && half == 1) {
 #pragma unroll
               for (int j = 0; j < RM; ++j) s[j] *= sw;

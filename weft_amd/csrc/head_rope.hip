@@ -268,7 +268,7 @@ hipError_t fail(hipError_t e) {
 }
 
 bool heads_of(const weft_ggml_tensor* t, int64_t d, int64_t tokens, size_t unit) {
-  return t->ne[0] == d && t->ne[2] == tokens && t->ne[1] > 0 && t->ne[1] <= (1 << 20) && t->ne[3] == 1 && t->nb[0] == unit &&
+  return t->ne[0] == d && t->ne[2] == tokens && t->ne[1] > 0 && t->ne[1] <= (1 << 28) && t->ne[3] == 1 && t->nb[0] == unit &&
          t->nb[1] % unit == 0 && t->nb[2] % unit == 0 && t->nb[1] < ((size_t)1 << 40) && t->nb[2] < ((size_t)1 << 40) &&
          aligned(t->data, unit);
 }
