@@ -51,6 +51,12 @@ def test_strides_and_alignment(hip, blocks, t):
         check(hip, x, blocks, t, pad, y_pad, offset, y_offset, major)
 
 
+@pytest.mark.parametrize("rows,k,pad", [(1500, 1537, 0), (1300, 1664, 1), (2049, 2049, 0), (129, 17000, 8)])
+def test_many_blocks_that_share_lines(hip, rows, k, pad):
+    """More blocks than one turn of the launch's order, whole turns and a rest."""
+    check(hip, rows_of(rows, k, F32), True, F32, y_pad=pad)
+
+
 def test_every_code_and_every_tie(hip):
     """Factor 1: the codes' values, the points halfway between them and their neighbours."""
     v = VALUE[:127]
