@@ -13,6 +13,12 @@
 // after cutting them below 2^-13 of the largest one's power of two, and the rest in 32
 // bits.  Sums that end in a 16-bit output, whose own step is 2^-11, are taken so; 32-bit
 // outputs are exact.
+//
+// Bound by the way from L2 to LDS (about 12 TB/s over all CUs) and, where K is cut into ranges, by
+// writing and reading their sums: 509 tokens x 4101 x 11008 to 16 bits take 37 us (1.24 PF) and 7.5 for
+// the sums, the matrix pipe busy 28 % of the time; 24 x 11008 x 4096 to 32 bits 11.3 (4.0 TB/s of
+// weights) and 2.3 to 4.  Tried without gain: 256 x 128 tiles, operands read from LDS a step
+// ahead, two blocks of loads on their way, priority for the products.
 #include <algorithm>
 #include <type_traits>
 
@@ -313,21 +319,34 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
   output(std::conditional_t<kExact, float, _Float16>{});
 }
 
-// The ranges' sums added in their order, four weights a thread.
-template <class S>
-__global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, Parts parts, int tiles_n, long long threads) {
-  constexpr int kParts = S::RN * S::RM;
-  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (t >= threads) return;
-  const v4f* at = reinterpret_cast<const v4f*>(parts.sums) + t;
-  v4f v = at[0];
+// The ranges' sums added in their order.  A workgroup has 32 tokens of a tile and kSpan times 32 of its
+// weights, and stores them by way of LDS: 509 x 4101 outputs of 16 bits, three ranges, take 7.5 us,
+// straight from the registers 10.7.
+template <class S, int kSpan, typename Out>
+__global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, Parts parts, int tiles_n) {
+  constexpr int kWide = 32 * kSpan, kStripsN = S::kTn / kWide, kStrips = kStripsN * (S::kTm / 32);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[32 * kTileRow<kWide, Out>];
+  const int lane = threadIdx.x & (kWave - 1), g = threadIdx.x / kWave;
+  const int tile = (int)blockIdx.x / kStrips, strip = (int)blockIdx.x % kStrips;
+  const int sm = strip / kStripsN, sn = strip % kStripsN;
+  v4f v[kSpan];
+  const v4f* at[kSpan];
+#pragma unroll
+  for (int q = 0; q < kSpan; ++q) {
+    const int i = sn * kSpan + q;
+    const int wave = sm / S::RM * S::kWn + i / S::RN, part = i % S::RN * S::RM + sm % S::RM;
+    at[q] = reinterpret_cast<const v4f*>(parts.sums) + sum_place<S>(tile, wave, part, lane) + g * kWave;
+    v[q] = *at[q];
+  }
 #pragma unroll 4
-  for (int s = 1; s < parts.n; ++s) v += at[s * (parts.range / 4)];
-  const int lane = threadIdx.x & (kWave - 1), i = (int)(t / kWave);
-  const int g = i % 4, part = i / 4 % kParts, wave = i / 4 / kParts % S::kWaves, tile = i / 4 / kParts / S::kWaves;
-  const int m = tile / tiles_n * S::kTm + wave / S::kWn * (S::kTm / S::kWm) + 32 * (part % S::RM) + (lane & 31);
-  const int n = tile % tiles_n * S::kTn + wave % S::kWn * (S::kTn / S::kWn) + 32 * (part / S::RM) + 8 * g + 4 * (lane >> 5);
-  if (m < p.m) store_weights(p.y + m * p.y_row, n, p.n, p.half_out, v);
+  for (int s = 1; s < parts.n; ++s)
+#pragma unroll
+    for (int q = 0; q < kSpan; ++q) v[q] += at[q][s * (parts.range / 4)];
+#pragma unroll
+  for (int q = 0; q < kSpan; ++q)
+    tile_put<kWide, Out>(lds, lane & 31, 32 * q + 8 * g + 4 * (lane >> 5), v[q][0], v[q][1], v[q][2], v[q][3]);
+  __syncthreads();
+  tile_store<kWide, 32, 256, Out>(lds, p, tile % tiles_n * S::kTn + sn * kWide, tile / tiles_n * S::kTm + 32 * sm);
 }
 
 template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
@@ -339,8 +358,9 @@ void launch(const F8Product& p, const Parts& parts) {
                                                                                                        tiles_n);
   check_launch("f8_many_kernel");
   if (parts.n > 1) {
-    const long long threads = (long long)tiles_m * tiles_n * S::kThreads * S::RN * S::RM * 4;
-    f8_join_kernel<S><<<dim3((unsigned)((threads + 255) / 256)), 256, 0, current_stream()>>>(p, parts, tiles_n, threads);
+    constexpr int kSpan = TM / 32;
+    const dim3 grid((unsigned)(tiles_m * tiles_n * (TN / (32 * kSpan)) * (TM / 32)));
+    f8_join_kernel<S, kSpan, std::conditional_t<kExact, float, _Float16>><<<grid, 256, 0, current_stream()>>>(p, parts, tiles_n);
     check_launch("f8_join_kernel");
   }
 }

@@ -15,6 +15,10 @@
 // those, which n values at least reach; later ones have to beat the list's n-th.  What
 // passes goes to LDS and from there into the wave's list by rank: a key's place is the number of larger
 // ones.  The waves' lists, and in the join those of the ranges, meet by rank too.
+//
+// Long batches are bound by memory: 4096 rows of 50021 16-bit logits take 81 us (5.1 TB/s).  Few
+// rows are bound by chains of latency: 48 x 131072 to 20 alternatives 11.7 us (2.1 TB/s) and
+// 4.4 for the join, 1 x 32000 to five 8.8, where a list costs about 3.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
