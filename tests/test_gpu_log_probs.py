@@ -145,6 +145,14 @@ def test_temperatures(hip, scale, t):
     check(hip, logits(3, 20011, t), asked(3, 20011, 2), 10, scale)
 
 
+@pytest.mark.parametrize("scale", [1e-42, 1e-37, 3e37, 3.3e38])
+@pytest.mark.parametrize("v", [5, 700, 40000])
+def test_the_smallest_and_largest_scales(hip, v, scale):
+    """Flat, and split among the largest alone; a difference times the scale stays finite."""
+    x = (np.random.default_rng(v).integers(0, 5, (3, v)) / 4).astype(np.float32)
+    check(hip, x, asked(3, v, 2), min(v, 9), scale)
+
+
 @pytest.mark.parametrize("t", [G.F32, G.F16])
 def test_strides_and_alignment(hip, t):
     for v, pad, offset in ((1000, 8, 0), (1001, 3, 1), (33000, 5, 3), (33001, 0, 1)):

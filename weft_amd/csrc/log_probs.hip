@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kMostThreads) log_probs_kernel(LogProbsArgs a)
   // loads are 16-byte aligned: the first begins before a row that is not
   const int before = (int)(reinterpret_cast<uintptr_t>(x_row) & 15) / (kHalf ? 2 : 4);
   Given<kHalf> given(a, row, a.splits == 1);
-  const float log2_scale = a.scale * 1.44269504088896341f;
+  const float log2_scale = fminf(a.scale * 1.44269504088896341f, 3.402823466e38f);  // 0 x infinity is no number
 
   Stats st = {-3.402823466e38f, 0.f, 0.f};
   Best best(pending + wave * kPending);
