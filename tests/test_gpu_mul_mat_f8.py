@@ -113,11 +113,20 @@ def test_tiles_of_256(hip, m, n, src, kw):
     assert "f8_large_kernel" in hip._lib.launch_log()
 
 
+def test_rows_that_direct_loads_do_not_take(hip):
+    """A call of a shape that goes by two kernels where its rows are aligned."""
+    hip._lib.launch_log()
+    Case(hip, 2040, 9001, 1024, F8, F16, w_pad=8).check()
+    assert hip._lib.launch_log() == ["f8_many_kernel"]
+
+
 @pytest.mark.parametrize("m,n,k,src,dst,kernels", [
     (1, 4096, 4096, F32, F32, ["f8_few_kernel"]), (16, 300, 1024, F16, F16, ["f8_few_kernel"]),
     (16, 300, 1152, F16, F16, ["f8_quantize_rows_kernel", "f8_few_kernel"]), (9, 64, 4096, F8, F32, ["f8_few_kernel"]),
     (24, 2000, 4096, F32, F32, ["f8_quantize_rows_kernel", "f8_many_kernel", "f8_join_kernel"]),
-    (600, 9000, 512, F8, F16, ["f8_many_kernel"])])
+    (600, 9000, 512, F8, F16, ["f8_many_kernel"]),
+    (4096, 5000, 2048, F8, F16, ["f8_large_kernel", "f8_many_kernel"]),
+    (2040, 9001, 1024, F16, F16, ["f8_quantize_rows_kernel", "f8_large_kernel", "f8_many_kernel"])])
 def test_what_is_launched(hip, m, n, k, src, dst, kernels):
     hip._lib.launch_log()
     Case(hip, m, n, k, src, dst).check()

@@ -368,22 +368,29 @@ void launch(const F8Product& p, const Parts& parts) {
 // What a call takes: tiles of 128 weights x 32, 64 or 128 tokens, two workgroups of them a CU, with
 // K in ranges, or of 256 x 256 (16-bit outputs, whole blocks), by the least of these times.
 struct Plan {
-  int tokens;  // of a tile: 256, 128, 64 or 32
+  int tokens;     // of a tile: 256, 128, 64 or 32
   Parts parts;
+  int64_t large;  // of the weights go by tiles of 256, the rest as it would alone
+  double us;
 };
 
 // us, measured.  A step (a block of K) of a workgroup alone on its CU, and of each of several:
 // 128 tokens 0.8 and 0.72, 64 tokens 0.5 and 0.4, 32 tokens 0.4 and 0.3, twice that with operands
-// widened; of 256 x 256 1.85, and 7 for its output; 3 us to begin; ranges are written and read
+// widened; of 256 x 256 1.85, and 7 for its output, less in a round that does not fill the card (1.4 to
+// 1.7 of a third or half of it); 3 us to begin; ranges are written and read
 // again at about 5.5 TB/s and joined by a launch of their own (3 us).  So 509 x 4101 x 11008 takes three
 // ranges of 128-token tiles (48 us; two 53, one 76, 64-token tiles 59), 512 x 4096 x 4096 one of 64
 // (21; two 24, four of 128 26), 1024 x 4096 x 4096 the same (29; of 128 33 to 35), 24 x 11008 x 4096 five of
-// 32 (14.5; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160).
+// 32 (14.5; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160) for the
+// weights that whole rounds of them take and others for the rest (115; 4096 x 6000 x 4096 120 -> 110).
+constexpr int kCus = 256;
+double rounds_us(int64_t tiles, int64_t blocks) {
+  const double part = (double)(tiles % kCus) / kCus;
+  return (double)(tiles / kCus) * (1.85 * (double)blocks + 7) + (part > 0 ? (1.3 + 0.55 * part) * (double)blocks + 7 * part : 0);
+}
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
-  constexpr int kCus = 256;
   const int64_t blocks = f8_blocks(k);
   Plan best{};
-  double least = 0;
   for (const int tokens : {32, 64, 128, 256}) {
     if (tokens == 256 && (exact || k % kF8Block != 0)) continue;
     const int64_t rows = tokens == 256 ? 256 : 128;
@@ -395,19 +402,47 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
       const int64_t load = (tiles * parts + kCus - 1) / kCus;
       double us = 3;
       if (tokens == 256)
-        us += (double)load * (1.85 * (double)each + 7);
+        us += rounds_us(tiles, blocks);
       else
         us += (double)each * (load == 1 ? alone : shared * (double)load);
       if (parts > 1) us += 3 + (double)parts * (double)m * (double)n * 4 * 2 / 5.5e6;
-      if (least > 0 && us >= least) continue;
-      least = us;
+      if (best.us > 0 && us >= best.us) continue;
+      best.us = us;
       best.tokens = tokens;
       best.parts.n = (int)parts;
       best.parts.each = (int)each;
       best.parts.range = tiles * tokens * rows;
     }
+    // whole rounds of large tiles and the rest
+    const int64_t rounds = tiles / kCus, large = rounds * kCus / ((m + tokens - 1) / tokens) * rows;
+    if (tokens == 256 && large > 0 && large < n) {
+      Plan rest = plan_of(m, n - large, k, exact);
+      rest.us += rounds_us(rounds * kCus, blocks);
+      if (rest.us < best.us) {
+        best = rest;
+        best.large = large;
+      }
+    }
   }
   return best;
+}
+
+// A launch has fewer than 2^31 threads: a call in pieces of at most 65536 tokens and weights.
+template <class F>
+void in_launches(const F8Product& all, F launch) {
+  constexpr int kMost = 1 << 16;
+  for (int64_t m = 0; m < all.m; m += kMost)
+    for (int64_t n = 0; n < all.n; n += kMost) {
+      F8Product p = all;
+      p.m = (int)std::min<int64_t>(all.m - m, kMost);
+      p.n = (int)std::min<int64_t>(all.n - n, kMost);
+      p.x.codes += m * p.x.row;
+      p.x.scales += m * p.x.s_row;
+      p.w.codes += n * p.w.row;
+      p.w.scales += n / kF8Block * p.w.s_row;
+      p.y += m * p.y_row + n * (p.half_out ? 2 : 4);
+      launch(p);
+    }
 }
 
 }  // namespace
@@ -428,36 +463,42 @@ void f8_many(const F8Product& all, float* work) {
   const bool direct = all.k % 16 == 0 && all.w.row % 16 == 0 && all.x.row % 16 == 0 && aligned(all.w.codes, 16) &&
                       aligned(all.x.codes, 16) && all.w.row < (1 << 24) && all.x.row < (1 << 24);
   Plan plan = plan_of(all.m, all.n, all.k, exact);
+  if (plan.large > 0 && direct) {
+    F8Product p = all;
+    p.n = (int)plan.large;
+    in_launches(p, [](const F8Product& q) { f8_large(q); });
+    p = all;
+    p.n -= (int)plan.large;
+    p.w.codes += plan.large * p.w.row;
+    p.w.scales += plan.large / kF8Block * p.w.s_row;
+    p.y += plan.large * 2;
+    f8_many(p, work);
+    return;
+  }
+  if (plan.large > 0 || (plan.tokens == 256 && !direct)) {
+    plan.tokens = 128;
+    plan.parts.n = 1;
+    plan.parts.each = (int)f8_blocks(all.k);
+  }
   plan.parts.sums = work;
   const Parts& parts = plan.parts;
-  // a launch has fewer than 2^31 threads
-  constexpr int kMost = 1 << 16;
-  for (int64_t m = 0; m < all.m; m += kMost)
-    for (int64_t n = 0; n < all.n; n += kMost) {
-      F8Product p = all;
-      p.m = (int)std::min<int64_t>(all.m - m, kMost);
-      p.n = (int)std::min<int64_t>(all.n - n, kMost);
-      p.x.codes += m * p.x.row;
-      p.x.scales += m * p.x.s_row;
-      p.w.codes += n * p.w.row;
-      p.w.scales += n / kF8Block * p.w.s_row;
-      p.y += m * p.y_row + n * (p.half_out ? 2 : 4);
-      const auto run = [&](auto exactly) {
-        constexpr bool kExact = decltype(exactly)::value;
-        if (plan.tokens == 32)
-          direct ? launch<128, 32, 4, 1, 3, kExact, true>(p, parts) : launch<128, 32, 4, 1, 2, kExact, false>(p, parts);
-        else if (plan.tokens == 64)
-          direct ? launch<128, 64, 4, 1, 3, kExact, true>(p, parts) : launch<128, 64, 4, 1, 2, kExact, false>(p, parts);
-        else
-          direct ? launch<128, 128, 2, 2, 2, kExact, true>(p, parts) : launch<128, 128, 2, 2, 2, kExact, false>(p, parts);
-      };
-      if (plan.tokens == 256 && direct)
-        f8_large(p);
-      else if (exact)
-        run(std::true_type{});
+  in_launches(all, [&](const F8Product& p) {
+    const auto run = [&](auto exactly) {
+      constexpr bool kExact = decltype(exactly)::value;
+      if (plan.tokens == 32)
+        direct ? launch<128, 32, 4, 1, 3, kExact, true>(p, parts) : launch<128, 32, 4, 1, 2, kExact, false>(p, parts);
+      else if (plan.tokens == 64)
+        direct ? launch<128, 64, 4, 1, 3, kExact, true>(p, parts) : launch<128, 64, 4, 1, 2, kExact, false>(p, parts);
       else
-        run(std::false_type{});
-    }
+        direct ? launch<128, 128, 2, 2, 2, kExact, true>(p, parts) : launch<128, 128, 2, 2, 2, kExact, false>(p, parts);
+    };
+    if (plan.tokens == 256)
+      f8_large(p);
+    else if (exact)
+      run(std::true_type{});
+    else
+      run(std::false_type{});
+  });
 }
 
 }  // namespace weft
