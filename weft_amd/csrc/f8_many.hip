@@ -14,11 +14,13 @@
 // bits.  Sums that end in a 16-bit output, whose own step is 2^-11, are taken so; 32-bit
 // outputs are exact.
 //
-// Bound by the way from L2 to LDS (about 12 TB/s over all CUs) and, where K is cut into ranges, by
-// writing and reading their sums: 509 tokens x 4101 x 11008 to 16 bits take 37 us (1.24 PF) and 7.5 for
-// the sums, the matrix pipe busy 28 % of the time; 24 x 11008 x 4096 to 32 bits 11.3 (4.0 TB/s of
-// weights) and 2.3 to 4.  Tried without gain: 256 x 128 tiles, operands read from LDS a step
-// ahead, two blocks of loads on their way, priority for the products.
+// Bound by the parts of a step, which hardly overlap, and, where K is cut into ranges, by writing and
+// reading their sums.  A step of 128 x 128 tiles takes the two workgroups of a CU 1.44 us; alone, their
+// loads take 0.53 (30 TB/s over all CUs), their reads from LDS 0.32 and their products 0.44.  509 tokens x 4101 x
+// 11008 to 16 bits take 37 us (1.24 PF) and 7.5 for the sums, 24 x 11008 x 4096 to 32 bits 10 (4.5
+// TB/s of weights) and 2.3 to 4.  Tried without gain: 256 x 128 tiles, operands read from LDS a step
+// ahead, three and four blocks' places for 128 tokens, priority for the products, workgroups of a
+// CU half a step apart.
 #include <algorithm>
 #include <type_traits>
 
@@ -360,15 +362,21 @@ void launch(const F8Product& p, const Parts& parts) {
   if (parts.n > 1) {
     constexpr int kSpan = TM / 32;
     const dim3 grid((unsigned)(tiles_m * tiles_n * (TN / (32 * kSpan)) * (TM / 32)));
-    f8_join_kernel<S, kSpan, std::conditional_t<kExact, float, _Float16>><<<grid, 256, 0, current_stream()>>>(p, parts, tiles_n);
+    f8_join_kernel<Shape<TN, TM, WN, WM, 2, kExact, false>, kSpan, std::conditional_t<kExact, float, _Float16>><<<grid, 256, 0, current_stream()>>>(p, parts, tiles_n);
     check_launch("f8_join_kernel");
   }
 }
 
+// Steps' places in LDS, of 32 and 64 tokens: three where a workgroup is alone on its CU, so that a step has
+// two others' time to arrive; two where others run beside it, of which a CU then takes three (us, three
+// places and two: 32 x 5120 x 5120 10.2 and 11.3, 64 x 8192 x 8192 16.9 and 20.8; 24 x 11008 x 4096
+// 14.4 and 13.1, 1024 x 4096 x 4096 29.7 and 27.6, 512 x 11008 x 4096 45.6 and 41.6).
+//
 // What a call takes: tiles of 128 weights x 32, 64 or 128 tokens, two workgroups of them a CU, with
 // K in ranges, or of 256 x 256 (16-bit outputs, whole blocks), by the least of these times.
 struct Plan {
   int tokens;     // of a tile: 256, 128, 64 or 32
+  bool alone;     // on its CU, a workgroup
   Parts parts;
   int64_t large;  // of the weights go by tiles of 256, the rest as it would alone
   double us;
@@ -379,10 +387,10 @@ struct Plan {
 // widened; of 256 x 256 1.85, and 7 for its output, less in a round that does not fill the card (1.4 to
 // 1.7 of a third or half of it); 3 us to begin; ranges are written and read
 // again at about 5.5 TB/s and joined by a launch of their own (3 us).  So 509 x 4101 x 11008 takes three
-// ranges of 128-token tiles (48 us; two 53, one 76, 64-token tiles 59), 512 x 4096 x 4096 one of 64
-// (21; two 24, four of 128 26), 1024 x 4096 x 4096 the same (29; of 128 33 to 35), 24 x 11008 x 4096 five of
-// 32 (14.5; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160) for the
-// weights that whole rounds of them take and others for the rest (115; 4096 x 6000 x 4096 120 -> 110).
+// ranges of 128-token tiles (44 us; two 53, one 76, 64-token tiles 59), 512 x 4096 x 4096 one of 64
+// (21; two 24, four of 128 26), 1024 x 4096 x 4096 the same (28; of 128 29 to 31), 24 x 11008 x 4096 five of
+// 32 (13; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160) for the
+// weights that whole rounds of them take and others for the rest (109; 4096 x 6000 x 4096 120 -> 110).
 constexpr int kCus = 256;
 double rounds_us(int64_t tiles, int64_t blocks) {
   const double part = (double)(tiles % kCus) / kCus;
@@ -409,6 +417,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
       if (best.us > 0 && us >= best.us) continue;
       best.us = us;
       best.tokens = tokens;
+      best.alone = load == 1;
       best.parts.n = (int)parts;
       best.parts.each = (int)each;
       best.parts.range = tiles * tokens * rows;
@@ -486,9 +495,13 @@ void f8_many(const F8Product& all, float* work) {
     const auto run = [&](auto exactly) {
       constexpr bool kExact = decltype(exactly)::value;
       if (plan.tokens == 32)
-        direct ? launch<128, 32, 4, 1, 3, kExact, true>(p, parts) : launch<128, 32, 4, 1, 2, kExact, false>(p, parts);
+        !direct      ? launch<128, 32, 4, 1, 2, kExact, false>(p, parts)
+        : plan.alone ? launch<128, 32, 4, 1, 3, kExact, true>(p, parts)
+                     : launch<128, 32, 4, 1, 2, kExact, true>(p, parts);
       else if (plan.tokens == 64)
-        direct ? launch<128, 64, 4, 1, 3, kExact, true>(p, parts) : launch<128, 64, 4, 1, 2, kExact, false>(p, parts);
+        !direct      ? launch<128, 64, 4, 1, 2, kExact, false>(p, parts)
+        : plan.alone ? launch<128, 64, 4, 1, 3, kExact, true>(p, parts)
+                     : launch<128, 64, 4, 1, 2, kExact, true>(p, parts);
       else
         direct ? launch<128, 128, 2, 2, 2, kExact, true>(p, parts) : launch<128, 128, 2, 2, 2, kExact, false>(p, parts);
     };
