@@ -131,6 +131,17 @@ def test_sizes(hip, rows, v, t):
         check(hip, x, asked(rows, v, 3), top)
 
 
+@pytest.mark.parametrize("t", [G.F32, G.F16])
+@pytest.mark.parametrize("v,offset", [(98770, 0), (8192 + 37, 1), (16384 + 300, 0), (466, 0), (1090, 3), (70, 1)])
+def test_ends_of_few_values(hip, v, offset, t):
+    """A last range, or last waves, of fewer values than alternatives, and of a few more; many equal."""
+    x = logits(3, v, t)
+    x[1] = np.round(x[1])
+    x[2, -50:] += np.float32(20)  # the answer is there
+    for top in (5, 33, 64):
+        check(hip, x, asked(3, v, 1), top, offset=offset)
+
+
 @pytest.mark.parametrize("top", [0, 5])
 def test_parts_left_out(hip, top):
     x = logits(4, 3000)

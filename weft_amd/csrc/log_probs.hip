@@ -12,7 +12,9 @@
 // 64-bit keys of the value and the inverted index, so that of equal values the first wins.
 // Only few values are looked at: in the first chunk, with w waves and n asked for, each wave takes the
 // p-th largest of its lanes' maxima (p = ceil(n / w)) and all the ceil(n / p)-th largest of
-// those, which n values at least reach; later ones have to beat the list's n-th.  What
+// those, which n values at least reach.  Where the row's end leaves too few waves with values, a wave
+// counts its own values instead of lanes (98770 logits, five alternatives: 31 us without a bound for the
+// range that has the last 466, 12 with it).  Later ones have to beat the list's n-th.  What
 // passes goes to LDS and from there into the wave's list by rank: a key's place is the number of larger
 // ones.  The waves' lists, and in the join those of the ranges, meet by rank too.
 //
@@ -248,6 +250,25 @@ __device__ __forceinline__ float reached_by(float x, int n) {
   return bound > ordered(-INFINITY) ? from_ordered(bound) : -INFINITY;
 }
 
+// The same of all values of the wave's first loads (of N values a lane): near the n-th largest.
+template <int N>
+__device__ __forceinline__ float reached_by_values(const float (&x)[kHold], int loads, int n) {
+  uint32_t bound = 0;
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+    const float b = from_ordered(bound | bit);  // no number past the infinities: nothing reaches it
+    int count = 0;
+#pragma unroll
+    for (int j = 0; j < kHold / N; ++j) {
+      if (j >= loads) continue;
+#pragma unroll
+      for (int e = 0; e < N; ++e) count += __popcll(__ballot(x[j * N + e] >= b));
+    }
+    if (count >= n) bound |= bit;
+    if (count == n) break;
+  }
+  return bound > ordered(-INFINITY) ? from_ordered(bound) : -INFINITY;
+}
+
 // The given token of this thread (the first of them: others are read at the end), on its way before
 // the rest, and its logit, asked for when the rest is on its way.
 template <bool kHalf>
@@ -338,6 +359,13 @@ __global__ void __launch_bounds__(kMostThreads) log_probs_kernel(LogProbsArgs a)
         __syncthreads();  // all waves have a first chunk
         const int p = (a.top + waves - 1) / waves;
         limit = reached_by(lane < waves ? left[lane].bound : -INFINITY, (a.top + p - 1) / p);
+        // the row's end may leave too few waves with values
+        if (waves > 1 && limit == -INFINITY) {
+          int loads = 0;
+#pragma unroll
+          for (int j = 0; j < kHold / N; ++j) loads = (int)(first + (uint32_t)(j * N * threads)) < a.v ? j + 1 : loads;
+          limit = reached_by_values<N>(x, loads, a.top);
+        }
       }
       bool taken = false;
 #pragma unroll
@@ -402,7 +430,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_join_kernel(LogProbsArgs a
   if (a.top == 0) {
     given.fetch(a, a.row0 + row);
   } else {
-    const int p = (a.top + a.splits - 1) / a.splits;
+    const int p = (a.top + a.splits - 2) / (a.splits - 1);  // the last range may be short: without it
     const Key entry = lane < a.splits ? keys[(long long)lane * a.top + p - 1] : 0;
     given.fetch(a, a.row0 + row);
     const float limit = reached_by(entry ? value_of(entry) : -INFINITY, (a.top + p - 1) / p);
@@ -424,7 +452,8 @@ __global__ void __launch_bounds__(kThreads) log_probs_join_kernel(LogProbsArgs a
   if (place < a.top) answer_top(a, a.row0 + row, r, key.k, place);
 }
 
-// How a call is cut (us): workgroups of one wave for short rows, of 16 for few rows that fit one chunk
+// How a call is cut (us): workgroups of one wave for short rows, but for many alternatives, for which its
+// lanes' maxima are a poor bound (300 rows of 2048 to 64: 20.8, of four waves 8.2; 3000 of 2000 to 20 11.3 and 20.5), of 16 for few rows that fit one chunk
 // (256 rows of 32000: 13.2, in ranges of four waves 15.8), else of four in ranges until there are 1024
 // of them (48 rows of 131072: 17.0, of 16 waves 18.0; one row 12.8 and 15.1); 64 ranges a row at
 // most, a list a lane of the join.  Of the shape alone, as the work buffer's size is.
@@ -436,7 +465,7 @@ struct Plan {
 int64_t chunks_of(int64_t v, int threads) { return (v + (int64_t)threads * kHold - 1) / (threads * kHold); }
 Plan plan_of(int64_t v, int64_t rows, int64_t top) {
   Plan p{};
-  p.threads = v <= kWave * kHold ? kWave : v <= kMostThreads * kHold && v > kThreads * kHold && rows <= 512 ? kMostThreads : kThreads;
+  p.threads = v <= kWave * kHold && top <= 32 ? kWave : v <= kMostThreads * kHold && v > kThreads * kHold && rows <= 512 ? kMostThreads : kThreads;
   const int64_t chunks = chunks_of(v, p.threads);
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(rows, 1), chunks, kWave}));
   const int64_t each = (chunks + want - 1) / want;
