@@ -26,34 +26,25 @@
 namespace weft {
 namespace {
 
-// A lane's 32 codes of a block of 128: chunks g and g + 4 of 16, so that a load's four lanes of
-// a row read 64 contiguous bytes.  p: the block's first code, left: codes of the row from there;
-// zeros behind it.  kWide: rows in aligned groups of 16, so that a chunk is wholly in the row or
-// behind it.
+// A lane's 32 codes of block b of a row of k: chunks g and g + 4 of 16, so that a load's four lanes
+// of a row read 64 contiguous bytes; zeros behind the row's end.  kWide: rows in aligned groups of 16,
+// so that a chunk is wholly in the row or behind it.
 template <bool kWide>
-__device__ __forceinline__ v8i load32(const uint8_t* p, int g, int left) {
-  v8i v = {0, 0, 0, 0, 0, 0, 0, 0};
+__device__ __forceinline__ v8i load32(const uint8_t* row, int b, int g, int k) {
+  const int at = b * kF8Block + 16 * g;
+  uint4 q[2];
+  if constexpr (kWide) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int at = 64 * h + 16 * g;
-    if (kWide || left >= at + 16) {
-      if (left <= at) continue;
-      Bytes16 q;
-      if constexpr (kWide) {
-        const int4 w = *reinterpret_cast<const int4*>(p + at);
-        q = {{(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w}};
-      } else {
-        q = *reinterpret_cast<const Bytes16*>(p + at);
-      }
+    for (int h = 0; h < 2; ++h)
+      q[h] = at + 64 * h < k ? *reinterpret_cast<const uint4*>(row + at + 64 * h) : uint4{0, 0, 0, 0};
+  } else if ((b + 1) * kF8Block <= k) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[4 * h + e] = (int)q.w[e];
-    } else {
+    for (int h = 0; h < 2; ++h) q[h] = codes16(row + at + 64 * h);
+  } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (at + e < left) v[4 * h + e / 4] |= (int)((uint32_t)p[at + e] << (8 * (e & 3)));
-    }
+    for (int h = 0; h < 2; ++h) q[h] = codes16(row, at + 64 * h, k);
   }
-  return v;
+  return v8i{(int)q[0].x, (int)q[0].y, (int)q[0].z, (int)q[0].w, (int)q[1].x, (int)q[1].y, (int)q[1].z, (int)q[1].w};
 }
 
 // Plain rows of tokens, for a workgroup that quantizes them itself.
@@ -90,7 +81,7 @@ __global__ void __launch_bounds__(1024) f8_few_kernel(F8Product p, PlainRows pla
   float swv;
   auto load_weights = [&](int b) {
     if (b >= blocks) return;
-    wv = load32<kWide>(w + (long long)b * kF8Block, g, p.k - b * kF8Block);
+    wv = load32<kWide>(w, b, g, p.k);
     swv = sw[b * p.w.s_block];
   };
   load_weights(wave);
@@ -114,7 +105,7 @@ __global__ void __launch_bounds__(1024) f8_few_kernel(F8Product p, PlainRows pla
     if (b != wave) load_weights(b);
     // codes quantized here are whole blocks
     const v8i xv =
-        load32<kWide || kSource != kCodes>(x + (long long)b * kF8Block, g, kSource ? kF8Block : p.k - b * kF8Block);
+        load32<kWide || kSource != kCodes>(x, b, g, kSource ? blocks * kF8Block : p.k);
     const float s = swv * sx[b * sx_block];
     v4f c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

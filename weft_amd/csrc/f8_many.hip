@@ -122,28 +122,19 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
   // ---- the same through registers, for rows of any alignment
   uint4 held[kDirect ? 1 : LN + LM];
   float held_scale = 0.f;
-  auto fetch1 = [&](const uint8_t* row, int b) {
-    const int left = p.k - b * kF8Block - 16 * chunk;
-    uint4 v = {0, 0, 0, 0};
-    const uint8_t* q = row + (long long)b * kF8Block + 16 * chunk;
-    if (left >= 16) {
-      const Bytes16 r = *reinterpret_cast<const Bytes16*>(q);
-      v = {r.w[0], r.w[1], r.w[2], r.w[3]};
-    } else if (left > 0) {
-      uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (e < left) w[e / 4] |= (uint32_t)q[e] << (8 * (e & 3));
-      v = {w[0], w[1], w[2], w[3]};
-    }
-    return v;
-  };
   auto fetch = [&](int step) {
-    const int b = first + step;
+    const int b = first + step, at = b * kF8Block + 16 * chunk;
+    if ((b + 1) * kF8Block <= p.k) {
 #pragma unroll
-    for (int i = 0; i < LN; ++i) held[i] = fetch1(w_base + w_row(i) * p.w.row, b);
+      for (int i = 0; i < LN; ++i) held[i] = codes16(w_base + w_row(i) * p.w.row + at);
 #pragma unroll
-    for (int i = 0; i < LM; ++i) held[LN + i] = fetch1(x_base + x_row(i) * p.x.row, b);
+      for (int i = 0; i < LM; ++i) held[LN + i] = codes16(x_base + x_row(i) * p.x.row + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < LN; ++i) held[i] = codes16(w_base + w_row(i) * p.w.row, at, p.k);
+#pragma unroll
+      for (int i = 0; i < LM; ++i) held[LN + i] = codes16(x_base + x_row(i) * p.x.row, at, p.k);
+    }
     held_scale = s_at[b * s_step];
   };
   auto put = [&](int slot) {

@@ -17,6 +17,32 @@ struct __attribute__((packed, aligned(1))) Bytes16 {
   uint32_t w[4];
 };
 
+__device__ __forceinline__ uint4 codes16(const uint8_t* at) {
+  const Bytes16 r = *reinterpret_cast<const Bytes16*>(at);
+  return {r.w[0], r.w[1], r.w[2], r.w[3]};
+}
+// The 16 codes of a row of k from `at` on, zeros behind its end; without branches of lanes, so that
+// several of these do not wait for each other.  Rows of 16 and more: the 16 bytes that end with the row,
+// moved down.
+__device__ __forceinline__ uint4 codes16(const uint8_t* row, int at, int k) {
+  if (k >= 16) {
+    const int from = min(at, k - 16), s = at - from;
+    const uint4 v = codes16(row + from);
+    const uint64_t first = (uint64_t)v.y << 32 | v.x, last = (uint64_t)v.w << 32 | v.z;
+    const uint64_t a = s & 8 ? last : first, b = s & 8 ? 0 : last;
+    const int n = 8 * (s & 7);
+    const uint64_t lo = s < 16 ? a >> n | b << 1 << (63 - n) : 0, hi = s < 16 ? b >> n : 0;
+    return {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const uint32_t c = row[min(at + e, k - 1)];
+    w[e / 4] |= at + e < k ? c << (8 * (e & 3)) : 0;
+  }
+  return {w[0], w[1], w[2], w[3]};
+}
+
 // 16 (4) bytes per lane from global straight into LDS: lane l writes [lds + 16 l, +16)
 // ([lds + 4 l, +4)).  The kernel waits itself; nothing else in it uses M0.
 __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t off, uint32_t lds) {
