@@ -373,9 +373,8 @@ struct Plan {
   double us;
 };
 
-// us, measured.  A step (a block of K) of a workgroup alone on its CU, and of each of several:
-// 128 tokens 0.8 and 0.72, 64 tokens 0.5 and 0.4, 32 tokens 0.4 and 0.3, twice that with operands
-// widened; of 256 x 256 1.85, and 7 for its output, less in a round that does not fill the card (1.4 to
+// us, measured.  A step (a block of K) of a workgroup alone on its CU, and of each of several, takes
+// what kStepCost has, of 256 x 256 1.85, and 7 for its output, less in a round that does not fill the card (1.4 to
 // 1.7 of a third or half of it); 3 us to begin; ranges are written and read
 // again at about 5.5 TB/s and joined by a launch of their own (3 us).  So 509 x 4101 x 11008 takes three
 // ranges of 128-token tiles (44 us; two 53, one 76, 64-token tiles 59), 512 x 4096 x 4096 one of 64
@@ -383,6 +382,12 @@ struct Plan {
 // 32 (13; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160) for the
 // weights that whole rounds of them take and others for the rest (109; 4096 x 6000 x 4096 120 -> 110).
 constexpr int kCus = 256;
+struct StepCost {
+  double alone, shared;
+};
+// rows of whole 16 bytes and others, codes as they are and widened, 32, 64 and 128 tokens
+constexpr StepCost kStepCost[2][2][3] = {{{{0.4, 0.3}, {0.5, 0.4}, {0.8, 0.72}}, {{0.8, 0.6}, {1.0, 0.8}, {1.6, 1.44}}},
+                                         {{{0.9, 0.55}, {1.08, 0.7}, {1.6, 1.03}}, {{1.15, 0.6}, {1.2, 0.8}, {1.7, 1.5}}}};
 double rounds_us(int64_t tiles, int64_t blocks) {
   const double part = (double)(tiles % kCus) / kCus;
   return (double)(tiles / kCus) * (1.85 * (double)blocks + 7) + (part > 0 ? (1.3 + 0.55 * part) * (double)blocks + 7 * part : 0);
@@ -394,8 +399,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
     if (tokens == 256 && (exact || k % kF8Block != 0)) continue;
     const int64_t rows = tokens == 256 ? 256 : 128;
     const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + rows - 1) / rows);
-    const double alone = (tokens == 32 ? 0.4 : tokens == 64 ? 0.5 : 0.8) * (exact ? 2 : 1);
-    const double shared = (tokens == 32 ? 0.3 : tokens == 64 ? 0.4 : 0.72) * (exact ? 2 : 1);
+    const StepCost& cost = kStepCost[k % 16 != 0][exact][tokens == 32 ? 0 : tokens == 64 ? 1 : 2];
     for (int64_t want = 1; want <= 16 && (want == 1 || (tokens < 256 && tiles * want <= 2 * kCus && blocks >= 4 * want)); ++want) {
       const int64_t each = (blocks + want - 1) / want, parts = (blocks + each - 1) / each;
       const int64_t load = (tiles * parts + kCus - 1) / kCus;
@@ -403,7 +407,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
       if (tokens == 256)
         us += rounds_us(tiles, blocks);
       else
-        us += (double)each * (load == 1 ? alone : shared * (double)load);
+        us += (double)each * (load == 1 ? cost.alone : cost.shared * (double)load);
       if (parts > 1) us += 3 + (double)parts * (double)m * (double)n * 4 * 2 / 5.5e6;
       if (best.us > 0 && us >= best.us) continue;
       best.us = us;
