@@ -12,9 +12,9 @@
 // are kept in 64 bits as turns, t / 2 pi, of which the whole part is dropped before the sine
 // and cosine are taken in 32: at position 10^6 a turn in 32 bits would be off by 0.06.
 //
-// Bound by memory: 16384 tokens of 64 + 8 heads of 128 16-bit values take 140 us (4.3 TB/s; 147
-// with the frequencies computed in each wave), one token 3.5 us, of which a launch is 2.4.  Tried:
-// stores that pass the caches (135 us, and whoever reads the result next loses more), two
+// Bound by memory: 16384 tokens of 64 + 8 heads of 128 16-bit values take 134 us (4.5 TB/s; with the
+// frequencies computed in each wave 7 us more), one token 3.5 us, of which a launch is 2.4.  Tried:
+// stores that pass the caches (5 us less, and whoever reads the result next loses more), two
 // passes of loads on their way (nothing).
 #include <algorithm>
 #include <cmath>
@@ -345,11 +345,12 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
   a.units = a.pair_units + (int)((d - r->n_rot + 7) / 8);
   int g = 8;
   while (g < a.units) g *= 2;
-  // a token's heads go to as many waves as there are passes over them, until a launch has
-  // 4096 waves
+  // A token's heads go to as many waves as there are passes over them, until a launch has 4096 waves,
+  // and past that to waves of five to nine passes: 16384 tokens of 18 passes 140 us in waves of 18, 134 in
+  // six, 145 in four and five; 8192 tokens 86 and 73; 2116 of 16 passes 36 and 22.5.
   const int at_once = kWave / g;
   const int passes = (a.q.n + at_once - 1) / at_once + (a.k.n + at_once - 1) / at_once;
-  a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(passes, 4096 / tokens));
+  a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(passes, std::max<int64_t>(4096 / tokens, passes / 5)));
   if (in == 2 && out == 2)
     launch_io<true, true>(a, g);
   else if (in == 2)
