@@ -9,7 +9,7 @@
 // quarter of a step at a time, after the phase's first products are under way.
 //
 // Bound by the clock that its power leaves it, the matrix pipe and the output's stores, which nothing
-// covers: 8192^3 of random codes takes 492 to 528 us (2.1 to 2.2 PF) at about 1.95 GHz, the pipe busy 52 %
+// covers: 8192^3 of random codes takes 492 to 544 us, by the card (2.0 to 2.2 PF), at about 1.95 GHz, the pipe busy 52 %
 // of the time, and of zeros, the same instructions, 405 (2.7 PF).  Of
 // copies with a part left out, without the scales' multiply-adds 517 us, without loads 456,
 // without products 417; the stores take 29.  Tiles of 128 x 128 take 580.
