@@ -441,11 +441,9 @@ int weft_ggml_quantize_f8(const weft_ggml_tensor *x, const weft_ggml_tensor *cod
 /* dst = w x: w (K, N; F8_E4M3) with w_scales (ceil(K / 128), ceil(N / 128); F32), x (K, M)
  * as F32 or F16, quantized as above a row at a time (x_scales NULL), or as F8_E4M3 with
  * x_scales (ceil(K / 128), M; F32); dst (N, M): F32 or F16.  K >= 1; rows lie any whole
- * elements apart.  F32 outputs, and all of up to 16 tokens, are of exact products summed in 32
- * bits; F16 outputs of more tokens are those of the matrix instruction for 8-bit floats, which
- * cuts each eight products below 2^-13 of the largest one's power of two.  A block's sum
- * is multiplied by the product of its two scales, which has to be finite in 32 bits and loses bits
- * below 2^-126.  NaN codes reach their row's outputs and no others.
+ * elements apart.  Outputs are of exact products summed in 32 bits; the order of the sums, and so an
+ * output's last bits, depends on the shapes.  A block's sum is multiplied by the product of
+ * its two scales, which has to be finite in 32 bits and loses bits below 2^-126.  NaN codes reach their row's outputs and no others.
  * wdata: weft_ggml_mul_mat_f8_work_size bytes, 16-byte aligned (scratch; its content need
  * not be kept or cleared); the size depends on the shapes and types only. */
 size_t weft_ggml_mul_mat_f8_work_size(const weft_ggml_tensor *w, const weft_ggml_tensor *x);

@@ -7,22 +7,18 @@
 // a block's sums start at zero on the matrix pipe, then go to the part's sums times the two
 // scales, one multiply-add a value (a lane has one token, so one factor).
 //
-// kExact: operands are widened to 16-bit floats on their way from LDS, and products and sums
-// have 32 bits, at the rate of 16-bit products.  Else v_mfma_f32_32x32x64_f8f6f4 takes the codes as they
-// are, at twice the rate; measured on the device, it adds each eight products of a lane
-// after cutting them below 2^-13 of the largest one's power of two, and the rest in 32
-// bits.  Sums that end in a 16-bit output, whose own step is 2^-11, are taken so; 32-bit
-// outputs are exact.
+// Operands are widened to 16-bit floats on their way from LDS: e4m3 numbers are 16-bit floats, so products are
+// exact, and sums have 32 bits.  The matrix instructions that take the codes as they are run at twice the
+// rate, but cut each eight products of a lane below 2^-13 of the largest one's power of two (measured on
+// the device), so that sums whose large products cancel, or that have one large product beside small ones, lose
+// more than a 16-bit output's own rounding; they are not used.
 //
 // Bound by the parts of a step, which hardly overlap, and, where K is cut into ranges, by writing and
-// reading their sums.  A step of 128 x 128 tiles takes the two workgroups of a CU 1.44 us; alone, their
-// loads take 0.53 (30 TB/s over all CUs), their reads from LDS 0.32 and their products 0.44.  509 tokens x 4101 x
-// 11008 to 16 bits take 37 us (1.24 PF) and 7.5 for the sums, 24 x 11008 x 4096 to 32 bits 10 (4.5
-// TB/s of weights) and 2.3 to 4.  Tried without gain: 256 x 128 tiles, operands read from LDS a step
-// ahead, three and four blocks' places for 128 tokens, priority for the products, workgroups of a
-// CU half a step apart.
+// reading their sums: 2048 tokens x 4096 x 4096 take 73 us by 128-token tiles (0.94 PF), 8192^3 to 32 bits 1013 (1.09
+// PF), 24 x 11008 x 4096 10 (4.5 TB/s of weights) and 2.3 to 4 for the sums.  Tried without gain: 256 x 128 tiles,
+// operands read from LDS a step ahead, three and four blocks' places for 128 tokens, priority for the products,
+// workgroups of a CU half a step apart.
 #include <algorithm>
-#include <type_traits>
 
 #include "f8_tile.h"
 #include "runtime.h"
@@ -33,7 +29,7 @@ __device__ uint4 g_f8_zeros;  // the chunks past a row's end
 
 namespace {
 
-template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
+template <int TN, int TM, int WN, int WM, int STAGES, typename Out, bool kDirect>
 struct Shape {
   static constexpr int kTn = TN, kTm = TM, kWn = WN, kWm = WM;
   static constexpr int kWaves = WN * WM, kThreads = kWaves * kWave;
@@ -62,10 +58,10 @@ __device__ __forceinline__ long long sum_place(int tile, int wave, int part, int
   return (((long long)tile * S::kWaves + wave) * (S::RN * S::RM) + part) * 4 * kWave + lane;
 }
 
-template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
-__global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_many_kernel(F8Product p, Parts parts, int tiles_m,
+template <int TN, int TM, int WN, int WM, int STAGES, typename Out, bool kDirect>
+__global__ void __launch_bounds__(64 * WN * WM, kDirect ? 2 : 1) f8_many_kernel(F8Product p, Parts parts, int tiles_m,
                                                                  int tiles_n) {
-  using S = Shape<TN, TM, WN, WM, STAGES, kExact, kDirect>;
+  using S = Shape<TN, TM, WN, WM, STAGES, Out, kDirect>;
   constexpr int RN = S::RN, RM = S::RM, LN = S::kLoadsN, LM = S::kLoadsM;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -164,91 +160,35 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
     const uint8_t* w = lds + slot * S::kSlot + (wn * (TN / WN) + r) * kF8Block;
     const uint8_t* x = lds + slot * S::kSlot + TN * kF8Block + (wm * (TM / WM) + r) * kF8Block;
     const float* scales = reinterpret_cast<const float*>(lds + slot * S::kSlot + S::kData);
+    const float sw = scales[S::kTokenWaves * kWave + wn * (TN / WN) / kF8Block];
     float s[RM];
-    auto factors = [&] {
-      const float sw = scales[S::kTokenWaves * kWave + wn * (TN / WN) / kF8Block];
 #pragma unroll
-      for (int j = 0; j < RM; ++j) s[j] = sw * scales[wm * (TM / WM) + 32 * j + r];
-    };
-    if constexpr (kExact) {
-      factors();
-      half8 xh[RM][8];
+    for (int j = 0; j < RM; ++j) s[j] = sw * scales[wm * (TM / WM) + 32 * j + r];
+    half8 xh[RM][8];
 #pragma unroll
-      for (int j = 0; j < RM; ++j)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const v8i v = operand(x + 32 * j * kF8Block, half);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) xh[j][4 * half + q] = halves(v[2 * q], v[2 * q + 1]);
-        }
-#pragma unroll
-      for (int i = 0; i < RN; ++i) {
-        half8 wh[8];
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const v8i v = operand(w + 32 * i * kF8Block, half);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) wh[4 * half + q] = halves(v[2 * q], v[2 * q + 1]);
-        }
-#pragma unroll
-        for (int j = 0; j < RM; ++j) {
-          v16f c = zero;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(wh[q], xh[j][q], c, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[e], s[j], acc[i][j][e]);
-        }
-      }
-    } else {
-      constexpr int kW = RN * RM > 4 ? 1 : 2;  // weights of the next part on their way, where registers hold them
-      v8i xv[RM][2], wv[kW][2];
+    for (int j = 0; j < RM; ++j)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        wv[0][half] = operand(w, half);
+        const v8i v = operand(x + 32 * j * kF8Block, half);
 #pragma unroll
-        for (int j = 0; j < RM; ++j) xv[j][half] = operand(x + 32 * j * kF8Block, half);
+        for (int q = 0; q < 4; ++q) xh[j][4 * half + q] = halves(v[2 * q], v[2 * q + 1]);
       }
-      float sw = scales[S::kTokenWaves * kWave + wn * (TN / WN) / kF8Block];
 #pragma unroll
-      for (int j = 0; j < RM; ++j) s[j] = scales[wm * (TM / WM) + 32 * j + r];
-      __builtin_amdgcn_sched_barrier(0);
-      // a part's sums are added while the matrix pipe works on the next part
-      v16f c[2];
+    for (int i = 0; i < RN; ++i) {
+      half8 wh[8];
 #pragma unroll
-      for (int q = 0; q <= RN * RM; ++q) {
-        if (q < RN * RM) {
-          const int i = q / RM, j = q % RM;
-          if (kW == 2 && j == 0 && i + 1 < RN) {
+      for (int half = 0; half < 2; ++half) {
+        const v8i v = operand(w + 32 * i * kF8Block, half);
 #pragma unroll
-            for (int half = 0; half < 2; ++half) wv[(i + 1) % kW][half] = operand(w + 32 * (i + 1) * kF8Block, half);
-          }
+        for (int q = 0; q < 4; ++q) wh[4 * half + q] = halves(v[2 * q], v[2 * q + 1]);
+      }
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            // (the form without scales)
-            c[q & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wv[i % kW][half], xv[j][half], half ? c[q & 1] : zero, 0, 0,
-                                                                       0, 0, 0, 0);
-            if (q == 0 && half == 1) {
+      for (int j = 0; j < RM; ++j) {
+        v16f c = zero;
 #pragma unroll
-              for (int j = 0; j < RM; ++j) s[j] *= sw;
-            }
-            if (q > 0) {
-              const int i = (q - 1) / RM, j = (q - 1) % RM;
+        for (int q = 0; q < 8; ++q) c = __builtin_amdgcn_mfma_f32_32x32x16_f16(wh[q], xh[j][q], c, 0, 0, 0);
 #pragma unroll
-              for (int e = 8 * half; e < 8 * half + 8; ++e) acc[i][j][e] = fmaf(c[(q - 1) & 1][e], s[j], acc[i][j][e]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-          }
-        }
-        if (q == RN * RM) {
-          const int i = (q - 1) / RM, j = (q - 1) % RM;
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[(q - 1) & 1][e], s[j], acc[i][j][e]);
-        }
-        if (kW == 1 && q < RN * RM && q % RM == RM - 1 && q / RM + 1 < RN) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) wv[0][half] = operand(w + 32 * (q / RM + 1) * kF8Block, half);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(c[e], s[j], acc[i][j][e]);
       }
     }
   };
@@ -295,21 +235,17 @@ __global__ void __launch_bounds__(64 * WN * WM, kDirect || !kExact ? 2 : 1) f8_m
     return;
   }
   __syncthreads();  // every wave has left its operands
-  auto output = [&](auto out) {
-    using Out = decltype(out);
-    static_assert(TM * kTileRow<TN, Out> <= S::kLds, "the tile fits");
+  static_assert(TM * kTileRow<TN, Out> <= S::kLds, "the tile fits");
 #pragma unroll
-    for (int j = 0; j < RM; ++j)
+  for (int j = 0; j < RM; ++j)
 #pragma unroll
-      for (int i = 0; i < RN; ++i)
+    for (int i = 0; i < RN; ++i)
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
-          tile_put<TN, Out>(lds, wm * (TM / WM) + 32 * j + r, wn * (TN / WN) + 32 * i + 8 * g + 4 * h, acc[i][j][4 * g],
-                            acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
-    __syncthreads();
-    tile_store<TN, TM, S::kThreads, Out>(lds, p, n0, m0);
-  };
-  output(std::conditional_t<kExact, float, _Float16>{});
+      for (int g = 0; g < 4; ++g)
+        tile_put<TN, Out>(lds, wm * (TM / WM) + 32 * j + r, wn * (TN / WN) + 32 * i + 8 * g + 4 * h, acc[i][j][4 * g],
+                          acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]);
+  __syncthreads();
+  tile_store<TN, TM, S::kThreads, Out>(lds, p, n0, m0);
 }
 
 // The ranges' sums added in their order.  A workgroup has 32 tokens of a tile and kSpan times 32 of its
@@ -342,18 +278,18 @@ __global__ void __launch_bounds__(256) f8_join_kernel(F8Product p, Parts parts, 
   tile_store<kWide, 32, 256, Out>(lds, p, tile % tiles_n * S::kTn + sn * kWide, tile / tiles_n * S::kTm + 32 * sm);
 }
 
-template <int TN, int TM, int WN, int WM, int STAGES, bool kExact, bool kDirect>
+template <int TN, int TM, int WN, int WM, int STAGES, typename Out, bool kDirect>
 void launch(const F8Product& p, const Parts& parts) {
-  using S = Shape<TN, TM, WN, WM, STAGES, kExact, kDirect>;
+  using S = Shape<TN, TM, WN, WM, STAGES, Out, kDirect>;
   const int tiles_m = (p.m + TM - 1) / TM, tiles_n = (p.n + TN - 1) / TN;
-  f8_many_kernel<TN, TM, WN, WM, STAGES, kExact, kDirect>
+  f8_many_kernel<TN, TM, WN, WM, STAGES, Out, kDirect>
       <<<dim3((unsigned)(tiles_m * tiles_n), (unsigned)parts.n), S::kThreads, S::kLds, current_stream()>>>(p, parts, tiles_m,
                                                                                                        tiles_n);
   check_launch("f8_many_kernel");
   if (parts.n > 1) {
     constexpr int kSpan = TM / 32;
     const dim3 grid((unsigned)(tiles_m * tiles_n * (TN / (32 * kSpan)) * (TM / 32)));
-    f8_join_kernel<Shape<TN, TM, WN, WM, 2, kExact, false>, kSpan, std::conditional_t<kExact, float, _Float16>><<<grid, 256, 0, current_stream()>>>(p, parts, tiles_n);
+    f8_join_kernel<Shape<TN, TM, WN, WM, 2, Out, false>, kSpan, Out><<<grid, 256, 0, current_stream()>>>(p, parts, tiles_n);
     check_launch("f8_join_kernel");
   }
 }
@@ -373,33 +309,34 @@ struct Plan {
   double us;
 };
 
-// us, measured.  A step (a block of K) of a workgroup alone on its CU, and of each of several, takes
-// what kStepCost has, of 256 x 256 1.85, and 7 for its output, less in a round that does not fill the card (1.4 to
-// 1.7 of a third or half of it); 3 us to begin; ranges are written and read
-// again at about 5.5 TB/s and joined by a launch of their own (3 us).  So 509 x 4101 x 11008 takes three
-// ranges of 128-token tiles (44 us; two 53, one 76, 64-token tiles 59), 512 x 4096 x 4096 one of 64
-// (21; two 24, four of 128 26), 1024 x 4096 x 4096 the same (28; of 128 29 to 31), 24 x 11008 x 4096 five of
-// 32 (13; 64-token tiles 16.4), 2048 x 11008 x 4096 tiles of 256 (126; 128 tokens 160) for the
-// weights that whole rounds of them take and others for the rest (109; 4096 x 6000 x 4096 120 -> 110).
+// us, measured.  3 to begin; a step (a block of K) of a workgroup alone on its CU, and of each of several, and what a
+// workgroup takes beside its steps are in kCost; of 256 x 256 3.4 a step and 7, less in a round that does not fill
+// the card (a third of it 2.95 a step, half 3.05); ranges are written and read again at about 5.5 TB/s
+// and joined by a launch of their own (3).  So 509 x 4101 x 11008 takes three ranges of 128-token tiles (69 us; 64-token
+// tiles 77, 32 88), 512 x 4096 x 4096 one of 64 (27.7; two of 128 29.4), 600 x 9000 x 512 the same (12.1; of 128
+// 13.6, of 256 21), 2048 x 4096 x 4096 one of 128 (73; of 64 82), 24 x 11008 x 4096 five of 32 (13; 64-token
+// tiles 18), 4096 x 4096 x 4096 tiles of 256 (118; 128 139), which also take the weights of whole rounds
+// where others take the rest.
+// Costs go by K, as rows' alignment is not the shapes' and the work buffer's size is: rows of an even K
+// that direct loads do not take are cut as those that they do.
 constexpr int kCus = 256;
-struct StepCost {
-  double alone, shared;
+struct Cost {
+  double alone, shared, each;
 };
-// rows of whole 16 bytes and others, codes as they are and widened, 32, 64 and 128 tokens
-constexpr StepCost kStepCost[2][2][3] = {{{{0.4, 0.3}, {0.5, 0.4}, {0.8, 0.72}}, {{0.8, 0.6}, {1.0, 0.8}, {1.6, 1.44}}},
-                                         {{{0.9, 0.55}, {1.08, 0.7}, {1.6, 1.03}}, {{1.15, 0.6}, {1.2, 0.8}, {1.7, 1.5}}}};
+// K in whole 16 bytes and others; 32, 64 and 128 tokens
+constexpr Cost kCost[2][3] = {{{0.54, 0.37, 0.6}, {0.75, 0.57, 0.8}, {1.21, 1.0, 1.3}}, {{0.85, 0.57, 0.6}, {1.1, 0.85, 0.8}, {1.7, 1.72, 1.3}}};
 double rounds_us(int64_t tiles, int64_t blocks) {
   const double part = (double)(tiles % kCus) / kCus;
-  return (double)(tiles / kCus) * (1.85 * (double)blocks + 7) + (part > 0 ? (1.3 + 0.55 * part) * (double)blocks + 7 * part : 0);
+  return (double)(tiles / kCus) * (3.4 * (double)blocks + 7) + (part > 0 ? (2.75 + 0.6 * part) * (double)blocks + 7 * part : 0);
 }
-Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
+Plan plan_of(int64_t m, int64_t n, int64_t k, bool half_out) {
   const int64_t blocks = f8_blocks(k);
   Plan best{};
   for (const int tokens : {32, 64, 128, 256}) {
-    if (tokens == 256 && (exact || k % kF8Block != 0)) continue;
+    if (tokens == 256 && (!half_out || k % kF8Block != 0 || blocks < 2)) continue;
     const int64_t rows = tokens == 256 ? 256 : 128;
     const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + rows - 1) / rows);
-    const StepCost& cost = kStepCost[k % 16 != 0][exact][tokens == 32 ? 0 : tokens == 64 ? 1 : 2];
+    const Cost& cost = kCost[k % 16 != 0][tokens == 32 ? 0 : tokens == 64 ? 1 : 2];
     for (int64_t want = 1; want <= 16 && (want == 1 || (tokens < 256 && tiles * want <= 2 * kCus && blocks >= 4 * want)); ++want) {
       const int64_t each = (blocks + want - 1) / want, parts = (blocks + each - 1) / each;
       const int64_t load = (tiles * parts + kCus - 1) / kCus;
@@ -407,7 +344,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
       if (tokens == 256)
         us += rounds_us(tiles, blocks);
       else
-        us += (double)each * (load == 1 ? cost.alone : cost.shared * (double)load);
+        us += (double)load * ((double)each * (load == 1 ? cost.alone : cost.shared) + cost.each);
       if (parts > 1) us += 3 + (double)parts * (double)m * (double)n * 4 * 2 / 5.5e6;
       if (best.us > 0 && us >= best.us) continue;
       best.us = us;
@@ -420,7 +357,7 @@ Plan plan_of(int64_t m, int64_t n, int64_t k, bool exact) {
     // whole rounds of large tiles and the rest
     const int64_t rounds = tiles / kCus, large = rounds * kCus / ((m + tokens - 1) / tokens) * rows;
     if (tokens == 256 && large > 0 && large < n) {
-      Plan rest = plan_of(m, n - large, k, exact);
+      Plan rest = plan_of(m, n - large, k, half_out);
       rest.us += rounds_us(rounds * kCus, blocks);
       if (rest.us < best.us) {
         best = rest;
@@ -454,19 +391,18 @@ void in_launches(const F8Product& all, F launch) {
 size_t f8_many_work(int64_t m, int64_t n, int64_t k) {
   // for either output type
   size_t most = 0;
-  for (const bool exact : {false, true}) {
-    const Plan plan = plan_of(m, n, k, exact);
+  for (const bool half_out : {false, true}) {
+    const Plan plan = plan_of(m, n, k, half_out);
     if (plan.parts.n > 1) most = std::max(most, (size_t)plan.parts.n * (size_t)plan.parts.range * sizeof(float));
   }
   return most;
 }
 
 void f8_many(const F8Product& all, float* work) {
-  const bool exact = !all.half_out;
   // direct loads take rows in aligned chunks of 16 and 32-bit offsets in a tile
   const bool direct = all.k % 16 == 0 && all.w.row % 16 == 0 && all.x.row % 16 == 0 && aligned(all.w.codes, 16) &&
                       aligned(all.x.codes, 16) && all.w.row < (1 << 24) && all.x.row < (1 << 24);
-  Plan plan = plan_of(all.m, all.n, all.k, exact);
+  Plan plan = plan_of(all.m, all.n, all.k, all.half_out);
   if (plan.large > 0 && direct) {
     F8Product p = all;
     p.n = (int)plan.large;
@@ -487,25 +423,25 @@ void f8_many(const F8Product& all, float* work) {
   plan.parts.sums = work;
   const Parts& parts = plan.parts;
   in_launches(all, [&](const F8Product& p) {
-    const auto run = [&](auto exactly) {
-      constexpr bool kExact = decltype(exactly)::value;
+    const auto run = [&](auto out) {
+      using Out = decltype(out);
       if (plan.tokens == 32)
-        !direct      ? launch<128, 32, 4, 1, 2, kExact, false>(p, parts)
-        : plan.alone ? launch<128, 32, 4, 1, 3, kExact, true>(p, parts)
-                     : launch<128, 32, 4, 1, 2, kExact, true>(p, parts);
+        !direct      ? launch<128, 32, 4, 1, 2, Out, false>(p, parts)
+        : plan.alone ? launch<128, 32, 4, 1, 3, Out, true>(p, parts)
+                     : launch<128, 32, 4, 1, 2, Out, true>(p, parts);
       else if (plan.tokens == 64)
-        !direct      ? launch<128, 64, 4, 1, 2, kExact, false>(p, parts)
-        : plan.alone ? launch<128, 64, 4, 1, 3, kExact, true>(p, parts)
-                     : launch<128, 64, 4, 1, 2, kExact, true>(p, parts);
+        !direct      ? launch<128, 64, 4, 1, 2, Out, false>(p, parts)
+        : plan.alone ? launch<128, 64, 4, 1, 3, Out, true>(p, parts)
+                     : launch<128, 64, 4, 1, 2, Out, true>(p, parts);
       else
-        direct ? launch<128, 128, 2, 2, 2, kExact, true>(p, parts) : launch<128, 128, 2, 2, 2, kExact, false>(p, parts);
+        direct ? launch<128, 128, 2, 2, 2, Out, true>(p, parts) : launch<128, 128, 2, 2, 2, Out, false>(p, parts);
     };
     if (plan.tokens == 256)
       f8_large(p);
-    else if (exact)
-      run(std::true_type{});
+    else if (all.half_out)
+      run(_Float16{});
     else
-      run(std::false_type{});
+      run(float{});
   });
 }
 
