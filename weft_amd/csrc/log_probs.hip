@@ -49,7 +49,7 @@ struct LogProbsArgs {
   long long x_row, tokens_row, token_lp_row, entropy_row, top_ids_row, top_lp_row;  // x in bytes, others in elements
   uint8_t* work;
   long long row0;
-  float scale;
+  float half, scale;  // d = (half x - half max) scale: differences past the largest number come with small scales
   int v, given, top;
   int splits, chunks, chunks_each;
 };
@@ -57,22 +57,24 @@ struct LogProbsArgs {
 struct Stats {
   float m, s, t;  // maximum, sum of e^d, sum of e^d d
 };
+// half x - half m: rounded once, and finite for halves
+__device__ __forceinline__ float below(const LogProbsArgs& a, float x, float m) { return fmaf(x, a.half, -(m * a.half)); }
 
 // below 2^-126 zero: the largest term is 1
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
 
 // Two parts' sums over their common maximum.  A part of nothing has the lowest maximum and
 // sums of zero; the bound on d keeps 0 x infinity out of t.
-__device__ __forceinline__ Stats join(Stats a, Stats b, float scale) {
+__device__ __forceinline__ Stats join(const LogProbsArgs& args, Stats a, Stats b) {
   const float m = fmaxf(a.m, b.m);
-  const float da = fmaxf((a.m - m) * scale, -1e4f), db = fmaxf((b.m - m) * scale, -1e4f);
+  const float da = fmaxf(below(args, a.m, m) * args.scale, -1e4f), db = fmaxf(below(args, b.m, m) * args.scale, -1e4f);
   const float ea = exp_of(da), eb = exp_of(db);
   return {m, a.s * ea + b.s * eb, (a.t + da * a.s) * ea + (b.t + db * b.s) * eb};
 }
-__device__ __forceinline__ Stats join_wave(Stats a, float scale) {
+__device__ __forceinline__ Stats join_wave(const LogProbsArgs& args, Stats a) {
 #pragma unroll
   for (int o = 1; o < kWave; o <<= 1)
-    a = join(a, {__shfl_xor(a.m, o, kWave), __shfl_xor(a.s, o, kWave), __shfl_xor(a.t, o, kWave)}, scale);
+    a = join(args, a, {__shfl_xor(a.m, o, kWave), __shfl_xor(a.s, o, kWave), __shfl_xor(a.t, o, kWave)});
   return a;
 }
 
@@ -227,7 +229,7 @@ __device__ __forceinline__ Row row_of(const Stats& st) { return {st, logf(st.s),
 __device__ __forceinline__ void answer_top(const LogProbsArgs& a, long long row, const Row& r, Key k, int place) {
   a.top_ids[row * a.top_ids_row + place] = k ? index_of(k) : -1;
   a.top_lp[row * a.top_lp_row + place] =
-      k ? (r.none ? -INFINITY : (value_of(k) - r.st.m) * a.scale - r.log_s) : r.st.s + NAN;
+      k ? (r.none ? -INFINITY : below(a, value_of(k), r.st.m) * a.scale - r.log_s) : r.st.s + NAN;
 }
 
 __device__ __forceinline__ Stats* work_stats(const LogProbsArgs& a, long long row) {
@@ -293,7 +295,7 @@ __device__ __forceinline__ void answer(const LogProbsArgs& a, long long row, con
       g.fetch(a, row);
     }
     if ((uint32_t)g.id >= (uint32_t)a.v) continue;
-    a.token_lp[row * a.token_lp_row + i] = r.none ? -INFINITY : (g.x - r.st.m) * a.scale - r.log_s;
+    a.token_lp[row * a.token_lp_row + i] = r.none ? -INFINITY : below(a, g.x, r.st.m) * a.scale - r.log_s;
   }
   if (a.entropy != nullptr && threadIdx.x == 0) a.entropy[row * a.entropy_row] = r.none ? 0.f : r.log_s - r.st.t / r.st.s;
 }
@@ -344,16 +346,17 @@ __global__ void __launch_bounds__(kMostThreads) log_probs_kernel(LogProbsArgs a)
       if (lane == 0) left[wave].bound = bound;
     }
     const float m = fmaxf(st.m, wave_max(most));
-    const float d0 = fmaxf((st.m - m) * a.scale, -1e4f), e0 = exp_of(d0);
+    const float d0 = fmaxf(below(a, st.m, m) * a.scale, -1e4f), e0 = exp_of(d0);
     st = {m, st.s * e0, (st.t + d0 * st.s) * e0};
-    float t = 0.f;  // sum of e^d d / scale
+    const float m_half = m * a.half;
+    float t = 0.f;  // sum of e^d d / ln 2, which no scale takes past the largest number
 #pragma unroll
     for (int i = 0; i < kHold; ++i) {
-      const float d = x[i] - m, e = __builtin_amdgcn_exp2f(d * log2_scale);
+      const float d2 = fmaf(x[i], a.half, -m_half) * log2_scale, e = __builtin_amdgcn_exp2f(d2);
       st.s += e;
-      t = fmaf(e, fmaxf(d, -3.402823466e38f), t);  // minus infinity counts nothing; NaN stays in e
+      t = fmaf(e, fmaxf(d2, -3.402823466e38f), t);  // minus infinity counts nothing; NaN stays in e
     }
-    st.t = fmaf(t, a.scale, st.t);
+    st.t = fmaf(t, 0.693147180559945309f, st.t);
     if constexpr (kTop) {
       if (c == c0) {
         __syncthreads();  // all waves have a first chunk
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(kMostThreads) log_probs_kernel(LogProbsArgs a)
   else
     __syncthreads();
   st = left[0].st;
-  for (int w = 1; w < waves; ++w) st = join(st, left[w].st, a.scale);
+  for (int w = 1; w < waves; ++w) st = join(a, st, left[w].st);
   // places past the numbers have none
   const int place = !kTop ? a.top : tid < key.n ? key.place : tid;
   if (a.splits == 1) {
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(kThreads) log_probs_join_kernel(LogProbsArgs a
     // at most 64 are left
     if (best.n_pending > kWave) best.take(kWave, lane);
   }
-  st = join_wave(st, a.scale);
+  st = join_wave(a, st);
   const Row r = row_of(st);
   answer<kHalf>(a, a.row0 + row, r, given);
   if (a.top == 0) return;
@@ -528,7 +531,8 @@ hipError_t log_probs(const weft_ggml_tensor* x, const weft_ggml_tensor* tokens, 
     a.top_ids = static_cast<int32_t*>(top_ids->data), a.top_ids_row = (long long)(top_ids->nb[1] / 4);
     a.top_lp = static_cast<float*>(top_lp->data), a.top_lp_row = (long long)(top_lp->nb[1] / 4);
   }
-  a.scale = scale;
+  a.half = scale < 1.f ? 0.5f : 1.f;
+  a.scale = scale / a.half;
   a.v = (int)v;
   a.given = (int)given;
   a.top = (int)top;
