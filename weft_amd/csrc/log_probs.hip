@@ -459,17 +459,21 @@ __global__ void __launch_bounds__(kThreads) log_probs_join_kernel(LogProbsArgs a
 // lanes' maxima are a poor bound (300 rows of 2048 to 64: 20.8, of four waves 8.2; 3000 of 2000 to 20 11.3 and 20.5), of 16 for few rows that fit one chunk
 // (256 rows of 32000: 13.2, in ranges of four waves 15.8), else of four in ranges until there are 1024
 // of them (48 rows of 131072: 17.0, of 16 waves 18.0; one row 12.8 and 15.1); 64 ranges a row at
-// most, a list a lane of the join.  Of the shape alone, as the work buffer's size is.
+// most, a list a lane of the join.  A row that begins `late` values behind an aligned place may have a chunk more
+// and is cut as that many are: with the aligned row's ranges, of two chunks each, half of them would be
+// empty.  The work buffer's size is for either, of the shape alone.
 struct Plan {
-  int threads, splits;
+  int threads, chunks, splits;
   size_t row_bytes;  // of the work buffer
   int64_t rows;      // a launch
 };
 int64_t chunks_of(int64_t v, int threads) { return (v + (int64_t)threads * kHold - 1) / (threads * kHold); }
-Plan plan_of(int64_t v, int64_t rows, int64_t top) {
+Plan plan_of(int64_t v, int64_t rows, int64_t top, int64_t late) {
   Plan p{};
+  v += late;
   p.threads = v <= kWave * kHold && top <= 32 ? kWave : v <= kMostThreads * kHold && v > kThreads * kHold && rows <= 512 ? kMostThreads : kThreads;
   const int64_t chunks = chunks_of(v, p.threads);
+  p.chunks = (int)chunks;
   const int64_t want = std::max<int64_t>(1, std::min<int64_t>({1024 / std::max<int64_t>(rows, 1), chunks, kWave}));
   const int64_t each = (chunks + want - 1) / want;
   p.splits = (int)((chunks + each - 1) / each);
@@ -477,6 +481,12 @@ Plan plan_of(int64_t v, int64_t rows, int64_t top) {
   // a launch has fewer than 2^32 threads
   p.rows = std::max<int64_t>(1, ((int64_t)1 << 31) / kMostThreads / p.splits);
   return p;
+}
+// values that a row begins behind an aligned place, at most
+int64_t most_late(const weft_ggml_tensor* x) { return x->type == WEFT_GGML_TYPE_F16 ? 7 : 3; }
+size_t work_size(const weft_ggml_tensor* x, int64_t top) {
+  const int64_t v = x->ne[0], rows = x->ne[1];
+  return (size_t)rows * std::max(plan_of(v, rows, top, 0).row_bytes, plan_of(v, rows, top, most_late(x)).row_bytes);
 }
 
 hipError_t fail(hipError_t e) {
@@ -515,9 +525,10 @@ hipError_t log_probs(const weft_ggml_tensor* x, const weft_ggml_tensor* tokens, 
     return fail(hipErrorInvalidValue);
   if (rows == 0 || (given == 0 && top == 0 && entropy == nullptr)) return hipSuccess;
   if (x->data == nullptr) return fail(hipErrorInvalidValue);
-  const Plan p = plan_of(v, rows, top);
-  if (wsize < p.row_bytes * (size_t)rows || (p.row_bytes > 0 && (wdata == nullptr || !aligned(wdata, 16))))
-    return fail(hipErrorInvalidValue);
+  const size_t size = work_size(x, top);
+  if (wsize < size || (size > 0 && (wdata == nullptr || !aligned(wdata, 16)))) return fail(hipErrorInvalidValue);
+  const bool even = aligned(x->data, 16) && (rows == 1 || x->nb[1] % 16 == 0);
+  const Plan p = plan_of(v, rows, top, even ? 0 : most_late(x));
 
   LogProbsArgs a{};
   a.x = static_cast<const uint8_t*>(x->data);
@@ -537,9 +548,7 @@ hipError_t log_probs(const weft_ggml_tensor* x, const weft_ggml_tensor* tokens, 
   a.given = (int)given;
   a.top = (int)top;
   a.splits = p.splits;
-  // rows that are not 16-byte aligned begin up to seven values later
-  const bool even = aligned(x->data, 16) && (rows == 1 || x->nb[1] % 16 == 0);
-  a.chunks = (int)chunks_of(even ? v : v + 16 / (int64_t)x->nb[0] - 1, p.threads);
+  a.chunks = p.chunks;
   a.chunks_each = (a.chunks + p.splits - 1) / p.splits;
   const hipStream_t st = current_stream();
   const bool half = x->type == WEFT_GGML_TYPE_F16;
@@ -576,7 +585,7 @@ extern "C" size_t weft_ggml_log_probs_work_size(const weft_ggml_tensor* logits, 
   if (logits == nullptr || logits->ne[0] <= 0 || logits->ne[0] > INT32_MAX || logits->ne[1] <= 0 ||
       logits->ne[1] > INT32_MAX || n_top < 0 || n_top > weft::kMost)
     return 0;
-  return weft::plan_of(logits->ne[0], logits->ne[1], n_top).row_bytes * (size_t)logits->ne[1];
+  return weft::work_size(logits, n_top);
 }
 
 extern "C" int weft_ggml_log_probs(const weft_ggml_tensor* logits, const weft_ggml_tensor* tokens,
