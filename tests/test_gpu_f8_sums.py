@@ -163,3 +163,11 @@ def test_a_token_is_the_same_whatever_the_number_of_tokens(hip, n):
     # in the mean far fewer: two roundings of numbers that differ by e differ by a step with the chance e / step, and e is
     # 128 x 2^-24 of a value at most where steps are 2^-11 of it and more: 1.6 %
     assert (a != b).mean() <= 0.016
+
+
+@pytest.mark.parametrize("m,n,k", [(441, 33613, 256), (1874, 8710, 384), (4090, 3900, 512), (4096, 3841, 640), (3850, 4096, 1152)])
+def test_large_tiles_of_few_blocks(hip, m, n, k):
+    """Tiles of 256 load two blocks ahead: from two blocks on, odd and even numbers of them."""
+    hip._lib.launch_log()
+    sharp(Case(hip, m, n, k, F8, F16))
+    assert "f8_large_kernel" in hip._lib.launch_log()

@@ -43,8 +43,6 @@ struct Shape {
   static_assert(kDirect || STAGES == 2, "loads through registers fill the other slot");
 };
 
-// Two waves a SIMD, so that all registers are plain ones: sums in the matrix pipe's own are
-// copied out one by one (two instructions a value).
 // K in `n` ranges of `each` blocks, whose sums go to the work buffer as the lanes have them, a
 // tile after the other; n == 1: straight to the output.
 struct Parts {
@@ -58,6 +56,8 @@ __device__ __forceinline__ long long sum_place(int tile, int wave, int part, int
   return (((long long)tile * S::kWaves + wave) * (S::RN * S::RM) + part) * 4 * kWave + lane;
 }
 
+// Two waves a SIMD, so that all registers are plain ones: sums in the matrix pipe's own are
+// copied out one by one (two instructions a value).  Loads through registers need more than that leaves.
 template <int TN, int TM, int WN, int WM, int STAGES, typename Out, bool kDirect>
 __global__ void __launch_bounds__(64 * WN * WM, kDirect ? 2 : 1) f8_many_kernel(F8Product p, Parts parts, int tiles_m,
                                                                  int tiles_n) {
@@ -294,11 +294,6 @@ void launch(const F8Product& p, const Parts& parts) {
   }
 }
 
-// Steps' places in LDS, of 32 and 64 tokens: three where a workgroup is alone on its CU, so that a step has
-// two others' time to arrive; two where others run beside it, of which a CU then takes three (us, three
-// places and two: 32 x 5120 x 5120 10.2 and 11.3, 64 x 8192 x 8192 16.9 and 20.8; 24 x 11008 x 4096
-// 14.4 and 13.1, 1024 x 4096 x 4096 29.7 and 27.6, 512 x 11008 x 4096 45.6 and 41.6).
-//
 // What a call takes: tiles of 128 weights x 32, 64 or 128 tokens, two workgroups of them a CU, with
 // K in ranges, or of 256 x 256 (16-bit outputs, whole blocks), by the least of these times.
 struct Plan {
@@ -310,8 +305,8 @@ struct Plan {
 };
 
 // us, measured.  3 to begin; a step (a block of K) of a workgroup alone on its CU, and of each of several, and what a
-// workgroup takes beside its steps are in kCost; of 256 x 256 3.4 a step and 7, less in a round that does not fill
-// the card (a third of it 2.95 a step, half 3.05); ranges are written and read again at about 5.5 TB/s
+// workgroup takes beside its steps are in kCost; of 256 x 256 3.4 a step and 7, in a round that does not fill
+// the card 2.75 to 3.35 and 8; ranges are written and read again at about 5.5 TB/s
 // and joined by a launch of their own (3).  So 509 x 4101 x 11008 takes three ranges of 128-token tiles (69 us; 64-token
 // tiles 77, 32 88), 512 x 4096 x 4096 one of 64 (27.7; two of 128 29.4), 600 x 9000 x 512 the same (12.1; of 128
 // 13.6, of 256 21), 2048 x 4096 x 4096 one of 128 (73; of 64 82), 24 x 11008 x 4096 five of 32 (13; 64-token
@@ -327,12 +322,13 @@ struct Cost {
 constexpr Cost kCost[2][3] = {{{0.54, 0.37, 0.6}, {0.75, 0.57, 0.8}, {1.21, 1.0, 1.3}}, {{0.85, 0.57, 0.6}, {1.1, 0.85, 0.8}, {1.7, 1.72, 1.3}}};
 double rounds_us(int64_t tiles, int64_t blocks) {
   const double part = (double)(tiles % kCus) / kCus;
-  return (double)(tiles / kCus) * (3.4 * (double)blocks + 7) + (part > 0 ? (2.75 + 0.6 * part) * (double)blocks + 7 * part : 0);
+  return (double)(tiles / kCus) * (3.4 * (double)blocks + 7) + (part > 0 ? (2.75 + 0.6 * part) * (double)blocks + 8 : 0);
 }
 Plan plan_of(int64_t m, int64_t n, int64_t k, bool half_out) {
   const int64_t blocks = f8_blocks(k);
   Plan best{};
   for (const int tokens : {32, 64, 128, 256}) {
+    // (tiles of 256 load two blocks before they begin)
     if (tokens == 256 && (!half_out || k % kF8Block != 0 || blocks < 2)) continue;
     const int64_t rows = tokens == 256 ? 256 : 128;
     const int64_t tiles = ((m + tokens - 1) / tokens) * ((n + rows - 1) / rows);
@@ -425,6 +421,10 @@ void f8_many(const F8Product& all, float* work) {
   in_launches(all, [&](const F8Product& p) {
     const auto run = [&](auto out) {
       using Out = decltype(out);
+      // Steps' places in LDS, of 32 and 64 tokens: three where a workgroup is alone on its CU, so that a step has
+      // two others' time to arrive; two where others run beside it, of which a CU then takes three (us, three
+      // places and two: 32 x 5120 x 5120 10.9 and 11.8, 64 x 8192 x 8192 19.6 and 21.1; 24 x 11008 x 4096
+      // 14.2 and 13.2, 512 x 11008 x 4096 59.5 and 54.1).
       if (plan.tokens == 32)
         !direct      ? launch<128, 32, 4, 1, 2, Out, false>(p, parts)
         : plan.alone ? launch<128, 32, 4, 1, 3, Out, true>(p, parts)
