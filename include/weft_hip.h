@@ -443,7 +443,8 @@ int weft_ggml_quantize_f8(const weft_ggml_tensor *x, const weft_ggml_tensor *cod
  * x_scales (ceil(K / 128), M; F32); dst (N, M): F32 or F16.  K >= 1; rows lie any whole
  * elements apart.  Outputs are of exact products summed in 32 bits; the order of the sums, and so an
  * output's last bits, depends on the shapes.  A block's sum is multiplied by the product of
- * its two scales, which has to be finite in 32 bits and loses bits below 2^-126.  NaN codes reach their row's outputs and no others.
+ * its two scales, which has to be finite in 32 bits and loses bits below 2^-126.  NaN codes
+ * reach their row's outputs and no others.
  * wdata: weft_ggml_mul_mat_f8_work_size bytes, 16-byte aligned (scratch; its content need
  * not be kept or cleared); the size depends on the shapes and types only. */
 size_t weft_ggml_mul_mat_f8_work_size(const weft_ggml_tensor *w, const weft_ggml_tensor *x);
@@ -467,14 +468,15 @@ typedef struct weft_ggml_head_rope {
  * (same shapes, F32 or F16; a destination may be its source's own memory with its strides).
  * q_weight, k_weight: F32 (D) or NULL (ones; NULL without the norm); factors: F32 (n_rot / 2) or NULL (ones);
  * positions may be NULL if n_rot is 0.  D: at most 256, heads 2^28; heads and tokens lie any
- * whole elements apart.  Angles are reduced in 64 bits; sums have 32. */
+ * whole elements apart.  Angles are reduced in 64 bits; sums of squares have 32, so |x| is up to 1e18. */
 int weft_ggml_head_norm_rope(const weft_ggml_tensor *q, const weft_ggml_tensor *k,
                              const weft_ggml_tensor *q_dst, const weft_ggml_tensor *k_dst,
                              const weft_ggml_tensor *positions, const weft_ggml_head_rope *rope,
                              int32_t normed, float eps, const weft_ggml_tensor *q_weight,
                              const weft_ggml_tensor *k_weight, const weft_ggml_tensor *factors);
 
-/* Of rows of logits (V, rows; F32 or F16), each times scale (> 0: one over a temperature):
+/* Of rows of logits (V, rows; F32 or F16), each times scale (> 0: one over a temperature; past
+ * 2.3e38 differences below 1e-36 keep their order alone):
  * token_lp (n, rows; F32): the log probabilities of tokens (n, rows; I32); an id outside
  * [0, V) leaves its output as it was;
  * entropy (rows; F32), in nats;
@@ -485,7 +487,7 @@ int weft_ggml_head_norm_rope(const weft_ggml_tensor *q, const weft_ggml_tensor *
  * of minus infinity and entropy 0.  NaN or plus infinity makes its row's log
  * probabilities and entropy NaN; NaN is no alternative (id -1 where no other is left).
  * wdata: weft_ggml_log_probs_work_size(logits, A) bytes, 16-byte aligned (scratch); the size
- * depends on the shapes only. */
+ * depends on the shapes and the type only. */
 #define WEFT_GGML_MOST_ALTERNATIVES 64
 size_t weft_ggml_log_probs_work_size(const weft_ggml_tensor *logits, int64_t n_top);
 int weft_ggml_log_probs(const weft_ggml_tensor *logits, const weft_ggml_tensor *tokens,

@@ -9,8 +9,8 @@
 // registers, its place in LDS is loaded again at once, for the step after the next, and loads
 // have a whole step to arrive.
 //
-// Bound by the clock that its power leaves it and the matrix pipe: 8192^3 of random codes takes 883 to 920 us, by the
-// card (1.2 PF; tiles of 128 x 128 1010 to 1060), 4096^3 114 (137).
+// Bound by the matrix pipe (busy 54 % of the time), the VALU (51 %) and waits (31 % of the waves' time): 8192^3 of random
+// codes takes 864 to 920 us, by the card (1.2 to 1.27 PF, at 2.2 GHz; tiles of 128 x 128 1010 to 1060), 4096^3 111 to 118 (137).
 #include "f8_tile.h"
 #include "runtime.h"
 

@@ -346,8 +346,8 @@ hipError_t head_norm_rope(const weft_ggml_tensor* q, const weft_ggml_tensor* k, 
   int g = 8;
   while (g < a.units) g *= 2;
   // A token's heads go to as many waves as there are passes over them, until a launch has 4096 waves,
-  // and past that to waves of five to nine passes: 16384 tokens of 18 passes 140 us in waves of 18, 134 in
-  // six, 145 in four and five; 8192 tokens 86 and 73; 2116 of 16 passes 36 and 22.5.
+  // and past that to as many as leave each five passes or more: 16384 tokens of 18 passes 140 us in one wave, 134 in
+  // three of six, 145 in four of four and five; 8192 tokens 86 in one and 73; 2116 of 16 passes 36 and 22.5.
   const int at_once = kWave / g;
   const int passes = (a.q.n + at_once - 1) / at_once + (a.k.n + at_once - 1) / at_once;
   a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(passes, std::max<int64_t>(4096 / tokens, passes / 5)));
