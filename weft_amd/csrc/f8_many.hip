@@ -15,7 +15,7 @@
 //
 // Bound by the parts of a step, which hardly overlap, and, where K is cut into ranges, by writing and
 // reading their sums: 2048 tokens x 4096 x 4096 take 73 us by 128-token tiles (0.94 PF), 8192^3 to 32 bits 1013 (1.09
-// PF), 24 x 11008 x 4096 10.2 (4.4 TB/s of weights) and 2.5 to 4 for the sums.  Tried without gain: 256 x 128 tiles,
+// PF), 24 x 11008 x 4096 10.2 (4.4 TB/s of weights) and 2.5 to 4 for the sums.  Tried with the instructions that cut, without gain: 256 x 128 tiles,
 // operands read from LDS a step ahead, three and four blocks' places for 128 tokens, priority for the products,
 // workgroups of a CU half a step apart.
 #include <algorithm>
